@@ -109,6 +109,52 @@ inline bool stream_k_layout(int64_t ntiles, int64_t KT, int64_t cus, StreamKLayo
   return true;
 }
 
+// Whether the matrices a [rows, cols_a] (leading dimension lda) and b [rows,
+// cols_b] (ldb) of eb-byte elements share no element: their spans do not meet,
+// or, with equal leading dimensions, b's columns fall between a's in every row
+// (two column ranges of one buffer).  False when neither test tells.
+inline bool matrices_disjoint(uintptr_t a, int64_t lda, uintptr_t b, int64_t ldb, int64_t rows,
+                              int64_t cols_a, int64_t cols_b, int64_t eb) {
+  if (rows <= 0 || cols_a <= 0 || cols_b <= 0) return true;
+  typedef __int128 wide;
+  const wide a0 = a, b0 = b;
+  const wide a1 = a0 + ((wide)(rows - 1) * lda + cols_a) * eb;
+  const wide b1 = b0 + ((wide)(rows - 1) * ldb + cols_b) * eb;
+  if (a1 <= b0 || b1 <= a0) return true;
+  if (lda != ldb || lda <= 0) return false;
+  const wide row = (wide)lda * eb;
+  wide shift = (b0 - a0) % row;
+  if (shift < 0) shift += row;
+  return shift >= (wide)cols_a * eb && shift + (wide)cols_b * eb <= row;
+}
+
+// A stride of a decoder-layer operand, in elements: 2^40 of them keep every byte
+// offset, of up to 2^31 rows in one address, in range of the checks below.
+inline bool stride_ok(int64_t s) { return s >= 0 && s <= (int64_t(1) << 40); }
+
+// Whether rows of `width` contiguous elements at strides s[0 .. dims) with
+// extents n[] (at most 4 dims) share no element: with the strides in order, each
+// steps over everything the smaller ones span.
+inline bool strides_disjoint(const int64_t* n, const int64_t* s, int dims, int64_t width) {
+  typedef __int128 wide;
+  bool used[4] = {false, false, false, false};
+  if (dims < 0 || dims > 4) return false;
+  for (int i = 0; i < dims; ++i)
+    if (n[i] <= 0) return true;
+  wide span = width;
+  for (int k = 0; k < dims; ++k) {
+    int least = -1;
+    for (int i = 0; i < dims; ++i)
+      if (!used[i] && (least < 0 || s[i] < s[least] || (s[i] == s[least] && n[i] < n[least])))
+        least = i;
+    used[least] = true;
+    if (n[least] == 1) continue;
+    if (s[least] < span) return false;
+    span += (wide)(n[least] - 1) * s[least];
+  }
+  return true;
+}
+
 // One entry of the tuning-cache file: "op M N K bm bn bk waves_m waves_n
 // stages split_k reps".  Every field is read as 64-bit and range-checked
 // before it narrows, so an out-of-range value cannot wrap onto a compiled

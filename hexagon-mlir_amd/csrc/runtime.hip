@@ -120,7 +120,7 @@ hxm_status stream_workspace(hipStream_t stream, size_t bytes, void** out, int sl
   int dev = 0;
   if (grown) *grown = false;
   HXM_HIP_TRY(hipGetDevice(&dev));
-  if (slot != kWsMain && slot != kWsSplitK && slot != kWsStreamK)
+  if (slot < kWsMain || slot > kWsLayer)
     return fail(HXM_INVALID_ARG, "invalid-argument: workspace slot %d", slot);
   const bool capturing = stream_capturing(stream);
   const WsKey key(dev, reinterpret_cast<uintptr_t>(stream), slot);

@@ -25,6 +25,7 @@ W_NK, W_PACKED = 0, 1
 OP_W8A16, OP_W8A16_SWIGLU = 16, 17
 STREAM_K = 1024  # HXM_STREAM_K: split_k of a W8A16 config in stream-K form
 IMAGE_GEMM, IMAGE_W8A16 = 0, 1
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 
 
 class HxmError(RuntimeError):
@@ -76,6 +77,12 @@ class Plan(ctypes.Structure):
                 ("tiles", ctypes.c_int64), ("lds_bytes", ctypes.c_int64),
                 ("workspace_bytes", ctypes.c_int64), ("m", ctypes.c_int64),
                 ("n", ctypes.c_int64), ("k", ctypes.c_int64)]
+
+
+class RowNorm(ctypes.Structure):
+    """hxm_row_norm: one norm of hxm_residual_norm_rows."""
+    _fields_ = [("kind", ctypes.c_int32), ("eps", ctypes.c_float), ("gamma", ctypes.c_void_p),
+                ("beta", ctypes.c_void_p)]
 
 
 class ArmQuantiles(ctypes.Structure):
@@ -139,6 +146,9 @@ SIGNATURES = {
     "hxm_rmsnorm_rows": (_st, [_p, _i64, _p, _p, _i64, _i64, _i64, _f32, _i32, _p]),
     "hxm_layernorm_rows": (_st, [_p, _i64, _p, _p, _p, _i64, _p, _p, _i64, _i64, _f32, _i32,
                                  _p]),
+    "hxm_residual_norm_rows": (_st, [_p, _i64, _p, _i64, ctypes.POINTER(RowNorm), _p, _i64, _i64,
+                                     _f32, _f32, ctypes.POINTER(RowNorm), _p, _i64, _p, _i64,
+                                     _i64, _i64, _i32, _p]),
     "hxm_probe_copy": (_st, [_p, _p, _i64, _p]),
     "hxm_probe_read": (_st, [_p, _i64, _p, _p]),
     "hxm_probe_mfma": (_st, [_p, _i64, _p, _i64, _i32, _i32, _i64, _i32, _p, _p]),

@@ -14,8 +14,9 @@ from typing import Optional, Sequence
 
 import torch
 
-from ._lib import (B_KN, B_NK, BF16, F16, F32, I8, I32, IMAGE_GEMM, IMAGE_W8A16, OP_W8A16,
-                   OP_W8A16_SWIGLU, W_NK, W_PACKED, GemmConfig, check, lib)
+from ._lib import (B_KN, B_NK, BF16, F16, F32, I8, I32, IMAGE_GEMM, IMAGE_W8A16, NORM_LAYER,
+                   NORM_NONE, NORM_RMS, OP_W8A16, OP_W8A16_SWIGLU, W_NK, W_PACKED, GemmConfig,
+                   HxmError, RowNorm, check, lib)
 
 _DT = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32,
        torch.int8: I8, torch.int32: I32}
@@ -590,6 +591,90 @@ def layer_norm(x: torch.Tensor, normalized_shape: Sequence[int],
     if st:
         check(st, "hxm_layernorm_rows")
     return (out, mean, rstd) if return_stats else out
+
+
+def _on_current(t: torch.Tensor, name: str) -> None:
+    """The decoder-layer operators launch on the current device."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor (got {t.device})")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+
+
+_NORMS = {"none": NORM_NONE, "rms": NORM_RMS, "layer": NORM_LAYER}
+
+
+def _row_norm(kind: str, weight, bias, eps: float, x: torch.Tensor, name: str):
+    """The hxm_row_norm and the tensors it points to."""
+    import ctypes
+    if kind not in _NORMS:
+        raise ValueError(f"{name} must be one of {sorted(_NORMS)} (got {kind!r})")
+    w = _row_param(weight, x, x.shape[-1], f"{name}_weight")
+    b = _row_param(bias, x, x.shape[-1], f"{name}_bias")
+    n = RowNorm(_NORMS[kind], eps, None if w is None else w.data_ptr(),
+                None if b is None else b.data_ptr())
+    return ctypes.byref(n), (w, b)
+
+
+def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
+                  post_weight: Optional[torch.Tensor] = None,
+                  post_bias: Optional[torch.Tensor] = None, post_eps: float = 1e-6,
+                  pre: str = "rms", pre_weight: Optional[torch.Tensor] = None,
+                  pre_bias: Optional[torch.Tensor] = None, pre_eps: float = 1e-6,
+                  gate: Optional[torch.Tensor] = None, block_scale: float = 1.0,
+                  residual_scale: float = 1.0, out: Optional[torch.Tensor] = None,
+                  normed_out: Optional[torch.Tensor] = None, stream=None):
+    """The norms around a block fused with its gate and the residual
+    (hxm_residual_norm_rows): returns (y, z),
+
+        y = residual_scale * x + block_scale * gate * post(h)
+        z = pre(y)
+
+    for the block's output ``h`` and the residual stream ``x`` (same shape and
+    dtype).  ``post`` / ``pre``: "none", "rms" or "layer", with weights and
+    biases [cols]; ``pre="none"`` gives z = None.  ``gate``: [cols], or
+    [G, cols] with one row for every rows / G consecutive rows.  ``out`` (y)
+    and ``normed_out`` (z) may be ``x`` or ``h`` themselves."""
+    _on_current(h, "h")
+    if h.dtype not in _FLOATS:
+        raise TypeError(f"h must be {' or '.join(str(d) for d in _FLOATS)} (got {h.dtype})")
+    if h.dim() < 1 or h.shape[-1] < 1:
+        raise ValueError(f"h must have a last dimension of one element or more "
+                         f"(got {tuple(h.shape)})")
+    if x.shape != h.shape or x.dtype != h.dtype or x.device != h.device:
+        raise ValueError(f"x must be {h.dtype} {tuple(h.shape)} on {h.device} "
+                         f"(got {x.dtype} {tuple(x.shape)} on {x.device})")
+    h2, rows, cols = _rows(h)
+    x2, _, _ = _rows(x)
+    y, y2 = _rows_out(out, h, cols)
+    if pre == "none":
+        if normed_out is not None:
+            raise ValueError("normed_out needs a pre norm")
+        z = z2 = None
+    else:
+        z, z2 = _rows_out(normed_out, h, cols)
+    post_n, keep_post = _row_norm(post, post_weight, post_bias, post_eps, h, "post")
+    pre_n, keep_pre = _row_norm(pre, pre_weight, pre_bias, pre_eps, h, "pre")
+    G = 0
+    if gate is not None:
+        if gate.dtype != h.dtype or gate.device != h.device:
+            raise ValueError(f"gate must be {h.dtype} on {h.device} "
+                             f"(got {gate.dtype} on {gate.device})")
+        g2 = gate.view(1, -1) if gate.dim() == 1 else gate
+        if g2.dim() != 2 or g2.shape[1] != cols or g2.shape[0] < 1 or rows % g2.shape[0]:
+            raise ValueError(f"gate must be [{cols}] or [G, {cols}] with G dividing {rows} rows "
+                             f"(got {tuple(gate.shape)})")
+        gate = g2 if g2.stride(1) == 1 else g2.contiguous()
+        G = gate.shape[0]
+    st = lib.hxm_residual_norm_rows(
+        h2.data_ptr(), _ld(h2), x2.data_ptr(), _ld(x2), post_n,
+        gate.data_ptr() if G else None, _ld(gate) if G else 0, G, block_scale, residual_scale,
+        pre_n, y2.data_ptr(), _ld(y2), None if z2 is None else z2.data_ptr(),
+        0 if z2 is None else _ld(z2), rows, cols, _code(h), _stream(stream))
+    if st:
+        check(st, "hxm_residual_norm_rows")
+    return y, z
 
 
 def tune_gemm(A: torch.Tensor, B_nk: torch.Tensor, out: torch.Tensor, *, reps: int = 5,

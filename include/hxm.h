@@ -1,7 +1,8 @@
 /*
  * hxm.h - C ABI of the MI355X (gfx950) hot path: MFMA matmuls with resident
  * (pre-packed) weights, W8A16 skinny GEMM/GEMV, single-pass row reductions
- * (softmax / RMSNorm / LayerNorm) and the measured tile search.
+ * (softmax / RMSNorm / LayerNorm), the operators of a decoder layer around
+ * them, and the measured tile search.
  *
  * Boundary rules (every entry point):
  *   - plain pointers, sizes and leading dimensions (in ELEMENTS); no torch or
@@ -18,11 +19,11 @@
  *     buffer would exceed its stated limit, or would have to grow while the
  *     stream is capturing a HIP graph).  There is no silent fallback: a
  *     refused call computes nothing.
- *   - HIP graphs: the compute entries (matmul, GEMM, GEMV, row ops) may be
- *     captured; the tuners, the resident-weight cache and hxm_release_cache
+ *   - HIP graphs: the compute entries (matmul, GEMM, GEMV, row ops, the
+ *     decoder-layer operators) may be captured; the tuners, the resident-weight cache and hxm_release_cache
  *     allocate or synchronise and may not.  A compute entry that uses the
- *     per-stream workspace (f32 operands, a [K,N] B, a K split) needs it
- *     already large enough: one call of the shape on the stream before the
+ *     per-stream workspace (f32 operands, a [K,N] B, a K split, paged
+ *     attention, adapters) needs it already large enough: one call of the shape on the stream before the
  *     capture grows it (it is kept until hxm_release_cache, also past a later
  *     growth once a graph has captured it).  Such a graph holds the workspace
  *     of the stream it was captured on: it must not run at the same time as
@@ -483,6 +484,48 @@ hxm_status hxm_layernorm_rows(const void* x, int64_t ldx, const void* gamma,
                               float* mean_out, float* rstd_out, int64_t rows,
                               int64_t cols, float eps, int32_t dtype,
                               void* stream);
+
+/* ---- decoder-layer operators ---------------------------------------------
+ * What a decoder layer needs around its projections and its FFN block: the
+ * norms on both sides of a block with the residual add between them, rotary
+ * positions with the paged key-value cache, attention of one new token per
+ * sequence over that cache, and low-rank adapters beside a projection.  They
+ * have no counterpart in the reference, which stops at the single linalg ops;
+ * they continue its row reductions and its int8 matmuls.  All are for
+ * inference (no backward pass). */
+
+/* Norm of a row: kind HXM_NORM_NONE (the row itself), HXM_NORM_RMS
+ * (v * rsqrt(mean(v^2) + eps)) or HXM_NORM_LAYER ((v - mean) * rsqrt(var + eps),
+ * biased variance), then * gamma + beta (each [cols] of the rows' dtype, or
+ * NULL for 1 / 0; both must be NULL with HXM_NORM_NONE). */
+typedef enum hxm_norm_kind { HXM_NORM_NONE = 0, HXM_NORM_RMS = 1, HXM_NORM_LAYER = 2 } hxm_norm_kind;
+typedef struct hxm_row_norm {
+  int32_t kind;
+  float eps; /* >= 0 */
+  const void* gamma;
+  const void* beta;
+} hxm_row_norm;
+
+/* The norms before and after a block, fused with its gate and the residual:
+ *   y[r,:] = residual_scale * x[r,:] + block_scale * gate[r / (rows/gate_rows),:]
+ *                                                  * post(h[r,:])
+ *   z[r,:] = pre(y[r,:])
+ * h: the block's output, x: the residual stream, y: the stream after the
+ * block, z: the next block's input.  Everything is fp32 inside; y and z are
+ * each rounded once, z from the unrounded y.  dtype F16, BF16 or F32, one for
+ * all tensors.  gate [gate_rows, cols] (ldg) is NULL with gate_rows 0 (= 1),
+ * or has one row for each rows/gate_rows consecutive rows (1: one gate per
+ * channel; rows: one per row); rows must be a multiple of gate_rows.  With
+ * pre->kind HXM_NORM_NONE, z is not computed (z NULL).  y or z may be h or x
+ * itself (same pointer and ld); any other overlap of an output with h, x or
+ * the other output is refused (gamma, beta and gate must not overlap the
+ * outputs either).  rows up to 2^31 - 1. */
+hxm_status hxm_residual_norm_rows(const void* h, int64_t ldh, const void* x, int64_t ldx,
+                                  const hxm_row_norm* post, const void* gate, int64_t ldg,
+                                  int64_t gate_rows, float block_scale, float residual_scale,
+                                  const hxm_row_norm* pre, void* y, int64_t ldy, void* z,
+                                  int64_t ldz, int64_t rows, int64_t cols, int32_t dtype,
+                                  void* stream);
 
 /* ---- ceiling probes (measurement helpers; no counterpart in the reference) --
  * The practical ceiling of the HBM-bound kernels above, measured with the
