@@ -110,6 +110,17 @@ hxm_status pack_f32_operands(const float* A, int64_t lda, _Float16* ai, int64_t 
                              int64_t ldb, _Float16* bi, int64_t N, int64_t K, int64_t kp, bool kn,
                              hipStream_t stream);
 
+// Operands of the decoder-layer operators (rope.hip): a paged cache and
+// [tokens, heads, dim] views; `written` also asks that no two rows share an
+// element.
+hxm_status check_kv_cache(const char* op, const hxm_kv_cache* c, bool written);
+hxm_status check_heads(const char* op, const char* what, const hxm_heads* h, int64_t tokens,
+                       int64_t heads, int64_t dim, bool written);
+// Whether the written view `out` is `in` itself, or shares nothing with it.
+bool heads_same(const hxm_heads* out, const hxm_heads* in, int64_t tokens, int64_t heads);
+bool heads_apart(const hxm_heads* out, int64_t out_heads, const hxm_heads* in, int64_t in_heads,
+                 int64_t tokens, int64_t dim);
+
 // The skinny matmul (gemm_skinny.hip): takes 1 to kSkinnyRowsMax rows and is
 // the default where skinny_default says so (table: the operand dtype, or
 // kSkinnyW8 for f16 A and int8 B; epi: gemm_kernel.h's Epilogue); a caller names

@@ -85,6 +85,20 @@ class RowNorm(ctypes.Structure):
                 ("beta", ctypes.c_void_p)]
 
 
+class KvCache(ctypes.Structure):
+    """hxm_kv_cache: a paged key-value cache."""
+    _fields_ = ([("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
+                + [(n, ctypes.c_int64) for n in (
+                    "pages", "page_size", "heads", "dim", "k_page_stride", "k_head_stride",
+                    "k_token_stride", "v_page_stride", "v_head_stride", "v_token_stride")])
+
+
+class Heads(ctypes.Structure):
+    """hxm_heads: a [tokens, heads, dim] view."""
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
 class ArmQuantiles(ctypes.Structure):
     """hxm_arm_quantiles: one measured arm of a search round."""
     _fields_ = [("q20", ctypes.c_double), ("q50", ctypes.c_double), ("q80", ctypes.c_double)]
@@ -108,6 +122,7 @@ _f32 = ctypes.c_float
 _f64 = ctypes.c_double
 _st = ctypes.c_int  # hxm_status
 _cfgp = ctypes.POINTER(GemmConfig)
+_hp = ctypes.POINTER(Heads)
 
 # name -> (restype, argtypes); the exact list of include/hxm.h.
 SIGNATURES = {
@@ -149,6 +164,8 @@ SIGNATURES = {
     "hxm_residual_norm_rows": (_st, [_p, _i64, _p, _i64, ctypes.POINTER(RowNorm), _p, _i64, _i64,
                                      _f32, _f32, ctypes.POINTER(RowNorm), _p, _i64, _p, _i64,
                                      _i64, _i64, _i32, _p]),
+    "hxm_rope_append": (_st, [_hp, _hp, _i64, _hp, _hp, _p, _p, _i64, _i64, _i64, _i32, _p,
+                              ctypes.POINTER(KvCache), _i64, _i32, _p]),
     "hxm_probe_copy": (_st, [_p, _p, _i64, _p]),
     "hxm_probe_read": (_st, [_p, _i64, _p, _p]),
     "hxm_probe_mfma": (_st, [_p, _i64, _p, _i64, _i32, _i32, _i64, _i32, _p, _p]),

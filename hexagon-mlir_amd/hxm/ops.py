@@ -16,7 +16,7 @@ import torch
 
 from ._lib import (B_KN, B_NK, BF16, F16, F32, I8, I32, IMAGE_GEMM, IMAGE_W8A16, NORM_LAYER,
                    NORM_NONE, NORM_RMS, OP_W8A16, OP_W8A16_SWIGLU, W_NK, W_PACKED, GemmConfig,
-                   HxmError, RowNorm, check, lib)
+                   Heads, HxmError, KvCache, RowNorm, check, lib)
 
 _DT = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32,
        torch.int8: I8, torch.int32: I32}
@@ -675,6 +675,105 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
     if st:
         check(st, "hxm_residual_norm_rows")
     return y, z
+
+
+_HALVES = (torch.float16, torch.bfloat16)
+
+
+def _heads(t: torch.Tensor, like: torch.Tensor, shape, name: str) -> Heads:
+    """The hxm_heads of a [tokens, heads, dim] tensor of like's dtype and device."""
+    if t.shape != shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must be {like.dtype} {tuple(shape)} on {like.device} "
+                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
+    st = t.stride()
+    if st[2] != 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
+    return Heads(t.data_ptr(), st[0], st[1])
+
+
+def _kv_cache(k: torch.Tensor, v: torch.Tensor) -> KvCache:
+    """The hxm_kv_cache of [pages, heads, page_size, dim] tensors of any
+    strides (a cache that keeps tokens before heads is passed transposed)."""
+    _on_current(k, "k_cache")
+    if k.dim() != 4:
+        raise ValueError(f"k_cache must be [pages, heads, page_size, dim] (got {tuple(k.shape)})")
+    if k.dtype not in _HALVES:
+        raise TypeError(f"k_cache must be {' or '.join(str(d) for d in _HALVES)} (got {k.dtype})")
+    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError(f"v_cache must be {k.dtype} {tuple(k.shape)} on {k.device} "
+                         f"(got {v.dtype} {tuple(v.shape)} on {v.device})")
+    pages, heads, page, dim = k.shape
+    ks, vs = k.stride(), v.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError("k_cache and v_cache must have a contiguous last dimension")
+    return KvCache(k.data_ptr(), v.data_ptr(), pages, page, heads, dim, *ks[:3], *vs[:3])
+
+
+def _ints(t: torch.Tensor, shape, like: torch.Tensor, name: str) -> int:
+    """The address of an int32 tensor of this shape, contiguous, on like's device."""
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be torch.int32 (got {t.dtype})")
+    if t.shape != shape or t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {tuple(shape)} on {like.device} "
+                         f"(got {tuple(t.shape)} on {t.device})")
+    return t.data_ptr()
+
+
+def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                positions: Optional[torch.Tensor] = None,
+                cos_sin: Optional[torch.Tensor] = None, *, interleaved: bool = False,
+                q_out: Optional[torch.Tensor] = None, stream=None) -> Optional[torch.Tensor]:
+    """Rotary positions and the append to a paged cache in one launch
+    (hxm_rope_append): returns the rotated q and stores the rotated k and v.
+
+    q [T, Hq, D] (or None), k and v [T, Hkv, D] f16 / bf16, the last dimension
+    contiguous (heads of a fused projection's output are fine); the caches
+    [pages, Hkv, page_size, D], any strides; ``slots`` int32 [T]: page *
+    page_size + offset, all different, -1 for a row that stores nothing.
+    ``positions`` int32 [T] and ``cos_sin`` fp32 [max_pos, rot_dim] (cosines,
+    then sines) rotate the first rot_dim dims, in halves or (``interleaved``)
+    in neighbouring pairs; without cos_sin nothing is rotated.  ``q_out`` may be
+    q."""
+    import ctypes
+    cache = _kv_cache(k_cache, v_cache)
+    if k.dim() != 3:
+        raise ValueError(f"k must be [tokens, heads, dim] (got {tuple(k.shape)})")
+    T = k.shape[0]
+    kv_shape = (T, cache.heads, cache.dim)
+    kh, vh = _heads(k, k_cache, kv_shape, "k"), _heads(v, k_cache, kv_shape, "v")
+    slot_p = _ints(slots, (T,), k_cache, "slots")
+    pos_p = tab_p = None
+    rot = ld = max_pos = 0
+    if cos_sin is not None:
+        if positions is None:
+            raise ValueError("cos_sin needs positions")
+        pos_p = _ints(positions, (T,), k_cache, "positions")
+        _mat(cos_sin, "cos_sin")
+        if cos_sin.dtype != torch.float32 or cos_sin.device != k_cache.device:
+            raise ValueError(f"cos_sin must be torch.float32 on {k_cache.device} "
+                             f"(got {cos_sin.dtype} on {cos_sin.device})")
+        max_pos, rot = cos_sin.shape
+        tab_p, ld = cos_sin.data_ptr(), _ld(cos_sin)
+    qh = oh = None
+    hq = 0
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError(f"q must be [tokens, heads, dim] (got {tuple(q.shape)})")
+        hq = q.shape[1]
+        shape = (T, hq, cache.dim)
+        qh = _heads(q, k_cache, shape, "q")
+        if q_out is None:
+            q_out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        oh = _heads(q_out, k_cache, shape, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    st = lib.hxm_rope_append(qh, oh, hq, kh, vh, pos_p, tab_p, ld, max_pos, rot,
+                             int(interleaved), slot_p, ctypes.byref(cache), T, _DT[k.dtype],
+                             _stream(stream))
+    if st:
+        check(st, "hxm_rope_append")
+    return q_out
 
 
 def tune_gemm(A: torch.Tensor, B_nk: torch.Tensor, out: torch.Tensor, *, reps: int = 5,

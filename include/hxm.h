@@ -527,6 +527,51 @@ hxm_status hxm_residual_norm_rows(const void* h, int64_t ldh, const void* x, int
                                   int64_t ldz, int64_t rows, int64_t cols, int32_t dtype,
                                   void* stream);
 
+/* A paged key-value cache: element d of head h of the token at offset t of
+ * page p lies at p * page_stride + h * head_stride + t * token_stride + d
+ * (elements), for keys and for values.  Either order of heads and tokens
+ * inside a page is a choice of strides.  dim: a multiple of 8, 8 to 256; any
+ * page_size >= 1; pages * page_size < 2^31; no two elements may share an
+ * address. */
+typedef struct hxm_kv_cache {
+  void* k;
+  void* v;
+  int64_t pages, page_size, heads, dim;
+  int64_t k_page_stride, k_head_stride, k_token_stride;
+  int64_t v_page_stride, v_head_stride, v_token_stride;
+} hxm_kv_cache;
+
+/* [tokens, heads, dim] with dim contiguous: an own tensor, or heads of a fused
+ * projection's output. */
+typedef struct hxm_heads {
+  void* data;
+  int64_t token_stride, head_stride; /* elements, >= 0 */
+} hxm_heads;
+
+/* Rotary position embedding of queries and keys, the rotated keys and the
+ * values stored into a paged cache on the way.  For token t at position
+ * p = positions[t], pair j of the first rot_dim dims (x[j], x[j + rot_dim/2];
+ * interleaved != 0: x[2j], x[2j+1]) becomes
+ *   (a cos - b sin, b cos + a sin),  cos = cos_sin[p, j],
+ *                                    sin = cos_sin[p, rot_dim/2 + j];
+ * dims from rot_dim on stay.  fp32 inside, one rounding.  q_out[t] = the
+ * rotated q[t] (q_heads heads; q.data == q_out.data with equal strides is in
+ * place; q_heads 0: keys only); cache row slots[t] = page * page_size + offset
+ * receives the rotated k[t] and v[t].  A slot outside [0, pages * page_size),
+ * -1 by custom, marks padding: it stores nothing (q is rotated all the same).  The slots of
+ * one call must otherwise be distinct (of two tokens in one slot either may
+ * end there, element by element).  A position outside [0, max_pos) makes the
+ * rotated dims of that token NaN.  cos_sin: fp32 [max_pos, rot_dim]
+ * (ld_cos_sin); rot_dim even, 0 to dim (0: an append without rotation,
+ * positions and cos_sin unused).  The cache must
+ * not overlap the other tensors.  dtype F16 or BF16, one for all. */
+hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q_heads,
+                           const hxm_heads* k, const hxm_heads* v, const int32_t* positions,
+                           const float* cos_sin, int64_t ld_cos_sin, int64_t max_pos,
+                           int64_t rot_dim, int32_t interleaved, const int32_t* slots,
+                           const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
+                           void* stream);
+
 /* ---- ceiling probes (measurement helpers; no counterpart in the reference) --
  * The practical ceiling of the HBM-bound kernels above, measured with the
  * same access pattern (16-byte accesses, eight in flight per lane; the copy
