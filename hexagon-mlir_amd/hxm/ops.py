@@ -776,6 +776,46 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     return q_out
 
 
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                    scale: Optional[float] = None, window: int = 0,
+                    out: Optional[torch.Tensor] = None, return_lse: bool = False, stream=None):
+    """Attention of one new token per sequence over a paged cache
+    (hxm_paged_attention): q [B, Hq, D] f16 / bf16 against the caches [pages,
+    Hkv, page_size, D] (any strides; Hq a multiple of Hkv).  ``block_table``
+    int32 [B, table_pages] names each sequence's pages in order, ``seq_lens``
+    int32 [B] its tokens (the new one included; 0: the row gives zeros).
+    ``scale`` defaults to D ** -0.5; ``window`` keeps the last tokens only
+    (0: all).  Returns out, or (out, lse) with the fp32 [B, Hq] logarithm of
+    the softmax's sum."""
+    import ctypes
+    cache = _kv_cache(k_cache, v_cache)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [batch, heads, dim] (got {tuple(q.shape)})")
+    B, hq = q.shape[:2]
+    shape = (B, hq, cache.dim)
+    qh = _heads(q, k_cache, shape, "q")
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    oh = _heads(out, k_cache, shape, "out")
+    _mat(block_table, "block_table")
+    if block_table.dtype != torch.int32:
+        raise TypeError(f"block_table must be torch.int32 (got {block_table.dtype})")
+    if block_table.shape[0] != B or block_table.device != q.device:
+        raise ValueError(f"block_table must have {B} rows on {q.device} "
+                         f"(got {tuple(block_table.shape)} on {block_table.device})")
+    lens_p = _ints(seq_lens, (B,), q, "seq_lens")
+    lse = torch.empty((B, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    st = lib.hxm_paged_attention(qh, oh, hq, ctypes.byref(cache), block_table.data_ptr(),
+                                 _ld(block_table), block_table.shape[1], lens_p, B,
+                                 cache.dim ** -0.5 if scale is None else scale, window,
+                                 None if lse is None else lse.data_ptr(), _DT[q.dtype],
+                                 _stream(stream))
+    if st:
+        check(st, "hxm_paged_attention")
+    return (out, lse) if return_lse else out
+
+
 def tune_gemm(A: torch.Tensor, B_nk: torch.Tensor, out: torch.Tensor, *, reps: int = 5,
               stream=None):
     """Measured tile search on these operands; returns (GemmConfig, report dict).

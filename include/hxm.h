@@ -572,6 +572,29 @@ hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q
                            const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
                            void* stream);
 
+/* Attention of one new token per sequence over a paged cache:
+ *   out[b,h,:] = sum_t softmax_t(scale * q[b,h,:] . K[t,h',:]) V[t,h',:],
+ *   h' = h / (q_heads / cache->heads),
+ * over the tokens t in [max(0, n - window), n) (window 0: all), n =
+ * seq_lens[b]; token t lies at offset t % page_size of page block_table[b,
+ * t / page_size] (block_table int32 [batch, table_pages], row stride
+ * ld_table).  q_heads a multiple of cache->heads.  lse (fp32 [batch, q_heads],
+ * or NULL) receives log(sum_t exp(scale * q . K[t])).  A sequence without
+ * tokens (n <= 0) gives zeros, and -inf in lse.  Entries of the table past a
+ * sequence's last page, and what the cache holds outside its tokens (NaN
+ * included), are never used.  A page number outside [0, pages) among its
+ * tokens, or n beyond table_pages * page_size, makes that sequence's outputs
+ * NaN.  dtype F16 or BF16, one for q, cache and out; scores, the softmax's
+ * maximum and sum and the output's sum are fp32, the probabilities are rounded
+ * to dtype for the product with V.  out may be q itself.  A long cache is split over workgroups and
+ * joined in a fixed order: results do not depend on how the workgroups are
+ * scheduled.  Uses the per-stream workspace. */
+hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
+                               const hxm_kv_cache* cache, const int32_t* block_table,
+                               int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
+                               int64_t batch, float scale, int64_t window, float* lse,
+                               int32_t dtype, void* stream);
+
 /* ---- ceiling probes (measurement helpers; no counterpart in the reference) --
  * The practical ceiling of the HBM-bound kernels above, measured with the
  * same access pattern (16-byte accesses, eight in flight per lane; the copy
