@@ -168,6 +168,8 @@ SIGNATURES = {
                               ctypes.POINTER(KvCache), _i64, _i32, _p]),
     "hxm_paged_attention": (_st, [_hp, _hp, _i64, ctypes.POINTER(KvCache), _p, _i64, _i64, _p,
                                   _i64, _f32, _i64, _p, _i32, _p]),
+    "hxm_lora_add": (_st, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64,
+                           _i64, _i32, _p]),
     "hxm_probe_copy": (_st, [_p, _p, _i64, _p]),
     "hxm_probe_read": (_st, [_p, _i64, _p, _p]),
     "hxm_probe_mfma": (_st, [_p, _i64, _p, _i64, _i32, _i32, _i64, _i32, _p, _p]),

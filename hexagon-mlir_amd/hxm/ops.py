@@ -816,6 +816,48 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return (out, lse) if return_lse else out
 
 
+def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
+             index: torch.Tensor, scale: Optional[torch.Tensor] = None,
+             out: Optional[torch.Tensor] = None, *, stream=None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a projection they share
+    (hxm_lora_add): out[m] = y[m] + scale[a] * (x[m] @ A[a].T) @ B[a].T with
+    a = ``index``[m] (int32 [M]; -1: out[m] = y[m]).
+
+    y [M, N] is the projection's output and x [M, K] its input (f16 or bf16);
+    A [adapters, R, K] and B [adapters, N, R] contiguous, R a multiple of 8 up
+    to 256; scale fp32 [adapters].  ``out`` may be y."""
+    _on_current(y, "y")
+    _mat(y, "y"), _mat(x, "x")
+    _dtype(y, _HALVES, "y")
+    M, N = y.shape
+    K = x.shape[1]
+    for t, name in ((x, "x"), (A, "A"), (B, "B")):
+        if t.dtype != y.dtype or t.device != y.device:
+            raise ValueError(f"{name} must be {y.dtype} on {y.device} (got {t.dtype} on {t.device})")
+    if x.shape[0] != M:
+        raise ValueError(f"x must have {M} rows (got {x.shape[0]})")
+    if A.dim() != 3 or A.shape[2] != K or not A.is_contiguous():
+        raise ValueError(f"A must be contiguous [adapters, R, {K}] (got {tuple(A.shape)})")
+    L, R = A.shape[:2]
+    if B.shape != (L, N, R) or not B.is_contiguous():
+        raise ValueError(f"B must be contiguous {(L, N, R)} (got {tuple(B.shape)})")
+    index_p = _ints(index, (M,), y, "index")
+    if scale is not None:
+        if scale.device != y.device:
+            raise ValueError(f"scale must be on {y.device} (got {scale.device})")
+        scale = _f32_vec(scale, L, "scale")
+    if out is None:
+        out = torch.empty((M, N), dtype=y.dtype, device=y.device)
+    else:
+        _out(out, (M, N), (y.dtype,), y)
+    st = lib.hxm_lora_add(y.data_ptr(), _ld(y), x.data_ptr(), _ld(x), A.data_ptr(), B.data_ptr(),
+                          L, R, index_p, None if scale is None else scale.data_ptr(),
+                          out.data_ptr(), _ld(out), M, N, K, _DT[y.dtype], _stream(stream))
+    if st:
+        check(st, "hxm_lora_add")
+    return out
+
+
 def tune_gemm(A: torch.Tensor, B_nk: torch.Tensor, out: torch.Tensor, *, reps: int = 5,
               stream=None):
     """Measured tile search on these operands; returns (GemmConfig, report dict).

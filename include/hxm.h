@@ -595,6 +595,22 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
                                int64_t batch, float scale, int64_t window, float* lse,
                                int32_t dtype, void* stream);
 
+/* Low-rank adapters of many requests beside a projection they share:
+ *   out[m,:] = y[m,:] + scale[a] * (x[m,:] A[a]^T) B[a]^T,  a = index[m]
+ * y [M,N] the projection's output, x [M,K] its input; A [adapters, R, K] and
+ * B [adapters, N, R] contiguous; scale fp32 [adapters] or NULL (= 1).  index
+ * int32 [M]: -1 (any negative) leaves out[m] = y[m]; an index >= adapters makes
+ * the row NaN.  Rows of one adapter need not be neighbours, but runs of them
+ * are what large calls are fast at.  out may be y itself (same ld); any other
+ * overlap of out with y or x is refused.  x A^T accumulates in fp32 and enters the second
+ * product with 22 bits (f16) or 16 bits (bf16) of precision; one rounding to dtype.
+ * dtype F16 or BF16, one for all; K a multiple of 8, R a multiple of 8 up to
+ * 256.  Uses the per-stream workspace. */
+hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, const void* A,
+                        const void* B, int64_t adapters, int64_t R, const int32_t* index,
+                        const float* scale, void* out, int64_t ldo, int64_t M, int64_t N,
+                        int64_t K, int32_t dtype, void* stream);
+
 /* ---- ceiling probes (measurement helpers; no counterpart in the reference) --
  * The practical ceiling of the HBM-bound kernels above, measured with the
  * same access pattern (16-byte accesses, eight in flight per lane; the copy
