@@ -42,7 +42,7 @@ inline bool tile_rows_addressable(int64_t ld_bytes, int64_t row_bytes) {
 // Workgroup rows a K split of `split` launches: K bytes in slices of whole
 // stages, ceil(stages / split) stages each; the last slice may be short and
 // no slice is empty.  1 for no split or no K.
-inline int64_t ceil_div(int64_t a, int64_t b) {  // a >= 0, b > 0; no overflow
+constexpr int64_t ceil_div(int64_t a, int64_t b) {  // a >= 0, b > 0; no overflow
   return a / b + (a % b != 0);
 }
 inline int32_t k_slices(int64_t k_bytes, int64_t stage_bytes, int32_t split) {
@@ -153,6 +153,35 @@ inline bool strides_disjoint(const int64_t* n, const int64_t* s, int dims, int64
     span += (wide)(n[least] - 1) * s[least];
   }
   return true;
+}
+
+// Division of n < 2^31 by a fixed d in [1, 2^31): with l = ceil(log2 d) and
+// m = ceil(2^(31+l) / d), n / d = (n m) >> (31 + l): m d - 2^(31+l) < d <= 2^l, so
+// the product is off by less than 2^(31+l) / d.  m fits 32 bits (2^(l-1) < d);
+// d = 1 (l = 0) is m = 2^31, a shift by 31.
+struct FastDiv {
+  uint32_t mul, shift;  // (n * mul) >> shift, 64-bit product
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < d) ++l;
+  const uint64_t p = uint64_t(1) << (31 + l);
+  return FastDiv{static_cast<uint32_t>((p + d - 1) / d), 31 + l};
+}
+
+// How paged attention splits its sequences over workgroups.  A sequence spans
+// span tokens, in units of 32 rounded up; with T the sum of all spans in a batch,
+// a piece is at least T * heads / target of them, a multiple of kAttnPieceStep
+// (each of a workgroup's four waves has the same number of steps) and no fewer
+// than kAttnPieceMin.  Pieces of all sequences and heads then number at most
+// target + batch * heads (each sequence rounds up once), and those of sequences
+// of two pieces or more at most 2 * target: such a sequence has fewer than twice
+// span / piece.
+constexpr int64_t kAttnPieceStep = 4, kAttnPieceMin = 8;
+constexpr int64_t attn_piece(int64_t total_units, int64_t heads, int64_t target) {
+  const int64_t want = ceil_div(total_units * heads, target);
+  const int64_t piece = ceil_div(want, kAttnPieceStep) * kAttnPieceStep;
+  return piece < kAttnPieceMin ? kAttnPieceMin : piece;
 }
 
 // One entry of the tuning-cache file: "op M N K bm bn bk waves_m waves_n

@@ -54,12 +54,13 @@ hxm_status require_device(int* device_out);
 // one buffer per stream never races with itself.  Slot 0 holds per-call
 // operand packs and the tuner's reference output; slot 1 the split-K
 // partial planes, so the two never overwrite or reallocate each other.
-constexpr int kWsMain = 0, kWsSplitK = 1, kWsStreamK = 2, kWsLayer = 3;
+constexpr int kWsMain = 0, kWsSplitK = 1, kWsStreamK = 2, kWsLayer = 3, kWsCount = 4;
 // Largest split-K partial-plane buffer (S * M * N int32) a call may ask for;
 // the buffer stays allocated until hxm_release_cache().
 constexpr int64_t kSplitKPlaneBytesMax = int64_t(256) << 20;
 // Slot 2 holds the W8A16 stream-K partial tiles and arrival counters, slot 3 what
-// a decoder-layer operator keeps between its launches.
+// a decoder-layer operator keeps between its launches or workgroups, slot 4 the
+// arrival counters of paged attention (zero between launches).
 // *grown (when given) says whether the buffer was (re)allocated by this call.
 // True while `stream` captures a graph, or when that cannot be read (the null
 // stream during another stream's global-mode capture).

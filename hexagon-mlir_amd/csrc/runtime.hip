@@ -120,7 +120,7 @@ hxm_status stream_workspace(hipStream_t stream, size_t bytes, void** out, int sl
   int dev = 0;
   if (grown) *grown = false;
   HXM_HIP_TRY(hipGetDevice(&dev));
-  if (slot < kWsMain || slot > kWsLayer)
+  if (slot < kWsMain || slot > kWsCount)
     return fail(HXM_INVALID_ARG, "invalid-argument: workspace slot %d", slot);
   const bool capturing = stream_capturing(stream);
   const WsKey key(dev, reinterpret_cast<uintptr_t>(stream), slot);
@@ -161,6 +161,17 @@ hxm_status stream_workspace(hipStream_t stream, size_t bytes, void** out, int sl
       w.ptr = nullptr;
       return fail(HXM_OUT_OF_MEMORY, "out-of-memory: workspace of %zu bytes",
                   grow);
+    }
+    // Counters start at zero, the whole buffer: a later call may use more of it.
+    // (Never in a capture, where nothing grows.)
+    if (slot == kWsCount) {
+      const hipError_t e = hipMemsetAsync(w.ptr, 0, grow, stream);
+      if (e != hipSuccess) {
+        (void)hipFree(w.ptr);
+        w.ptr = nullptr;
+        return fail(HXM_HIP_ERROR, "hip-error: clearing a workspace failed: %s",
+                    hipGetErrorString(e));
+      }
     }
     w.bytes = grow;
     if (grown) *grown = true;
