@@ -5,23 +5,33 @@
 // query heads that shares a key head is the 16-wide side of the MFMAs (padded
 // with zeros), so one read serves the whole group.
 //
-// A wave takes 32 tokens at a time.  With K as the left operand and Q^T as the
-// right one, S^T = K Q^T leaves lane (g, c) = (lane / 16, lane % 16) the scores of
-// head c; the rows of the two 16-token products are assigned so that they are
-// those of tokens 8g .. 8g+7.  That is how O^T = V^T P^T wants P^T as its right
-// operand: the probabilities go from the first product to the second in the
-// registers they are in, and running maximum, sum and output of a head live
-// in the lanes of one column.  V's left operand has tokens along a lane's
-// registers: a lane loads the 8 tokens x dim/16 dims whose transpose it needs
-// (whole rows per 16 lanes) and transposes them in registers with byte permutes.
-// No LDS until the waves of a workgroup are joined.
+// A wave takes 32 tokens at a time, in two steps whose data stays in registers.
+// S^T = K Q^T, K the left operand, leaves lane (g, c) = (lane / 16, lane % 16)
+// scores of head c; the rows of the two 16-token products are assigned so that
+// they are those of tokens 4j + g, j < 8.  O^T = V^T P^T wants exactly those of P^T as its
+// right operand, so the probabilities go from one product to the other in the lane they
+// are in, and running maximum, sum and output of a head live in one column
+// of lanes.
+//
+// Keys and values come in whole rows, 1 KiB of neighbouring bytes an
+// instruction in the order of a page, nontemporal: nothing is read twice.  (Keys
+// loaded in the operand's own layout, 64 bytes of 16 rows an instruction, read
+// every line in two halves, which the caches had to join: 8 x 32768 tokens, 8
+// heads of 128, 98 us and 91 nontemporal, against 88.)  A lane then holds 8
+// tokens x dim / 16 dims of V and transposes them in registers with byte permutes; K
+// becomes the left operand through the wave's own piece of LDS, where row t has its
+// 16-byte chunk q at q ^ t % 16 (of 8 chunks: q ^ t / 2 % 8, two rows to all 64
+// banks), so that neither side meets a bank twice.  The next tile's keys are on their way as soon as this one's are in
+// LDS, its values as soon as this one's are used.
 //
 // The running maximum moves only when a score passes it by more than 2^8 in
 // the exponent's base 2: exp2(s - m) stays far below fp32's limit, and the
-// output is rescaled a few times per sequence and not per tile.  f16
-// probabilities are scaled by 2^7 on the way into the product, so that with
-// those 8 binary orders of headroom they stay below 65504 and the smallest
-// normal one is 2^-21 of the largest.
+// output is rescaled a few times per sequence and not per tile.  The probabilities enter
+// the second product as two 16-bit halves (22 bits of them in f16, 16 in bf16;
+// one half alone added as much to the error as the output's own rounding, and the
+// second costs no time that shows: 98.3 against 98.5 us).  f16 ones are scaled by
+// 2^7 on the way, so that with those 8 binary orders of headroom they stay below
+// 65504 and the smallest normal one is 2^-21 of the largest.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,9 +46,24 @@ namespace {
 constexpr int kTile = 32;       // tokens of a wave's step
 constexpr int kHeads = 16;      // query heads of a workgroup
 constexpr int kWaves = 4;
+constexpr int kUnit = kWaves * kTile;
+constexpr int64_t kMaxTokens = int64_t(1) << 30;  // of a sequence
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;  // of the running maximum, in powers of two
-constexpr int64_t kTarget = 1024;  // workgroups a batch is split into
+
+// Pieces a batch is cut into where it can be, one for each CU: what a workgroup has
+// under way (a tile of each wave) keeps its CU at its share of the memory's rate, fewer
+// pieces are fewer to join, and all run at once.  More at once only starve each
+// other: with three workgroups a CU, 8 x 32768 tokens, the first to end took 31 us and the
+// last 79; 32768 tokens of one sequence, 8 heads of 8, 32 us with 256 pieces, 42 with 768.
+constexpr int kGroups = 256;
+// Where sequences times heads are more than that, kFine times as many pieces level
+// what their lengths differ by (16 x 8192 tokens at most, 32 heads: 150 us with 2, 141 with
+// 3, 143 with 4 and more; 64 x 4096, 8 heads: 81.5, 80.7, 80.7).
+constexpr int kFine = 3;
+// Waves a SIMD, by the registers of a tile and the output: many short sequences
+// hide each other's start.
+constexpr int attn_waves(int dt) { return dt <= 64 ? 4 : dt <= 128 ? 2 : 1; }
 
 struct AttnArgs {
   const void* q;
@@ -86,119 +111,140 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float shfl_xor(float v, int m) { return __shfl_xor(v, m, 64); }
 
-__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
-  // Row totals by DPP, then the four rows'.
-  auto step = [&](auto ctrl) {
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v),
-                                                           decltype(ctrl)::value, 0xF, 0xF, true));
-  };
-  step(std::integral_constant<int, kDppQuadXor1>{});
-  step(std::integral_constant<int, kDppQuadXor2>{});
-  step(std::integral_constant<int, kDppRowHalfMirror>{});
-  step(std::integral_constant<int, kDppRowMirror>{});
-  const int i = static_cast<int>(v);
-  return static_cast<uint32_t>(__builtin_amdgcn_readlane(i, 0)) +
-         static_cast<uint32_t>(__builtin_amdgcn_readlane(i, 16)) +
-         static_cast<uint32_t>(__builtin_amdgcn_readlane(i, 32)) +
-         static_cast<uint32_t>(__builtin_amdgcn_readlane(i, 48));
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, true));
 }
-
-// Sum of v over lanes 0 .. lane.
+__device__ __forceinline__ uint32_t lane_u32(uint32_t v, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+// Sum of v over lanes 0 .. lane: within the 16-lane rows by row_shr 1, 2, 4, 8
+// (zeros come in), then the totals of the rows before.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {
-  auto step = [&](auto ctrl) {  // row_shr by 1, 2, 4, 8; zeros come in
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v),
-                                                           decltype(ctrl)::value, 0xF, 0xF, true));
-  };
-  step(std::integral_constant<int, 0x111>{});
-  step(std::integral_constant<int, 0x112>{});
-  step(std::integral_constant<int, 0x114>{});
-  step(std::integral_constant<int, 0x118>{});
-  const uint32_t r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31),
-                 r2 = __builtin_amdgcn_readlane(v, 47);
-  return v + (lane >= 16 ? r0 : 0u) + (lane >= 32 ? r1 : 0u) + (lane >= 48 ? r2 : 0u);
+  v += dpp_u32<0x111>(v);
+  v += dpp_u32<0x112>(v);
+  v += dpp_u32<0x114>(v);
+  v += dpp_u32<0x118>(v);
+  return v + (lane >= 16 ? lane_u32(v, 15) : 0u) + (lane >= 32 ? lane_u32(v, 31) : 0u) +
+         (lane >= 48 ? lane_u32(v, 47) : 0u);
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+  v += dpp_u32<kDppQuadXor1>(v);
+  v += dpp_u32<kDppQuadXor2>(v);
+  v += dpp_u32<kDppRowHalfMirror>(v);
+  v += dpp_u32<kDppRowMirror>(v);
+  return lane_u32(v, 0) + lane_u32(v, 16) + lane_u32(v, 32) + lane_u32(v, 48);
 }
 
 // A workgroup's piece of the batch.
 struct Piece {
-  int b;             // sequence, -1: none
-  int n, lo;         // its tokens [lo, n)
-  int begin, end;    // the piece's, begin a multiple of 32
-  int pieces, index; // of the sequence, and this one
-  uint32_t slot;     // of its first partial result (pieces > 1)
-  bool over;         // longer than its table row
+  int b;              // sequence, -1: none
+  int n, lo;          // its tokens [lo, n)
+  int begin, end;     // the piece's, begin a multiple of kTile
+  int pieces, index;  // of the sequence's head, and this one
+  uint32_t slot;      // partial slots (of one head) of the sequences before
+  bool over;          // longer than its table row
 };
 
-// Piece number u of the batch, its sequences in order.  Every wave works it out
-// from the lengths (they are on the device: the host cannot), 64 sequences at a
-// time; a batch of 64 or fewer reads them once.
+// Piece u of the batch, its sequences in order.  Every wave works it out from the
+// lengths, 64 sequences at a time: they are on the device, so the host cannot.
+//
+// Lengths count in units of kUnit tokens; a sequence of up to four is one
+// piece, since a join costs about what three units do (1 x 300 tokens, 32 heads: 7.8
+// us whole, 9.2 in two).  Longer ones are cut into equal pieces of at most `size`
+// units: with share = all units / kGroups, the least of share, 5/4, 3/2 and 2
+// shares that gives no more than kGroups pieces; where none does (many sequences), 1 / kFine
+// of a share, but eight units or more.  Then there are at most kFine * kGroups + batch * heads
+// pieces, fewer than 2 * kFine * kGroups of them parts of a sequence: one cut in c pieces
+// has more than (c - 1) * size units, so size * c is less than twice its units.
 __device__ __forceinline__ Piece find_piece(const AttnArgs& a, uint32_t u, int lane) {
-  auto length = [&](int b, int* lo, bool* over) {
-    const int32_t len = b < a.batch ? a.lens[b] : 0;
-    *over = len > a.capacity;
-    const int n = *over ? 0 : max(len, 0);
+  auto tokens = [&](int32_t len, int* lo) {
+    const int n = len > a.capacity ? 0 : max(len, 0);
     *lo = a.window > 0 ? max(0, n - a.window) : 0;
     return n;
   };
-  auto units = [](int n, int lo) {
-    return static_cast<uint32_t>((n - (lo & ~(kTile - 1)) + kTile - 1) / kTile);
+  // Zero past the last sequence; at most 2^23.
+  auto units = [&](int b, int32_t len) {
+    int lo;
+    const int n = tokens(len, &lo);
+    const uint32_t w = static_cast<uint32_t>(n - (lo & ~(kTile - 1)) + kUnit - 1) / kUnit;
+    return b < a.batch ? max(1u, w) : 0u;
   };
-  int lo;
-  bool over;
-  int n = length(lane, &lo, &over);
-  uint32_t w = units(n, lo);
-  uint64_t total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    if (b0 > 0) {
-      int l2;
-      bool o2;
-      const int n2 = length(b0 + lane, &l2, &o2);
-      w = units(n2, l2);
+  auto length = [&](int b) { return b < a.batch ? a.lens[b] : 0; };
+  const int32_t len0 = length(lane);
+  const uint32_t w0 = units(lane, len0);
+  uint64_t total = wave_sum(w0);
+  for (int b = 64; b < a.batch; b += 64) total += wave_sum(units(b + lane, length(b + lane)));
+  // (No sequence has more than 2^23 units: a larger share cuts nothing either.)
+  const uint32_t share = static_cast<uint32_t>(
+      min<uint64_t>((total * a.heads + kGroups - 1) / kGroups, uint64_t(1) << 24));
+  auto cut = [](uint32_t w, uint32_t size) {
+    return w <= 4u ? min(w, 1u) : (w + size - 1) / size;
+  };
+  uint32_t size = max(2u, share);
+  bool fits = false;
+  if (a.batch <= 64)
+    for (uint32_t k = 0; k < 4 && !fits; ++k) {
+      size = max(2u, share + (k < 3 ? k : 4) * share / 4);
+      fits = wave_sum(cut(w0, size)) * a.heads <= static_cast<uint32_t>(kGroups);
     }
-    // 2^26 units a lane: 64 of them do not fit 32 bits.
-    total += wave_sum(w & 0xffffu) + (static_cast<uint64_t>(wave_sum(w >> 16)) << 16);
-  }
-  const uint32_t piece = static_cast<uint32_t>(
-      min(attn_piece(static_cast<int64_t>(total), a.heads, kTarget), int64_t(1) << 30));
+  if (!fits) size = max(8u, (share + kFine - 1) / kFine);
   Piece r{};
   r.b = -1;
-  uint32_t first = 0, slots = 0;  // pieces and partial slots of the sequences before
+  uint32_t first = 0, slots = 0;  // pieces, and partial slots, of the sequences before
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    if (a.batch > 64) n = length(b0 + lane, &lo, &over);
-    w = units(n, lo);
-    const uint32_t c = b0 + lane < a.batch ? max(1u, (w + piece - 1) / piece) : 0u;
-    const uint32_t upto = wave_scan(c, lane);
-    const uint32_t cs = c > 1 ? c : 0u, upto_s = wave_scan(cs, lane);
+    const int32_t len = b0 == 0 ? len0 : length(b0 + lane);
+    const uint32_t w = units(b0 + lane, len);
+    const uint32_t c = cut(w, size), cs = c > 1 ? c : 0u;
+    const uint32_t upto = wave_scan(c, lane), upto_s = wave_scan(cs, lane);
     const uint64_t hit = __ballot(u < first + upto);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      auto at = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, l)); };
+      const int32_t len_l = static_cast<int32_t>(lane_u32(static_cast<uint32_t>(len), l));
+      const uint32_t pieces = lane_u32(c, l);
+      const int step = static_cast<int>((lane_u32(w, l) + pieces - 1) / pieces) * kUnit;
       r.b = b0 + l;
-      r.n = static_cast<int>(at(n)), r.lo = static_cast<int>(at(lo));
-      r.over = at(over) != 0;
-      r.pieces = static_cast<int>(at(c));
-      r.index = static_cast<int>(u - (first + at(upto) - at(c)));
-      r.slot = slots + at(upto_s) - at(cs);
-      r.begin = (r.lo & ~(kTile - 1)) + r.index * static_cast<int>(piece) * kTile;
-      r.end = r.index + 1 < r.pieces ? r.begin + static_cast<int>(piece) * kTile : r.n;
+      r.n = tokens(len_l, &r.lo);
+      r.over = len_l > a.capacity;
+      r.pieces = static_cast<int>(pieces);
+      r.index = static_cast<int>(u - (first + lane_u32(upto, l) - pieces));
+      r.slot = slots + lane_u32(upto_s, l) - lane_u32(cs, l);
+      r.begin = (r.lo & ~(kTile - 1)) + r.index * step;
+      r.end = r.index + 1 < r.pieces ? min(r.n, r.begin + step) : r.n;
       return r;
     }
-    first += __builtin_amdgcn_readlane(upto, 63);
-    slots += __builtin_amdgcn_readlane(upto_s, 63);
+    first += lane_u32(upto, 63);
+    slots += lane_u32(upto_s, 63);
   }
   return r;
 }
 
-// D_FULL: dim == DT, no dims to mask.  P8: page_size a multiple of 8, so that 8
-// aligned tokens share a page.
+// D_FULL: dim == DT, no dims to mask.  P8: page_size a multiple of 8, and 8 rows
+// of a page within 2^31 bytes: the tile's four groups of 8 tokens then have one
+// page each, whose number and address the scalar unit works out.
 template <typename T, int DT, bool D_FULL, bool P8>
-__global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64)
+    __attribute__((amdgpu_waves_per_eu(attn_waves(DT)))) void paged_attention_kernel(AttnArgs a) {
   using F = Frag<T>;
   using V8 = typename F::V;
-  constexpr int KK = DT / 32;         // K steps of the first product
-  constexpr int VW = DT / 32;         // dwords of a token's DT / 16 value dims in a lane
-  constexpr int VE = DT / 16;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int KK = DT / 32;       // K steps of the first product
+  constexpr int VW = DT / 32;       // dwords of a token's value dims in a lane
+  constexpr int VE = DT / 16;       // and dims
+  constexpr int CK = DT / 8;        // 16-byte chunks of a key row
+  constexpr int RI = 64 / CK;       // key rows of a load
+  constexpr int KI = kTile / RI;    // loads of a tile's keys
+  constexpr int PITCH = DT + 4;     // floats of a row of the join
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int g = lane >> 4, c = lane & 15;
+  // Keys of the waves' tiles, and after the last one the waves' outputs.
+  constexpr int kKeyBytes = kTile * DT * 2, kOutBytes = kHeads * PITCH * 4;
+  constexpr int kWaveBytes = kKeyBytes > kOutBytes ? kKeyBytes : kOutBytes;
+  __shared__ __align__(16) uint8_t lds[kWaves * kWaveBytes];
+  __shared__ float sm[kWaves][kHeads], sl[kWaves][kHeads];
+  __shared__ int last;
+
   const int head = blockIdx.x % a.heads;
   const Piece w = find_piece(a, blockIdx.x / a.heads, lane);
   if (w.b < 0) return;
@@ -207,88 +253,136 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
   const int h0 = hk * a.group + tile * kHeads;
   const int D = D_FULL ? DT : a.dim;
   const int b = w.b, n = w.n, lo = w.lo;
-  const int32_t* table = a.table + b * a.ld_table;
 
+  // Q^T: dims 32k + 8g .. of head c, zeros for the heads past the last and the dims
+  // past D.
   V8 qf[KK];
   {
     const T* q = static_cast<const T*>(a.q) + b * a.q_ts + (h0 + min(c, rows - 1)) * a.q_hs;
 #pragma unroll
     for (int k = 0; k < KK; ++k) {
       const int d = k * 32 + g * 8;
-      const bool in = c < rows && (D_FULL || d < D);
       const v4u32_t x = *reinterpret_cast<const any4*>(q + (D_FULL || d < D ? d : 0));
-      qf[k] = __builtin_bit_cast(V8, in ? x : v4u32_t(0u));
+      qf[k] = __builtin_bit_cast(V8, c < rows && (D_FULL || d < D) ? x : v4u32_t(0u));
     }
   }
   const T* kbase = static_cast<const T*>(a.kc) + hk * a.khs;
   const T* vbase = static_cast<const T*>(a.vc) + hk * a.vhs;
-
-  // The tokens whose K and V rows a lane loads: keys base + 8 (c / 4) + 4u + c % 4,
-  // values base + 8g + j.  Those outside [lo, n) are read as others that are
-  // inside, or beside them in their page, and masked below.
-  auto inside = [&](int tok) { return min(max(tok, lo), n - 1); };
+  // The table is constant memory to this kernel: uniform entries are scalar loads.
+  typedef const int32_t __attribute__((address_space(4))) * ConstInts;
+  const ConstInts table =
+      (ConstInts)(reinterpret_cast<uintptr_t>(a.table + static_cast<int64_t>(b) * a.ld_table));
   auto page_of = [&](int tok) {
-    return static_cast<uint32_t>((static_cast<uint64_t>(tok) * a.page_div.mul) >>
-                                 a.page_div.shift);
-  };
-  constexpr int NK = P8 ? 1 : 2, NV = P8 ? 1 : 8;
-  struct Pages {  // page numbers of the lane's key and value tokens
-    int32_t k[NK], v[NV];
-  };
-  auto key_token = [&](int base, int u) {
-    return P8 ? base + 8 * (c >> 2) : base + 8 * (c >> 2) + 4 * u + (c & 3);
-  };
-  auto value_token = [&](int base, int j) { return base + 8 * g + (P8 ? 0 : j); };
-  auto fetch_pages = [&](int base, Pages& p) {
-#pragma unroll
-    for (int u = 0; u < NK; ++u) p.k[u] = table[page_of(inside(key_token(base, u)))];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) p.v[j] = table[page_of(inside(value_token(base, j)))];
-  };
-  // The offset in its page; of an aligned group of 8, that of its first token.
-  auto offset = [&](int tok) {
-    const int t = inside(tok);
-    const int off = t - static_cast<int>(page_of(t) * a.page_size);
-    return P8 ? off & ~7 : off;
-  };
-  auto row = [&](const T* base, int32_t page, int off, int64_t ps, int64_t ts) {
-    const bool good = static_cast<uint32_t>(page) < a.pages;
-    return base + (good ? page : 0) * ps + off * ts;
+    return static_cast<uint32_t>((static_cast<uint64_t>(static_cast<uint32_t>(tok)) *
+                                  a.page_div.mul) >> a.page_div.shift);
   };
 
-  v4u32_t kt[2][KK];
+  // A lane's key rows are tokens RI i + lane / CK (i < KI) in chunk lane % CK, its value
+  // rows tokens 4 j + g (j < 8) in dims VC c (VC = 4 or 8, of each 128).
+  const int krow = lane / CK, kchunk = lane % CK;
+  const int kdim = D_FULL || kchunk * 8 < D ? kchunk * 8 : 0;
+  constexpr int VC = VE < 8 ? VE : 8;
+  v4u32_t kr[KI];
   uint32_t vt[8][VW];
-  auto load_keys = [&](int base, const Pages& p) {
+  auto load_value = [&](int j, const T* r) {  // r: the token's row
+    if constexpr (DT == 64) {
+      const u32x2 x = __builtin_nontemporal_load(
+          reinterpret_cast<const any2*>(r + (D_FULL || VC * c < D ? VC * c : 0)));
+      vt[j][0] = x[0], vt[j][1] = x[1];
+    } else {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int off = offset(key_token(base, u)) + (P8 ? 4 * u + (c & 3) : 0);
-      const T* r = row(kbase, p.k[P8 ? 0 : u], off, a.kps, a.kts);
+      for (int s = 0; s < DT / 128; ++s) {
+        const int d = 128 * s + VC * c;
+        const v4u32_t x =
+            __builtin_nontemporal_load(reinterpret_cast<const any4*>(r + (D_FULL || d < D ? d : 0)));
 #pragma unroll
-      for (int k = 0; k < KK; ++k) {
-        const int d = k * 32 + g * 8;
-        const v4u32_t x = *reinterpret_cast<const any4*>(r + (D_FULL || d < D ? d : 0));
-        kt[u][k] = D_FULL || d < D ? x : v4u32_t(0u);
+        for (int y = 0; y < 4; ++y) vt[j][4 * s + y] = x[y];
       }
     }
   };
-  auto load_values = [&](int base, const Pages& p) {
+  // Where a tile's rows lie: P8, the page of each group of 8 tokens and the
+  // group's offset in it; otherwise nothing, rows are located one by one.  Tokens
+  // outside [lo, n) are read from rows of the nearest group inside (or as the
+  // nearest token), and masked below.
+  struct Where {
+    uint32_t page[P8 ? 4 : 1];
+    int off[P8 ? 4 : 1];
+    bool bad;
+  };
+  auto locate = [&](int base) {
+    Where p{};
+    if constexpr (P8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = min(max(base + 8 * i, lo & ~7), (n - 1) & ~7);
+        const uint32_t k = page_of(t);
+        p.page[i] = static_cast<uint32_t>(table[k]);
+        p.off[i] = t - static_cast<int>(k * a.page_size);
+      }
+    }
+    return p;
+  };
+  auto check = [&](Where& p) {  // page numbers out of range: row 0 is read, the tile poisoned
+    if constexpr (P8) {
+      p.bad = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool good = p.page[i] < a.pages;
+        p.bad |= !good;
+        p.page[i] = good ? p.page[i] : 0u;
+      }
+    }
+  };
+  auto row_of = [&](int tok, const T* base, int64_t ps, int64_t ts, bool* bad) {
+    const int t = min(max(tok, lo), n - 1);
+    const uint32_t k = page_of(t), id = static_cast<uint32_t>(table[k]);
+    const bool good = id < a.pages;
+    *bad |= !good;
+    return base + static_cast<int64_t>(good ? id : 0u) * ps +
+           static_cast<int64_t>(t - static_cast<int>(k * a.page_size)) * ts;
+  };
+  auto load_keys = [&](int base, Where& p) {
+    if constexpr (P8) {
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const int grp = i * RI / 8, in = i * RI % 8;  // the load's group, its first row there
+        const T* r = kbase + static_cast<int64_t>(p.page[grp]) * a.kps +
+                     static_cast<int64_t>(p.off[grp] + in) * a.kts;
+        const int o = krow * static_cast<int>(a.kts) + kdim;
+        kr[i] = __builtin_nontemporal_load(reinterpret_cast<const any4*>(r + o));
+      }
+    } else {
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const T* r = row_of(base + i * RI + krow, kbase, a.kps, a.kts, &bad);
+        kr[i] = __builtin_nontemporal_load(reinterpret_cast<const any4*>(r + kdim));
+      }
+      p.bad = __any(bad);
+    }
+    if (!D_FULL && kchunk * 8 >= D) {
+#pragma unroll
+      for (int i = 0; i < KI; ++i) kr[i] = v4u32_t(0u);
+    }
+  };
+  auto load_values = [&](int base, const Where& p) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int off = offset(value_token(base, j)) + (P8 ? j : 0);
-      const T* r = row(vbase, p.v[P8 ? 0 : j], off, a.vps, a.vts);
-      if constexpr (DT == 64) {
-        const u32x2 x = *reinterpret_cast<const any2*>(r + (D_FULL || 4 * c < D ? 4 * c : 0));
-        vt[j][0] = x[0], vt[j][1] = x[1];
+      if constexpr (P8) {
+        const T* r = vbase + static_cast<int64_t>(p.page[j / 2]) * a.vps +
+                     static_cast<int64_t>(p.off[j / 2] + 4 * (j % 2)) * a.vts;
+        load_value(j, r + g * static_cast<int>(a.vts));
       } else {
-#pragma unroll
-        for (int s = 0; s < DT / 128; ++s) {
-          const int d = 128 * s + 8 * c;
-          const v4u32_t x = *reinterpret_cast<const any4*>(r + (D_FULL || d < D ? d : 0));
-#pragma unroll
-          for (int y = 0; y < 4; ++y) vt[j][4 * s + y] = x[y];
-        }
+        bool bad = false;
+        load_value(j, row_of(base + 4 * j + g, vbase, a.vps, a.vts, &bad));
       }
     }
+  };
+
+  uint8_t* keys = lds + wave * kWaveBytes;  // the wave's key tile
+  auto key_at = [&](int t, int q) {         // chunk q of its row t
+    const int x = DT == 64 ? (t >> 1) & 7 : t & 15;
+    return reinterpret_cast<v4u32_t*>(keys + t * (DT * 2) + ((q ^ x) << 4));
   };
 
   float m = -__builtin_huge_valf(), l = 0.0f;
@@ -297,33 +391,34 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
   for (int e = 0; e < VE; ++e) acc[e] = v4f32(0.0f);
   const float scale2 = a.scale * kLog2e;
 
-  // One tile; more: its successor's keys are loaded as soon as the scores are
-  // made, its values as soon as this tile's are used, into the same registers.
-  Pages here, next;
+  Where here, next;
   auto step = [&](int base, auto more) {
     constexpr bool MORE = decltype(more)::value;
-    // S^T: the scores of head c at tokens base + 8g + 4u + i.
+    const int after = base + kUnit;
+    const bool poisoned = here.bad;
+#pragma unroll
+    for (int i = 0; i < KI; ++i)
+      *key_at(i * RI + krow, kchunk) = kr[i];
+    if constexpr (MORE) {
+      check(next);
+      load_keys(after, next);
+    }
+    // Other lanes' keys: the wave's LDS operations are in order, and stay so.
+    asm volatile("" ::: "memory");
+    // S^T: row 4g + i of product u is token 16u + 4i + g.
+    v4f32 d[2] = {v4f32(0.0f), v4f32(0.0f)};
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const v4u32_t x = *key_at(16 * u + 4 * (c & 3) + (c >> 2), 4 * k + g);
+        d[u] = F::mfma(__builtin_bit_cast(V8, x), qf[k], d[u]);
+      }
+    }
     float s[8];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      v4f32 d = v4f32(0.0f);
-#pragma unroll
-      for (int k = 0; k < KK; ++k) d = F::mfma(__builtin_bit_cast(V8, kt[u][k]), qf[k], d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * u + i] = d[i] * scale2;
-    }
-    // A token on a bad page poisons its sequence (the lanes' keys are all the
-    // tile's tokens).
-    bool bad = false;
-#pragma unroll
-    for (int u = 0; u < NK; ++u) bad |= static_cast<uint32_t>(here.k[u]) >= a.pages;
-    const bool poisoned = __any(bad);
-    const int after = base + kWaves * kTile;
-    if constexpr (MORE) {
-      here = next;
-      load_keys(after, here);
-      fetch_pages(after + kWaves * kTile, next);
-    }
+    for (int j = 0; j < 8; ++j) s[j] = d[j / 4][j % 4] * scale2;
+    asm volatile("" ::: "memory");
     if (poisoned) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] = __builtin_nanf("");
@@ -331,7 +426,7 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
     if (base < lo || base + kTile > n) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int tok = base + 8 * g + j;
+        const int tok = base + 4 * j + g;
         const bool in = tok >= lo && tok < n;
         s[j] = in ? s[j] : -__builtin_huge_valf();
         // 0 * V must be 0 for what lies in the cache there.
@@ -353,12 +448,13 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
       for (int e = 0; e < VE; ++e) acc[e] *= alpha;
     }
     const float ref = (m == -__builtin_huge_valf() ? 0.0f : m) - F::kShift;
-    V8 p;
+    V8 p, rest;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float e = __builtin_amdgcn_exp2f(s[j] - ref);
       l += e;
       p[j] = fromf<T>(e);
+      rest[j] = fromf<T>(e - tof(p[j]));
     }
     // O^T: dims of this lane's transposed 8-token columns.
 #pragma unroll
@@ -369,28 +465,33 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
         col[x] = __builtin_amdgcn_perm(vt[2 * x + 1][e / 2], vt[2 * x][e / 2],
                                        e & 1 ? 0x07060302u : 0x05040100u);
       acc[e] = F::mfma(__builtin_bit_cast(V8, col), p, acc[e]);
+      acc[e] = F::mfma(__builtin_bit_cast(V8, col), rest, acc[e]);
     }
-    if constexpr (MORE) load_values(after, here);
+    if constexpr (MORE) {
+      load_values(after, next);
+      here = next;
+      next = locate(after + kUnit);
+    }
   };
   int base = w.begin + wave * kTile;
   if (base < w.end) {
-    fetch_pages(base, here);
+    here = locate(base);
+    check(here);
     load_keys(base, here);
     load_values(base, here);
-    fetch_pages(base + kWaves * kTile, next);
-    for (; base + kWaves * kTile < w.end; base += kWaves * kTile) step(base, std::true_type{});
+    next = locate(base + kUnit);
+    for (; base + kUnit < w.end; base += kUnit) step(base, std::true_type{});
     step(base, std::false_type{});
   }
 
   // Joins the waves: outputs [wave][head][dim] with their maximum and sum.
-  constexpr int PITCH = DT + 4;
-  __shared__ __align__(16) float so[kWaves][kHeads][PITCH];
-  __shared__ float sm[kWaves][kHeads], sl[kWaves][kHeads];
   l += shfl_xor(l, 16);
   l += shfl_xor(l, 32);
   if (g == 0) sm[wave][c] = m, sl[wave][c] = l;
-  // acc[e][i] is dim VC * (4g + i) + e of head c (of each 128 dims).
-  constexpr int VC = VE < 8 ? VE : 8;
+  auto out_at = [&](int v, int h, int d) {
+    return reinterpret_cast<float*>(lds + v * kWaveBytes) + h * PITCH + d;
+  };
+  // acc[e][i] is dim VC (4g + i) + e of head c (of each 128 dims).
 #pragma unroll
   for (int e = 0; e < VE; e += 4)
 #pragma unroll
@@ -398,7 +499,7 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
       v4f32 x;
 #pragma unroll
       for (int y = 0; y < 4; ++y) x[y] = acc[e + y][i];
-      *reinterpret_cast<v4f32*>(&so[wave][c][(e / 8) * 128 + VC * (4 * g + i) + e % 8]) = x;
+      *reinterpret_cast<v4f32*>(out_at(wave, c, (e / 8) * 128 + VC * (4 * g + i) + e % 8)) = x;
     }
   __syncthreads();
 
@@ -427,9 +528,9 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
   const __amdgpu_buffer_rsrc_t parts = __builtin_amdgcn_make_buffer_rsrc(
       a.parts, static_cast<short>(0), a.parts_bytes, 0x00020000);
   constexpr int kSc1 = 16;
-  const uint32_t slot0 = (w.slot * a.heads + head * static_cast<uint32_t>(w.pieces));
+  const uint32_t slot0 = w.slot * a.heads + head * static_cast<uint32_t>(w.pieces);
   auto part_at = [&](int s, int word) {
-    return (static_cast<uint32_t>(slot0 + s) * static_cast<uint32_t>(slot_floats) +
+    return ((slot0 + static_cast<uint32_t>(s)) * static_cast<uint32_t>(slot_floats) +
             static_cast<uint32_t>(word)) * 4u;
   };
   for (int x = threadIdx.x; x < items; x += kWaves * 64) {
@@ -442,7 +543,7 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
       const float f = __builtin_amdgcn_exp2f(sm[v][h] - finite(M));
-      const v4f32 y = *reinterpret_cast<const v4f32*>(&so[v][h][4 * d]);
+      const v4f32 y = *reinterpret_cast<const v4f32*>(out_at(v, h, 4 * d));
       L = fmaf(f, sl[v][h], L);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
@@ -463,7 +564,6 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
 
   // The workgroup that arrives last joins the pieces, in their order whichever
   // it is, and clears the counter for the next launch.  Nobody waits.
-  __shared__ int last;
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
   if (threadIdx.x == 0) {
     uint32_t* count = a.counts + static_cast<int64_t>(b) * a.heads + head;
@@ -474,11 +574,13 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
   }
   __syncthreads();
   if (!last) return;
-  // NG groups of threads take consecutive shares of the pieces, eight loads in
-  // flight each, and are joined through LDS.
+  // NG groups of threads take consecutive shares of the pieces, sixteen loads in flight
+  // each, and are joined through LDS.
+  constexpr int kThreads = kWaves * 64;
   int NG = 1;
-  while (2 * NG * items <= kWaves * 64 && 2 * NG <= w.pieces) NG *= 2;
-  const int grp = static_cast<int>(threadIdx.x) / min(items, kWaves * 64);
+  while (2 * NG * items <= kThreads && 2 * NG <= w.pieces) NG *= 2;
+  const int width = min(items, kThreads);
+  const int grp = static_cast<int>(threadIdx.x) / width;
   const int s_begin = static_cast<int>(static_cast<int64_t>(w.pieces) * grp / NG);
   const int s_end = static_cast<int>(static_cast<int64_t>(w.pieces) * (grp + 1) / NG);
   struct Joined {
@@ -494,24 +596,23 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
 #pragma unroll
     for (int e = 0; e < 4; ++e) j.o[e] = fmaf(fb, o[e], fa * j.o[e]);
   };
-  Joined* shared = reinterpret_cast<Joined*>(&so[0][0][0]);
-  static_assert(sizeof(Joined) == 32 && sizeof(so) >= kWaves * 64 * sizeof(Joined), "LDS of a join");
-  for (int x = static_cast<int>(threadIdx.x) % min(items, kWaves * 64); x < items && grp < NG;
-       x += kWaves * 64) {
+  Joined* shared = reinterpret_cast<Joined*>(lds);
+  static_assert(sizeof(Joined) == 32 && sizeof(lds) >= kThreads * sizeof(Joined), "LDS of a join");
+  for (int x = static_cast<int>(threadIdx.x) % width; x < items && grp < NG; x += kThreads) {
     const int h = x / d4, d = x - h * d4;
     Joined j{v4f32(0.0f), -__builtin_huge_valf(), 0.0f};
-    for (int s = s_begin; s < s_end; s += 8) {
-      v4u32_t o[8];
-      u32x2 ml[8];
+    for (int s = s_begin; s < s_end; s += 16) {
+      v4u32_t o[16];
+      u32x2 ml[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 16; ++i) {
         const int si = min(s + i, s_end - 1);
         o[i] = __builtin_amdgcn_raw_buffer_load_b128(
             parts, part_at(si, 2 * a.slot_rows + h * a.dim + 4 * d), 0, kSc1);
         ml[i] = __builtin_amdgcn_raw_buffer_load_b64(parts, part_at(si, 2 * h), 0, kSc1);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 16; ++i)
         if (s + i < s_end) {
           const uint32_t mi = ml[i][0], li = ml[i][1];
           merge(j, __builtin_bit_cast(v4f32, o[i]), __builtin_bit_cast(float, mi),
@@ -535,9 +636,17 @@ __global__ __launch_bounds__(kWaves * 64) void paged_attention_kernel(AttnArgs a
 }
 
 template <typename T, int DT>
-hxm_status launch_attention(const AttnArgs& a, int64_t groups, hipStream_t stream) {
+hxm_status launch_attention(const AttnArgs& a, hipStream_t stream) {
+  // Pieces at most, by either rule of find_piece and by what a sequence can have.
+  const int64_t bh = static_cast<int64_t>(a.batch) * a.heads;
+  const int64_t units = ceil_div(a.capacity + kTile, kUnit);
+  const int64_t groups = std::max(std::min<int64_t>(kGroups, bh * (units / 2 + 1)),
+                                  std::min(kFine * kGroups + bh, bh * (units / 8 + 1)));
+  hxm_status st = check_grid("paged attention", groups, kWaves * 64);
+  if (st != HXM_OK) return st;
   const unsigned n = static_cast<unsigned>(groups);
-  const bool full = a.dim == DT, p8 = a.page_size % 8 == 0;
+  const bool full = a.dim == DT;
+  const bool p8 = a.page_size % 8 == 0 && std::max(a.kts, a.vts) <= (int64_t(1) << 24);
   if (full && p8) paged_attention_kernel<T, DT, true, true><<<n, kWaves * 64, 0, stream>>>(a);
   else if (full) paged_attention_kernel<T, DT, true, false><<<n, kWaves * 64, 0, stream>>>(a);
   else if (p8) paged_attention_kernel<T, DT, false, true><<<n, kWaves * 64, 0, stream>>>(a);
@@ -546,10 +655,10 @@ hxm_status launch_attention(const AttnArgs& a, int64_t groups, hipStream_t strea
 }
 
 template <typename T>
-hxm_status launch_attention_dim(const AttnArgs& a, int64_t groups, hipStream_t stream) {
-  if (a.dim <= 64) return launch_attention<T, 64>(a, groups, stream);
-  if (a.dim <= 128) return launch_attention<T, 128>(a, groups, stream);
-  return launch_attention<T, 256>(a, groups, stream);
+hxm_status launch_attention_dim(const AttnArgs& a, hipStream_t stream) {
+  if (a.dim <= 64) return launch_attention<T, 64>(a, stream);
+  if (a.dim <= 128) return launch_attention<T, 128>(a, stream);
+  return launch_attention<T, 256>(a, stream);
 }
 
 }  // namespace
@@ -573,7 +682,9 @@ extern "C" hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* o
                 "invalid-argument: paged_attention batch=%lld, %lld query heads over %lld, "
                 "window=%lld",
                 (long long)batch, (long long)q_heads, (long long)cache->heads, (long long)window);
-  if (q_heads > 65535 || batch > INT32_MAX / 65536)
+  // 2^24 sequences times heads keep every count of pieces in 32 bits.
+  constexpr int64_t kMaxBatchHeads = int64_t(1) << 24;
+  if (q_heads > 65535 || batch > kMaxBatchHeads || batch * q_heads > kMaxBatchHeads)
     return fail(HXM_UNSUPPORTED_SHAPE, "tile-alignment: paged_attention batch=%lld, %lld heads",
                 (long long)batch, (long long)q_heads);
   if ((st = check_heads("paged_attention", "q", q, batch, q_heads, cache->dim, false)) != HXM_OK ||
@@ -600,7 +711,8 @@ extern "C" hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* o
   a.kps = cache->k_page_stride, a.khs = cache->k_head_stride, a.kts = cache->k_token_stride;
   a.vps = cache->v_page_stride, a.vhs = cache->v_head_stride, a.vts = cache->v_token_stride;
   a.table = block_table, a.lens = seq_lens, a.lse = lse;
-  a.ld_table = ld_table, a.capacity = table_pages * cache->page_size;
+  a.ld_table = ld_table;
+  a.capacity = std::min(table_pages * cache->page_size, kMaxTokens);
   a.pages = static_cast<uint32_t>(cache->pages);
   a.page_size = static_cast<uint32_t>(cache->page_size);
   a.page_div = fast_div(a.page_size);
@@ -612,10 +724,10 @@ extern "C" hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* o
   a.dim = static_cast<int>(cache->dim);
   a.window = window > INT32_MAX ? 0 : static_cast<int>(window);
   a.scale = scale;
-  // Partial results of at most 2 * kTarget pieces, 34 MB for the largest heads,
-  // and a counter for each sequence and head, zero between launches.
+  // Partial results of the sequences cut in pieces, and a counter for each
+  // sequence and head, zero between launches.
   a.slot_rows = std::min(a.group, kHeads);
-  const int64_t parts = 2 * kTarget * a.slot_rows * (a.dim + 2) * 4;
+  const int64_t parts = int64_t(2 * kFine * kGroups) * a.slot_rows * (a.dim + 2) * 4;
   const int64_t counts = batch * a.heads * 4;
   void* ws = nullptr;
   hipStream_t s = as_stream(stream);
@@ -624,8 +736,6 @@ extern "C" hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* o
   if ((st = stream_workspace(s, static_cast<size_t>(parts), &ws, kWsLayer)) != HXM_OK) return st;
   a.parts = static_cast<float*>(ws);
   a.parts_bytes = static_cast<int>(parts);
-  const int64_t groups = kTarget + batch * a.heads;
-  if ((st = check_grid("paged attention", groups, kWaves * 64)) != HXM_OK) return st;
-  return dtype == HXM_F16 ? launch_attention_dim<_Float16>(a, groups, s)
-                          : launch_attention_dim<__bf16>(a, groups, s);
+  return dtype == HXM_F16 ? launch_attention_dim<_Float16>(a, s)
+                          : launch_attention_dim<__bf16>(a, s);
 }

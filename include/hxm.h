@@ -583,10 +583,10 @@ hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q
  * tokens (n <= 0) gives zeros, and -inf in lse.  Entries of the table past a
  * sequence's last page, and what the cache holds outside its tokens (NaN
  * included), are never used.  A page number outside [0, pages) among its
- * tokens, or n beyond table_pages * page_size, makes that sequence's outputs
- * NaN.  dtype F16 or BF16, one for q, cache and out; scores, the softmax's
- * maximum and sum and the output's sum are fp32, the probabilities are rounded
- * to dtype for the product with V.  out may be q itself.  A long cache is split over workgroups and
+ * tokens, or n beyond table_pages * page_size or 2^30, makes that sequence's
+ * outputs NaN.  dtype F16 or BF16, one for q, cache and out; scores, the softmax's
+ * maximum and sum and the output's sum are fp32, the probabilities enter the
+ * product with V with 22 bits (f16) or 16 (bf16).  out may be q itself.  A long cache is split over workgroups and
  * joined in a fixed order: results do not depend on how the workgroups are
  * scheduled.  Uses the per-stream workspace. */
 hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
