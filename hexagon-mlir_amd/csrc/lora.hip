@@ -1,22 +1,29 @@
 // Low-rank adapters of many requests beside a projection they share:
 //   out[m] = y[m] + scale[a] * (x[m] A[a]^T) B[a]^T,  a = index[m].
 //
-// Two launches.  The first makes t = x A^T, R values a row, split over K (fp32
-// partial planes in the stream's workspace, added in order by the second); the
-// second makes t B^T and adds it to y in one read and one write of y.  Bound by
-// memory: y twice, x once, and R * (K + N) elements of each adapter in use,
-// against 2 R operations for each element of x and y.
+// The first launch makes t = x A^T, R values a row, split over K (fp32 partial
+// planes in the stream's workspace, added in order); the last makes t B^T and adds it to
+// y in one read and one write of y.  Bound by memory: y twice, x once, and R * (K + N)
+// elements of each adapter in use, against 2 R operations for each element of x and y.
 //
-// Both work on tiles of 16 rows, any order of adapters among them: a tile's
-// MFMAs run once for each adapter it holds, all 16 rows as one operand, and a
-// row keeps the results of its own adapter alone (chosen, not multiplied by
-// zero: what another adapter's weights hold does not reach it).  Few rows of
-// many adapters cost what reading those adapters costs; a long run of one
-// adapter one pass.
+// Both work on tiles of 16 rows, any order of adapters among them: a tile's MFMAs
+// run once for each adapter it holds, all its rows as one operand, and a row
+// keeps the results of its own adapter alone (chosen, not multiplied by zero: what
+// another adapter's weights hold does not reach it).
+//
+// Few rows are a matter of latency and of reading many adapters: each adapter of a
+// tile is a workgroup of the first launch and a wave of the second, every load under
+// way at once.  Many rows mostly share one adapter per tile: there a launch between makes
+// the second operand once, and the last walks the columns with 128 rows a workgroup.
+// One form for both, 16 rows and the adapters of a tile in turn, ran 10.9 us for 48 rows of 16
+// adapters, 4096 -> 4096, R 16, against 9.9; 64.6 for 2048 rows of 4, 4096 -> 11008, R 64, against
+// 59; 43 for 256 rows of 16 against 18.  Of the 59 about 20 are the first launch and 33 the
+// last, whose reads of y alone take 22, its weights from L2 10 and its products 7: they
+// hardly overlap.
 //
 // t enters the second product as two 16-bit halves, t = hi + lo: 22 bits of it
-// in f16, 16 in bf16, where one would round t to the weights' 11 or 8.  f16 rows
-// are scaled by a power of two first, so that no t over- or underflows; it
+// in f16, 16 in bf16, where one would round t to the weights' 11 or 8.  Rows
+// are scaled by a power of two first, so that no t over- or underflows in f16; it
 // comes back in fp32 with the adapter's scale.
 #include <algorithm>
 
@@ -28,8 +35,11 @@ namespace hxm {
 
 namespace {
 
-constexpr int kRows = 16;   // rows of a tile
+constexpr int kRows = 16;   // rows of an MFMA operand
 constexpr int kWaves = 4;
+// Rows from which the form for many is taken (R 16, 4096 -> 4096: 256 rows of 4 adapters 12.2 us
+// with it, 14.0 without; 512 rows of 16 mixed adapters 26.6 and 31).
+constexpr int64_t kManyRows = 256;
 
 struct LoraArgs {
   const void* y;
@@ -37,12 +47,15 @@ struct LoraArgs {
   const void* A;
   const void* B;
   void* out;
-  float* t;  // [splits][M][R]
+  float* t;        // [splits][M][R]
+  void* halves;    // [M][2][R] of the rows' type, and
+  float* factors;  // [M], for many rows
   const int32_t* index;
   const float* scale;
   int64_t ldy, ldx, ldo, K, N;
   int M, R, adapters, splits;
-  int k_per_split;  // a multiple of 32 * kWaves
+  int tiles;        // of rows, of the second launch
+  int k_per_split;  // a multiple of what a workgroup's waves take together
   int n_per_group;  // columns of a workgroup of the second launch
 };
 
@@ -65,177 +78,455 @@ struct Mma<__bf16> {
 
 typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
 
-// The adapter of this lane's row of the tile (lane % 16), -1 past the last row.
-__device__ __forceinline__ int row_adapter(const LoraArgs& a, int m0, int c) {
-  return m0 + c < a.M ? a.index[m0 + c] : -1;
+// The adapter of row m, -1 past the last row.
+__device__ __forceinline__ int row_adapter(const LoraArgs& a, int m) {
+  return m < a.M ? a.index[m] : -1;
 }
 
-// Workgroup (tile, j, split): t of the tile's rows under the adapter of row j,
-// unless an earlier row has the same.  Its waves take 32 of K in turn.
+// 32-wide steps of K whose loads a wave has under way together.
+constexpr int shrink_steps(int rt) { return rt <= 1 ? 8 : rt <= 4 ? 4 : 2; }
+
+// t of 16 rows, RT * 16 ranks, a part of K.  Workgroup (tile, y, ranks and part) takes the
+// tile's adapters y, y + ways, .. in the order of their first rows; its waves
+// take steps of K in turn and are summed in order.
 template <typename T, int RT>
 __global__ __launch_bounds__(kWaves * 64) void lora_shrink_kernel(LoraArgs a) {
   using V = typename Mma<T>::V;
+  constexpr int U = shrink_steps(RT);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-  const int m0 = blockIdx.x * kRows, j = blockIdx.y, split = blockIdx.z;
-  const int mine = row_adapter(a, m0, c);
-  const int id = __builtin_amdgcn_readlane(mine, j);
-  if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.adapters)) return;
-  const uint32_t same = static_cast<uint32_t>(__ballot(mine == id)) & 0xffffu;
-  if (same & ((1u << j) - 1)) return;
-  const bool hit = mine == id;
-
-  const T* x = static_cast<const T*>(a.x) + static_cast<int64_t>(hit ? m0 + c : m0 + j) * a.ldx;
-  const T* A = static_cast<const T*>(a.A) + static_cast<int64_t>(id) * a.R * a.K;
-  v4f32 acc[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) acc[r] = v4f32(0.0f);
-  const int64_t k_end = min(a.K, static_cast<int64_t>(split + 1) * a.k_per_split);
-  for (int64_t k0 = static_cast<int64_t>(split) * a.k_per_split + wave * 32; k0 < k_end;
-       k0 += 32 * kWaves) {
-    const int64_t k = k0 + 8 * g;
-    const bool in = k < a.K;
-    v4u32_t xw = *reinterpret_cast<const any4*>(x + (in ? k : 0));
-    if (!in) xw = v4u32_t(0u);
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int row = min(r * 16 + c, a.R - 1);
-      v4u32_t w = *reinterpret_cast<const any4*>(A + row * a.K + (in ? k : 0));
-      if (!in) w = v4u32_t(0u);
-      acc[r] = Mma<T>::run(__builtin_bit_cast(V, w), __builtin_bit_cast(V, xw), acc[r]);
-    }
-  }
-  // acc[r][i]: rank 16r + 4g + i of row c.
+  const int m0 = blockIdx.x * kRows, ways = gridDim.y;
+  const int split = blockIdx.z % a.splits, r0 = blockIdx.z / a.splits * (RT * 16);
+  const int mine = row_adapter(a, m0 + c);
+  const bool live = static_cast<uint32_t>(mine) < static_cast<uint32_t>(a.adapters);
+  const int64_t k_begin = static_cast<int64_t>(split) * a.k_per_split;
+  const int64_t k_end = min(a.K, k_begin + a.k_per_split);
   __shared__ __align__(16) float sum[kWaves][RT * 16][kRows + 1];
+  int seen = 0;
+  bool dirty = false;
+  for (uint64_t todo = __ballot(live) & 0xffffull; todo; ++seen) {
+    const int row0 = __builtin_ctzll(todo);
+    const int id = __builtin_amdgcn_readlane(mine, row0);
+    const uint64_t same = __ballot(mine == id);
+    todo &= ~same;
+    if (seen % ways != static_cast<int>(blockIdx.y)) continue;
+    // Rows of another adapter are read as row0; their results are not kept.
+    const T* x = static_cast<const T*>(a.x) +
+                 static_cast<int64_t>(m0 + (mine == id ? c : row0)) * a.ldx;
+    const T* A = static_cast<const T*>(a.A) + static_cast<int64_t>(id) * a.R * a.K;
+    v4f32 acc[RT];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+    for (int r = 0; r < RT; ++r) acc[r] = v4f32(0.0f);
+    for (int64_t k0 = k_begin + wave * (32 * U); k0 < k_end; k0 += 32 * U * kWaves) {
+      v4u32_t xv[U], av[U][RT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[wave][16 * r + 4 * g + i][c] = acc[r][i];
-  __syncthreads();
-  for (int e = threadIdx.x; e < kRows * a.R; e += kWaves * 64) {
-    const int row = e / a.R, r = e - row * a.R;
-    if (!((same >> row) & 1)) continue;
-    const float v = (sum[0][r][row] + sum[1][r][row]) + (sum[2][r][row] + sum[3][r][row]);
-    a.t[(static_cast<int64_t>(split) * a.M + m0 + row) * a.R + r] = v;
+      for (int u = 0; u < U; ++u) {
+        const int64_t k = k0 + 32 * u + 8 * g;
+        const int64_t kc = k < k_end ? k : 0;
+        xv[u] = *reinterpret_cast<const any4*>(x + kc);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+          av[u][r] = *reinterpret_cast<const any4*>(
+              A + static_cast<int64_t>(min(r0 + r * 16 + c, a.R - 1)) * a.K + kc);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool in = k0 + 32 * u + 8 * g < k_end;
+        xv[u] = in ? xv[u] : v4u32_t(0u);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          av[u][r] = in ? av[u][r] : v4u32_t(0u);
+          acc[r] = Mma<T>::run(__builtin_bit_cast(V, av[u][r]), __builtin_bit_cast(V, xv[u]),
+                               acc[r]);
+        }
+      }
+    }
+    if (dirty) __syncthreads();
+    dirty = true;
+    // acc[r][i]: rank 16r + 4g + i of row c.
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[wave][16 * r + 4 * g + i][c] = acc[r][i];
+    __syncthreads();
+    const int ranks = min(RT * 16, a.R - r0);
+    for (int e = threadIdx.x; e < kRows * ranks; e += kWaves * 64) {
+      const int row = e / ranks, r = e - row * ranks;
+      if (!((same >> row) & 1)) continue;
+      const float v = (sum[0][r][row] + sum[1][r][row]) + (sum[2][r][row] + sum[3][r][row]);
+      a.t[(static_cast<int64_t>(split) * a.M + m0 + row) * a.R + r0 + r] = v;
+    }
   }
 }
 
-// Workgroup (columns, tile): 32 columns of 16 rows per wave and step.  KS: steps
-// of 32 ranks.
+// t of a row, ranks 32 s + 8 g .. + 8, as two halves scaled by 2^-ex, and the factor
+// that takes the product back: the adapter's scale times 2^ex.
 template <typename T, int KS>
-__global__ __launch_bounds__(kWaves * 64) void lora_expand_kernel(LoraArgs a) {
-  using V = typename Mma<T>::V;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-  const int m0 = blockIdx.y * kRows, m = m0 + c;
-  const int mine = row_adapter(a, m0, c);
-  const bool live = static_cast<uint32_t>(mine) < static_cast<uint32_t>(a.adapters);
-
-  // t of row c, ranks 32 s + 8 g ..+8, as hi + lo.
-  V hi[KS], lo[KS];
-  float factor = 0.0f;
-  {
-    float t[KS][8];
+struct RowFactors {
+  typename Mma<T>::V hi[KS], lo[KS];
+  float factor;
+};
+// For rows m0 + 16 w + c, w < RW.  The planes are added in order, P of all rows' loads
+// under way at once (past the last plane, its own again, which is not added).
+template <typename T, int KS, int RW>
+__device__ __forceinline__ void load_factors(const LoraArgs& a, int m0, const int (&id)[RW],
+                                             const bool (&live)[RW], int g, int c,
+                                             RowFactors<T, KS> (&f)[RW]) {
+  constexpr int P = RW * KS >= 4 ? 1 : 4 / (RW * KS);
+  float t[RW][KS][8];
+#pragma unroll
+  for (int w = 0; w < RW; ++w)
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[w][s][e] = 0.0f;
+  auto inside = [&](int w, int s) { return live[w] && 32 * s + 8 * g < a.R; };
+  if (a.adapters > 0)
+    for (int p0 = 0; p0 < a.splits; p0 += P) {
+      v4f32 v[P][RW][KS][2];
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int w = 0; w < RW; ++w)
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            // A row without an adapter, or ranks past the last, read the plane's start.
+            const int64_t at = static_cast<int64_t>(min(p0 + i, a.splits - 1)) * a.M * a.R +
+                               (inside(w, s) ? static_cast<int64_t>(m0 + 16 * w + c) * a.R +
+                                                   32 * s + 8 * g
+                                             : 0);
+            const v4f32* tp = reinterpret_cast<const v4f32*>(a.t + at);
+            v[i][w][s][0] = tp[0], v[i][w][s][1] = tp[1];
+          }
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if (p0 + i < a.splits)
+#pragma unroll
+          for (int w = 0; w < RW; ++w)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                t[w][s][e] += inside(w, s) ? v[i][w][s][e / 4][e % 4] : 0.0f;
+    }
+#pragma unroll
+  for (int w = 0; w < RW; ++w) {
     float top = 0.0f;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int r = 32 * s + 8 * g;
-      const bool in = live && r < a.R;
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[s][e] = 0.0f;
-      if (in)
-        for (int p = 0; p < a.splits; ++p) {
-          const v4f32* tp = reinterpret_cast<const v4f32*>(
-              a.t + (static_cast<int64_t>(p) * a.M + m) * a.R + r);
-          const v4f32 u = tp[0], w = tp[1];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t[s][e] += u[e], t[s][4 + e] += w[e];
-        }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(t[s][e]));
-    }
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(t[w][s][e]));
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    // Power of two that takes the row's largest |t| to [1/2, 1); 0, infinities
-    // and NaN stay as they are.
+    // 2^-ex takes the row's largest |t| to [1/2, 1); 0, infinities and NaN stay as
+    // they are.
     int ex = 0;
     if (top > 0.0f && top < __builtin_huge_valf()) ex = __builtin_amdgcn_frexp_expf(top);
-    factor = live ? __builtin_amdgcn_ldexpf(a.scale ? a.scale[mine] : 1.0f, ex) : 0.0f;
+    f[w].factor =
+        live[w] ? __builtin_amdgcn_ldexpf(a.scale ? a.scale[id[w]] : 1.0f, ex) : 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_amdgcn_ldexpf(t[s][e], -ex);
-        hi[s][e] = fromf<T>(v);
+        const float v = __builtin_amdgcn_ldexpf(t[w][s][e], -ex);
+        f[w].hi[s][e] = fromf<T>(v);
         // An infinite or NaN hi needs no remainder (it would be NaN).
-        const float rest = v - tof(hi[s][e]);
-        lo[s][e] = fromf<T>(rest == rest ? rest : 0.0f);
+        const float rest = v - tof(f[w].hi[s][e]);
+        f[w].lo[s][e] = fromf<T>(rest == rest ? rest : 0.0f);
       }
   }
+}
 
-  const int n_end = static_cast<int>(
-      min(a.N, static_cast<int64_t>(blockIdx.x + 1) * a.n_per_group));
-  for (int n0 = blockIdx.x * a.n_per_group + wave * 32; n0 < n_end; n0 += 32 * kWaves) {
-    v4f32 acc[2] = {v4f32(0.0f), v4f32(0.0f)};
-    // The tile's adapters, each at its first row.
-    uint64_t todo = __ballot(live) & 0xffffull;
-    while (todo) {
-      const int id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
-      const bool hit = mine == id;
-      todo &= ~__ballot(hit);
-      const T* B = static_cast<const T*>(a.B) + static_cast<int64_t>(id) * a.N * a.R;
+// Many rows: each row's factors made once, for the many workgroups that read them.  16 rows a
+// wave; halves [M][hi, lo][R] and the factors [M].  (Made by each workgroup from the planes they
+// were 67 MB of reads beside y's 90: 2048 rows, 4096 -> 11008, R 64, 9 us of 63; the
+// launch gives 4 of them back.)
+template <typename T, int KS>
+__global__ __launch_bounds__(kWaves * 64) void lora_halves_kernel(LoraArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+  const int m0 = (blockIdx.x * kWaves + wave) * kRows, m = m0 + c;
+  const int id = row_adapter(a, m);
+  const bool live = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.adapters);
+  RowFactors<T, KS> f[1];
+  load_factors<T, KS, 1>(a, m0, {id}, {live}, g, c, f);
+  if (m >= a.M) return;
+  T* halves = static_cast<T*>(a.halves) + static_cast<int64_t>(m) * 2 * a.R;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        v4f32 d = v4f32(0.0f);
-        // Row c of the product is column 8 (c / 4) + 4u + c % 4, so that a lane
-        // ends with 8 neighbouring columns.
-        const int64_t n = min(a.N - 1, static_cast<int64_t>(n0 + 8 * (c >> 2) + 4 * u + (c & 3)));
+  for (int s = 0; s < KS; ++s) {
+    const int r = 32 * s + 8 * g;
+    if (r < a.R) {
+      *reinterpret_cast<typename Mma<T>::V*>(halves + r) = f[0].hi[s];
+      *reinterpret_cast<typename Mma<T>::V*>(halves + a.R + r) = f[0].lo[s];
+    }
+  }
+  if (g == 0) a.factors[m] = f[0].factor;
+}
+// A row's factors as lora_halves_kernel left them (zeros past the last rank).
+template <typename T, int KS>
+__device__ __forceinline__ void load_halves(const LoraArgs& a, int m, int g,
+                                            RowFactors<T, KS>& f) {
+  using V = typename Mma<T>::V;
+  const int row = min(m, a.M - 1);
+  const T* halves = static_cast<const T*>(a.halves) + static_cast<int64_t>(row) * 2 * a.R;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int r = 32 * s + 8 * g;
-          v4u32_t w = *reinterpret_cast<const any4*>(B + n * a.R + (r < a.R ? r : 0));
-          if (r >= a.R) w = v4u32_t(0u);
-          d = Mma<T>::run(__builtin_bit_cast(V, w), hi[s], d);
-          d = Mma<T>::run(__builtin_bit_cast(V, w), lo[s], d);
+  for (int s = 0; s < KS; ++s) {
+    const int r = 32 * s + 8 * g;
+    const V hi = *reinterpret_cast<const V*>(halves + (r < a.R ? r : 0));
+    const V lo = *reinterpret_cast<const V*>(halves + a.R + (r < a.R ? r : 0));
+    f.hi[s] = r < a.R ? hi : V(T(0));
+    f.lo[s] = r < a.R ? lo : V(T(0));
+  }
+  f.factor = a.factors[row];
+}
+
+// Rows r of B (columns of the output) as the left operand of 32 columns: product
+// u, row c is column 8 (c / 4) + 4u + c % 4, so that a lane ends with 8 neighbouring
+// columns of one row.
+template <typename T, int KS>
+__device__ __forceinline__ void load_b(const LoraArgs& a, int id, int n0, int u, int g, int c,
+                                       v4u32_t (&w)[KS]) {
+  const int64_t n = min(a.N - 1, static_cast<int64_t>(n0 + 8 * (c >> 2) + 4 * u + (c & 3)));
+  const T* B = static_cast<const T*>(a.B) + (static_cast<int64_t>(id) * a.N + n) * a.R;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int r = 32 * s + 8 * g;
+    w[s] = *reinterpret_cast<const any4*>(B + (r < a.R ? r : 0));
+    if (r >= a.R) w[s] = v4u32_t(0u);
+  }
+}
+template <typename T, int KS>
+__device__ __forceinline__ v4f32 times_b(const v4u32_t (&w)[KS], const RowFactors<T, KS>& f) {
+  using V = typename Mma<T>::V;
+  v4f32 d = v4f32(0.0f);
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    d = Mma<T>::run(__builtin_bit_cast(V, w[s]), f.hi[s], d);
+    d = Mma<T>::run(__builtin_bit_cast(V, w[s]), f.lo[s], d);
+  }
+  return d;
+}
+// Eight columns n .. of row m: y + factor * d, `left` of them inside.
+template <typename T>
+__device__ __forceinline__ RawVec<T> load_y(const LoraArgs& a, int m, int n, int left) {
+  const T* y = static_cast<const T*>(a.y) + m * a.ldy + n;
+  return left >= 8 ? load_any(y) : load_tail(y, 0, left, T(0));
+}
+template <typename T>
+__device__ __forceinline__ void store_out(const LoraArgs& a, int m, int n, int left, int id,
+                                          RawVec<T> y, v4f32 d0, v4f32 d1, float factor) {
+  if (id < 0 && a.out == a.y) return;
+  if (id >= 0) {
+    const bool live = id < a.adapters;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = e < 4 ? d0[e & 3] : d1[e & 3];
+      y[e] = fromf<T>(live ? fmaf(factor, d, tof(y[e])) : __builtin_nanf(""));
+    }
+  }
+  // Plain stores: the next operator reads them.
+  T* out = static_cast<T*>(a.out) + m * a.ldo + n;
+  if (left >= 8) *reinterpret_cast<AnyVec<T>*>(out) = y;
+  else store_tail(out, 0, left, y);
+}
+
+// Few rows: workgroup (32 columns, 16 rows), wave w the tile's adapters w, w + 4, ..
+// by first row, and their rows; rows without an adapter go to wave 0.
+template <typename T, int KS>
+__global__ __launch_bounds__(kWaves * 64) void lora_expand_few_kernel(LoraArgs a) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int m = blockIdx.y * kRows + c, n0 = blockIdx.x * 32;
+  const int mine = row_adapter(a, m);
+  const bool live = static_cast<uint32_t>(mine) < static_cast<uint32_t>(a.adapters);
+  constexpr int PER = kRows / kWaves;
+  int ids[PER], count = 0, seen = 0;
+  bool here = wave == 0 && !live && m < a.M;
+  for (uint64_t todo = __ballot(live) & 0xffffull; todo; ++seen) {
+    const int id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+    todo &= ~__ballot(mine == id);
+    if (seen % kWaves != wave) continue;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (i == count) ids[i] = id;
+    ++count;
+    here |= mine == id;
+  }
+  if (!__any(here)) return;
+  // As many adapters' weights at once as 64 registers hold.
+  constexpr int BATCH = KS >= 8 ? 1 : KS >= 4 ? 2 : PER;
+  const int n = n0 + 8 * g;
+  const int left = static_cast<int>(min<int64_t>(a.N - n, 8));
+  RawVec<T> y;
+  if (here && left > 0) y = load_y<T>(a, m, n, left);
+  v4f32 acc[2] = {v4f32(0.0f), v4f32(0.0f)};
+  RowFactors<T, KS> f[1];
+#pragma unroll
+  for (int i0 = 0; i0 < PER; i0 += BATCH) {
+    v4u32_t w[BATCH][2][KS];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (i0 + i < count)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) load_b<T, KS>(a, ids[i0 + i], n0, u, g, c, w[i][u]);
+    if (i0 == 0)
+      load_factors<T, KS, 1>(a, blockIdx.y * kRows, {mine}, {live && here}, g, c, f);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (i0 + i < count) {
+        const bool hit = mine == ids[i0 + i];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const v4f32 d = times_b<T, KS>(w[i][u], f[0]);
+          acc[u] = hit ? d : acc[u];
         }
-        acc[u] = hit ? d : acc[u];
       }
-    }
-    if (m >= a.M) continue;
-    const int n = n0 + 8 * g;
-    if (n >= n_end) continue;
-    if (mine < 0 && a.out == a.y) continue;
-    const T* y = static_cast<const T*>(a.y) + m * a.ldy + n;
-    T* out = static_cast<T*>(a.out) + m * a.ldo + n;
-    const int left = n_end - n;
-    RawVec<T> v = left >= 8 ? load_any(y) : load_tail(y, 0, left, T(0));
-    if (mine >= 0) {
+  }
+  if (here && left > 0) store_out<T>(a, m, n, left, mine, y, acc[0], acc[1], f[0].factor);
+}
+
+// Many rows: workgroup (columns, rows), a wave RW * 16 rows and 32 * NB columns at a time,
+// the adapters of its rows one after another; the waves walk the same columns, so
+// that the L1 serves three of four reads of the weights.  The next weights load as
+// soon as the products have used these, the next rows of y as soon as these are
+// stored, into the same registers (a copy from others would wait for the load).
+//
+// Workgroups go to the XCDs in turn: XCD i takes the column groups i, i + 8, .. and
+// walks the rows with each, so that its L2 holds the group's weights.
+template <typename T, int KS, int RW, int NB>
+__global__ __launch_bounds__(kWaves * 64) void lora_expand_kernel(LoraArgs a) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int turn = blockIdx.x / 8;
+  const int m0 = (turn % a.tiles * kWaves + wave) * (kRows * RW);
+  const int64_t n_begin =
+      (turn / a.tiles * 8 + static_cast<int64_t>(blockIdx.x % 8)) * a.n_per_group;
+  constexpr int STEP = 32 * NB;
+  if (n_begin >= a.N || m0 >= a.M) return;
+  const int n_end = static_cast<int>(min(a.N, n_begin + a.n_per_group));
+  int mine[RW];
+  uint64_t all = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = e < 4 ? acc[0][e & 3] : acc[1][e & 3];
-        v[e] = fromf<T>(live ? fmaf(factor, d, tof(v[e])) : __builtin_nanf(""));
+  for (int w = 0; w < RW; ++w) {
+    mine[w] = row_adapter(a, m0 + 16 * w + c);
+    const bool live = static_cast<uint32_t>(mine[w]) < static_cast<uint32_t>(a.adapters);
+    all |= (__ballot(live) & 0xffffull) << (16 * w);
+  }
+  auto first_of = [&](uint64_t todo) {
+    const int row = __builtin_ctzll(todo);
+    int id = __builtin_amdgcn_readlane(mine[0], row & 15);
+    if constexpr (RW == 2) id = row < 16 ? id : __builtin_amdgcn_readlane(mine[1], row & 15);
+    return id;
+  };
+  auto rows_of = [&](int id) {
+    uint64_t r = 0;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) r |= (__ballot(mine[w] == id) & 0xffffull) << (16 * w);
+    return r;
+  };
+  v4u32_t b[NB][2][KS];
+  RawVec<T> y[RW][NB];
+  auto load_weights = [&](int id, int n0) {
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) load_b<T, KS>(a, id, n0 + 32 * k, u, g, c, b[k][u]);
+  };
+  auto left_of = [&](int n0, int k) { return min(8, n_end - (n0 + 32 * k + 8 * g)); };
+  auto load_rows = [&](int n0) {
+#pragma unroll
+    for (int w = 0; w < RW; ++w)
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const int left = left_of(n0, k);
+        if (m0 + 16 * w + c < a.M && left > 0)
+          y[w][k] = load_y<T>(a, m0 + 16 * w + c, n0 + 32 * k + 8 * g, left);
       }
+  };
+  int n0 = static_cast<int>(n_begin), id = -1;
+  load_rows(n0);
+  if (all) {
+    id = first_of(all);
+    load_weights(id, n0);
+  }
+  RowFactors<T, KS> f[RW];
+#pragma unroll
+  for (int w = 0; w < RW; ++w) load_halves<T, KS>(a, m0 + 16 * w + c, g, f[w]);
+  for (; n0 < n_end; n0 += STEP) {
+    v4f32 acc[RW][NB][2];
+#pragma unroll
+    for (int w = 0; w < RW; ++w)
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) acc[w][k][u] = v4f32(0.0f);
+    for (uint64_t todo = all; todo;) {
+      const int now = id;
+      todo &= ~rows_of(now);
+#pragma unroll
+      for (int w = 0; w < RW; ++w) {
+        const bool hit = mine[w] == now;
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const v4f32 d = times_b<T, KS>(b[k][u], f[w]);
+            acc[w][k][u] = hit ? d : acc[w][k][u];
+          }
+      }
+      // The next adapter of these columns, or the first of the next ones (past the
+      // last, of the last column).
+      id = first_of(todo ? todo : all);
+      load_weights(id, todo ? n0 : n0 + STEP);
     }
-    if (left >= 8) store_any(out, v);
-    else store_tail(out, 0, left, v);
+#pragma unroll
+    for (int w = 0; w < RW; ++w)
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const int left = left_of(n0, k);
+        if (m0 + 16 * w + c < a.M && left > 0)
+          store_out<T>(a, m0 + 16 * w + c, n0 + 32 * k + 8 * g, left, mine[w], y[w][k],
+                       acc[w][k][0], acc[w][k][1], f[w].factor);
+      }
+    load_rows(n0 + STEP);
   }
 }
 
 template <typename T>
-hxm_status launch_lora(const LoraArgs& a, hipStream_t stream) {
-  const int tiles = static_cast<int>(ceil_div(a.M, kRows));
+hxm_status launch_lora(LoraArgs a, hipStream_t stream) {
+  const bool few = a.M < kManyRows;
   hxm_status st = HXM_OK;
-  const dim3 gs(tiles, std::min(kRows, a.M), a.splits);
   if (a.adapters > 0) {
-#define HXM_LORA_SHRINK(RT) lora_shrink_kernel<T, RT><<<gs, kWaves * 64, 0, stream>>>(a)
-    if (a.R <= 16) HXM_LORA_SHRINK(1);
-    else if (a.R <= 32) HXM_LORA_SHRINK(2);
-    else if (a.R <= 64) HXM_LORA_SHRINK(4);
-    else if (a.R <= 128) HXM_LORA_SHRINK(8);
-    else HXM_LORA_SHRINK(16);
-#undef HXM_LORA_SHRINK
+    // Few rows take all adapters of a tile at once, of which many rows have one or two.
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.M, kRows)), few ? std::min(kRows, a.M) : 4,
+                    static_cast<unsigned>(a.splits * ceil_div(a.R, 128)));
+    if (a.R <= 16) lora_shrink_kernel<T, 1><<<grid, kWaves * 64, 0, stream>>>(a);
+    else if (a.R <= 32) lora_shrink_kernel<T, 2><<<grid, kWaves * 64, 0, stream>>>(a);
+    else if (a.R <= 64) lora_shrink_kernel<T, 4><<<grid, kWaves * 64, 0, stream>>>(a);
+    else lora_shrink_kernel<T, 8><<<grid, kWaves * 64, 0, stream>>>(a);
     if ((st = check_launch("lora shrink")) != HXM_OK) return st;
   }
-  const dim3 ge(static_cast<unsigned>(ceil_div(a.N, a.n_per_group)), tiles);
-#define HXM_LORA_EXPAND(KS) lora_expand_kernel<T, KS><<<ge, kWaves * 64, 0, stream>>>(a)
+#define HXM_LORA_EXPAND(KS)                                                                    \
+  do {                                                                                         \
+    constexpr int RW = KS <= 2 ? 2 : 1, NB = 1;                                                \
+    if (few) {                                                                                 \
+      lora_expand_few_kernel<T, KS>                                                            \
+          <<<dim3(static_cast<unsigned>(ceil_div(a.N, 32)),                                    \
+                  static_cast<unsigned>(ceil_div(a.M, kRows))),                                \
+             kWaves * 64, 0, stream>>>(a);                                                     \
+    } else {                                                                                   \
+      /* Columns of a workgroup, in whole steps: what leaves four workgroups a CU. */          \
+      const int64_t tiles = ceil_div(a.M, kRows * RW * kWaves), step = 32 * NB;                \
+      const int64_t want = std::max<int64_t>(1, 1024 / tiles);                                 \
+      a.n_per_group = static_cast<int>(ceil_div(ceil_div(a.N, want), step) * step);            \
+      a.tiles = static_cast<int>(tiles);                                                       \
+      const int64_t groups = ceil_div(ceil_div(a.N, a.n_per_group), 8) * 8 * tiles;            \
+      if ((st = check_grid("lora expand", groups, kWaves * 64)) != HXM_OK) return st;          \
+      lora_halves_kernel<T, KS>                                                                \
+          <<<static_cast<unsigned>(ceil_div(a.M, kRows * kWaves)), kWaves * 64, 0, stream>>>(  \
+              a);                                                                              \
+      lora_expand_kernel<T, KS, RW, NB>                                                        \
+          <<<static_cast<unsigned>(groups), kWaves * 64, 0, stream>>>(a);                      \
+    }                                                                                          \
+  } while (0)
   if (a.R <= 32) HXM_LORA_EXPAND(1);
   else if (a.R <= 64) HXM_LORA_EXPAND(2);
   else if (a.R <= 128) HXM_LORA_EXPAND(4);
@@ -293,21 +584,22 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
   a.ldy = ldy, a.ldx = ldx, a.ldo = ldo, a.K = K, a.N = N;
   a.R = static_cast<int>(R), a.adapters = static_cast<int>(adapters);
   const int64_t piece = std::min(std::min(M, kLoraRows), (kLoraPlaneBytes / (R * 4)) & ~int64_t(15));
-  // K split until about 512 workgroups, each with 512 of K or more.
+  // K split until about 512 workgroups, in 8 parts at most, each a step of all its waves
+  // or more.
   const int64_t tiles = ceil_div(piece, kRows);
-  int64_t splits = std::max<int64_t>(1, std::min(ceil_div(512, tiles), K / 512));
-  const int64_t step = 32 * kWaves;
+  const int64_t step = 32 * kWaves * shrink_steps(R <= 16 ? 1 : R <= 64 ? 4 : 8);
+  const int64_t splits = std::min<int64_t>(std::min<int64_t>(8, ceil_div(512, tiles)), ceil_div(K, step));
   a.k_per_split = static_cast<int>(ceil_div(ceil_div(K, splits), step) * step);
   a.splits = static_cast<int>(ceil_div(K, a.k_per_split));
-  // Columns of a workgroup: as few as keep 1024 workgroups busy.
-  const int64_t want = std::max<int64_t>(1, 1024 / tiles);
-  a.n_per_group = static_cast<int>(ceil_div(ceil_div(N, want), step) * step);
   void* ws = nullptr;
-  if (adapters > 0 &&
-      (st = stream_workspace(as_stream(stream), static_cast<size_t>(a.splits * piece * R * 4), &ws,
+  const int64_t plane_bytes = a.splits * piece * R * 4, halves_bytes = piece * R * 4;
+  if ((st = stream_workspace(as_stream(stream),
+                             static_cast<size_t>(plane_bytes + halves_bytes + piece * 4), &ws,
                              kWsLayer)) != HXM_OK)
     return st;
   a.t = static_cast<float*>(ws);
+  a.halves = static_cast<char*>(ws) + plane_bytes;
+  a.factors = reinterpret_cast<float*>(static_cast<char*>(ws) + plane_bytes + halves_bytes);
   for (int64_t m = 0; m < M; m += piece) {
     a.M = static_cast<int>(std::min(piece, M - m));
     a.y = static_cast<const char*>(y) + m * ldy * 2;
