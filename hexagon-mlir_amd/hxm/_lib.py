@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libhxm.so")
 
@@ -79,24 +80,12 @@ class Plan(ctypes.Structure):
                 ("n", ctypes.c_int64), ("k", ctypes.c_int64)]
 
 
-class RowNorm(ctypes.Structure):
-    """hxm_row_norm: one norm of hxm_residual_norm_rows."""
-    _fields_ = [("kind", ctypes.c_int32), ("eps", ctypes.c_float), ("gamma", ctypes.c_void_p),
-                ("beta", ctypes.c_void_p)]
-
-
-class KvCache(ctypes.Structure):
-    """hxm_kv_cache: a paged key-value cache."""
-    _fields_ = ([("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
-                + [(n, ctypes.c_int64) for n in (
-                    "pages", "page_size", "heads", "dim", "k_page_stride", "k_head_stride",
-                    "k_token_stride", "v_page_stride", "v_head_stride", "v_token_stride")])
-
-
-class Heads(ctypes.Structure):
-    """hxm_heads: a [tokens, heads, dim] view."""
-    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
-                ("head_stride", ctypes.c_int64)]
+# The structures of the decoder-layer operators, as the bytes the C side reads
+# (a call packs them anew each time: a tenth of what building a ctypes.Structure
+# of their fields takes).
+ROW_NORM = struct.Struct("@ifPP")   # hxm_row_norm: kind, eps, gamma, beta
+HEADS = struct.Struct("@Pqq")       # hxm_heads: data, token stride, head stride
+KV_CACHE = struct.Struct("@PP10q")  # hxm_kv_cache: k, v, pages, page_size, heads, dim, strides
 
 
 class ArmQuantiles(ctypes.Structure):
@@ -122,7 +111,6 @@ _f32 = ctypes.c_float
 _f64 = ctypes.c_double
 _st = ctypes.c_int  # hxm_status
 _cfgp = ctypes.POINTER(GemmConfig)
-_hp = ctypes.POINTER(Heads)
 
 # name -> (restype, argtypes); the exact list of include/hxm.h.
 SIGNATURES = {
@@ -161,13 +149,12 @@ SIGNATURES = {
     "hxm_rmsnorm_rows": (_st, [_p, _i64, _p, _p, _i64, _i64, _i64, _f32, _i32, _p]),
     "hxm_layernorm_rows": (_st, [_p, _i64, _p, _p, _p, _i64, _p, _p, _i64, _i64, _f32, _i32,
                                  _p]),
-    "hxm_residual_norm_rows": (_st, [_p, _i64, _p, _i64, ctypes.POINTER(RowNorm), _p, _i64, _i64,
-                                     _f32, _f32, ctypes.POINTER(RowNorm), _p, _i64, _p, _i64,
-                                     _i64, _i64, _i32, _p]),
-    "hxm_rope_append": (_st, [_hp, _hp, _i64, _hp, _hp, _p, _p, _i64, _i64, _i64, _i32, _p,
-                              ctypes.POINTER(KvCache), _i64, _i32, _p]),
-    "hxm_paged_attention": (_st, [_hp, _hp, _i64, ctypes.POINTER(KvCache), _p, _i64, _i64, _p,
-                                  _i64, _f32, _i64, _p, _i32, _p]),
+    "hxm_residual_norm_rows": (_st, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _f32, _f32, _p,
+                                     _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
+    "hxm_rope_append": (_st, [_p, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p, _p, _i64,
+                              _i32, _p]),
+    "hxm_paged_attention": (_st, [_p, _p, _i64, _p, _p, _i64, _i64, _p, _i64, _f32, _i64, _p,
+                                  _i32, _p]),
     "hxm_lora_add": (_st, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64,
                            _i64, _i32, _p]),
     "hxm_probe_copy": (_st, [_p, _p, _i64, _p]),

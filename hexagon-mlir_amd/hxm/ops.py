@@ -15,8 +15,8 @@ from typing import Optional, Sequence
 import torch
 
 from ._lib import (B_KN, B_NK, BF16, F16, F32, I8, I32, IMAGE_GEMM, IMAGE_W8A16, NORM_LAYER,
-                   NORM_NONE, NORM_RMS, OP_W8A16, OP_W8A16_SWIGLU, W_NK, W_PACKED, GemmConfig,
-                   Heads, HxmError, KvCache, RowNorm, check, lib)
+                   HEADS, KV_CACHE, NORM_NONE, NORM_RMS, OP_W8A16, OP_W8A16_SWIGLU, ROW_NORM,
+                   W_NK, W_PACKED, GemmConfig, HxmError, check, lib)
 
 _DT = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32,
        torch.int8: I8, torch.int32: I32}
@@ -593,28 +593,50 @@ def layer_norm(x: torch.Tensor, normalized_shape: Sequence[int],
     return (out, mean, rstd) if return_stats else out
 
 
-def _on_current(t: torch.Tensor, name: str) -> None:
-    """The decoder-layer operators launch on the current device."""
+# The current device's number, without the Python around torch.cuda.current_device().
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _on_current(t: torch.Tensor, name: str) -> int:
+    """The device of a GPU tensor, which must be the current one (the
+    decoder-layer operators launch there)."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor (got {t.device})")
-    if t.device.index != torch.cuda.current_device():
+    dev = t.get_device()
+    if dev != _current_device():
         raise ValueError(f"{name} is on {t.device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+                         f"cuda:{_current_device()}")
+    return dev
+
+
+def _tensor(t: torch.Tensor, dtype: torch.dtype, shape, dev: int, name: str) -> torch.Tensor:
+    """t, checked to be of this dtype and shape on this device."""
+    if t.dtype != dtype or t.shape != shape or t.get_device() != dev:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on cuda:{dev} "
+                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
+    return t
+
+
+def _ints(t: torch.Tensor, shape, dev: int, name: str) -> int:
+    """The address of a contiguous int32 tensor of this shape on this device."""
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be torch.int32 (got {t.dtype})")
+    if not _tensor(t, torch.int32, shape, dev, name).is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
 
 
 _NORMS = {"none": NORM_NONE, "rms": NORM_RMS, "layer": NORM_LAYER}
 
 
-def _row_norm(kind: str, weight, bias, eps: float, x: torch.Tensor, name: str):
-    """The hxm_row_norm and the tensors it points to."""
-    import ctypes
+def _row_norm(kind: str, weight, bias, eps: float, x: torch.Tensor, cols: int, name: str):
+    """The hxm_row_norm, and the tensors it points to (to be kept until the call)."""
     if kind not in _NORMS:
         raise ValueError(f"{name} must be one of {sorted(_NORMS)} (got {kind!r})")
-    w = _row_param(weight, x, x.shape[-1], f"{name}_weight")
-    b = _row_param(bias, x, x.shape[-1], f"{name}_bias")
-    n = RowNorm(_NORMS[kind], eps, None if w is None else w.data_ptr(),
-                None if b is None else b.data_ptr())
-    return ctypes.byref(n), (w, b)
+    w = _row_param(weight, x, cols, f"{name}_weight") if weight is not None else None
+    b = _row_param(bias, x, cols, f"{name}_bias") if bias is not None else None
+    return ROW_NORM.pack(_NORMS[kind], eps, 0 if w is None else w.data_ptr(),
+                         0 if b is None else b.data_ptr()), w, b
 
 
 def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
@@ -636,42 +658,42 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
     biases [cols]; ``pre="none"`` gives z = None.  ``gate``: [cols], or
     [G, cols] with one row for every rows / G consecutive rows.  ``out`` (y)
     and ``normed_out`` (z) may be ``x`` or ``h`` themselves."""
-    _on_current(h, "h")
-    if h.dtype not in _FLOATS:
-        raise TypeError(f"h must be {' or '.join(str(d) for d in _FLOATS)} (got {h.dtype})")
-    if h.dim() < 1 or h.shape[-1] < 1:
+    dev = _on_current(h, "h")
+    dtype, shape = h.dtype, h.shape
+    if dtype not in _FLOATS:
+        raise TypeError(f"h must be {' or '.join(str(d) for d in _FLOATS)} (got {dtype})")
+    if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"h must have a last dimension of one element or more "
-                         f"(got {tuple(h.shape)})")
-    if x.shape != h.shape or x.dtype != h.dtype or x.device != h.device:
-        raise ValueError(f"x must be {h.dtype} {tuple(h.shape)} on {h.device} "
-                         f"(got {x.dtype} {tuple(x.shape)} on {x.device})")
+                         f"(got {tuple(shape)})")
+    _tensor(x, dtype, shape, dev, "x")
     h2, rows, cols = _rows(h)
     x2, _, _ = _rows(x)
     y, y2 = _rows_out(out, h, cols)
     if pre == "none":
         if normed_out is not None:
             raise ValueError("normed_out needs a pre norm")
-        z = z2 = None
+        z = None
+        z_ptr, ldz = None, 0
     else:
         z, z2 = _rows_out(normed_out, h, cols)
-    post_n, keep_post = _row_norm(post, post_weight, post_bias, post_eps, h, "post")
-    pre_n, keep_pre = _row_norm(pre, pre_weight, pre_bias, pre_eps, h, "pre")
-    G = 0
+        z_ptr, ldz = z2.data_ptr(), _ld(z2)
+    post_n, *keep_post = _row_norm(post, post_weight, post_bias, post_eps, h, cols, "post")
+    pre_n, *keep_pre = _row_norm(pre, pre_weight, pre_bias, pre_eps, h, cols, "pre")
+    gate_ptr, ldg, G = None, 0, 0
     if gate is not None:
-        if gate.dtype != h.dtype or gate.device != h.device:
-            raise ValueError(f"gate must be {h.dtype} on {h.device} "
+        if gate.dtype != dtype or gate.get_device() != dev:
+            raise ValueError(f"gate must be {dtype} on cuda:{dev} "
                              f"(got {gate.dtype} on {gate.device})")
         g2 = gate.view(1, -1) if gate.dim() == 1 else gate
         if g2.dim() != 2 or g2.shape[1] != cols or g2.shape[0] < 1 or rows % g2.shape[0]:
             raise ValueError(f"gate must be [{cols}] or [G, {cols}] with G dividing {rows} rows "
                              f"(got {tuple(gate.shape)})")
         gate = g2 if g2.stride(1) == 1 else g2.contiguous()
-        G = gate.shape[0]
-    st = lib.hxm_residual_norm_rows(
-        h2.data_ptr(), _ld(h2), x2.data_ptr(), _ld(x2), post_n,
-        gate.data_ptr() if G else None, _ld(gate) if G else 0, G, block_scale, residual_scale,
-        pre_n, y2.data_ptr(), _ld(y2), None if z2 is None else z2.data_ptr(),
-        0 if z2 is None else _ld(z2), rows, cols, _code(h), _stream(stream))
+        gate_ptr, ldg, G = gate.data_ptr(), _ld(gate), gate.shape[0]
+    st = lib.hxm_residual_norm_rows(h2.data_ptr(), _ld(h2), x2.data_ptr(), _ld(x2), post_n,
+                                    gate_ptr, ldg, G, block_scale, residual_scale, pre_n,
+                                    y2.data_ptr(), _ld(y2), z_ptr, ldz, rows, cols, _DT[dtype],
+                                    _stream(stream))
     if st:
         check(st, "hxm_residual_norm_rows")
     return y, z
@@ -680,43 +702,32 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
 _HALVES = (torch.float16, torch.bfloat16)
 
 
-def _heads(t: torch.Tensor, like: torch.Tensor, shape, name: str) -> Heads:
-    """The hxm_heads of a [tokens, heads, dim] tensor of like's dtype and device."""
-    if t.shape != shape or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be {like.dtype} {tuple(shape)} on {like.device} "
-                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
-    st = t.stride()
-    if st[2] != 1:
+def _heads(t: torch.Tensor, dtype: torch.dtype, shape, dev: int, name: str) -> bytes:
+    """The hxm_heads of a [tokens, heads, dim] tensor."""
+    ts, hs, inner = _tensor(t, dtype, shape, dev, name).stride()
+    if inner != 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
-    return Heads(t.data_ptr(), st[0], st[1])
+    return HEADS.pack(t.data_ptr(), ts, hs)
 
 
-def _kv_cache(k: torch.Tensor, v: torch.Tensor) -> KvCache:
-    """The hxm_kv_cache of [pages, heads, page_size, dim] tensors of any
-    strides (a cache that keeps tokens before heads is passed transposed)."""
-    _on_current(k, "k_cache")
-    if k.dim() != 4:
-        raise ValueError(f"k_cache must be [pages, heads, page_size, dim] (got {tuple(k.shape)})")
-    if k.dtype not in _HALVES:
-        raise TypeError(f"k_cache must be {' or '.join(str(d) for d in _HALVES)} (got {k.dtype})")
-    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
-        raise ValueError(f"v_cache must be {k.dtype} {tuple(k.shape)} on {k.device} "
-                         f"(got {v.dtype} {tuple(v.shape)} on {v.device})")
-    pages, heads, page, dim = k.shape
-    ks, vs = k.stride(), v.stride()
-    if ks[3] != 1 or vs[3] != 1:
+def _kv_cache(k: torch.Tensor, v: torch.Tensor):
+    """The hxm_kv_cache of [pages, heads, page_size, dim] tensors of any strides
+    (a cache that keeps tokens before heads is passed transposed), its heads
+    and dim, dtype and device."""
+    dev = _on_current(k, "k_cache")
+    dtype, shape = k.dtype, k.shape
+    if len(shape) != 4:
+        raise ValueError(f"k_cache must be [pages, heads, page_size, dim] (got {tuple(shape)})")
+    if dtype not in _HALVES:
+        raise TypeError(f"k_cache must be {' or '.join(str(d) for d in _HALVES)} (got {dtype})")
+    _tensor(v, dtype, shape, dev, "v_cache")
+    pages, heads, page, dim = shape
+    kp, kh, kt, ki = k.stride()
+    vp, vh, vt, vi = v.stride()
+    if ki != 1 or vi != 1:
         raise ValueError("k_cache and v_cache must have a contiguous last dimension")
-    return KvCache(k.data_ptr(), v.data_ptr(), pages, page, heads, dim, *ks[:3], *vs[:3])
-
-
-def _ints(t: torch.Tensor, shape, like: torch.Tensor, name: str) -> int:
-    """The address of an int32 tensor of this shape, contiguous, on like's device."""
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} must be torch.int32 (got {t.dtype})")
-    if t.shape != shape or t.device != like.device or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {tuple(shape)} on {like.device} "
-                         f"(got {tuple(t.shape)} on {t.device})")
-    return t.data_ptr()
+    return (KV_CACHE.pack(k.data_ptr(), v.data_ptr(), pages, page, heads, dim, kp, kh, kt, vp, vh,
+                          vt), heads, dim, dtype, dev)
 
 
 def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
@@ -735,23 +746,22 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     then sines) rotate the first rot_dim dims, in halves or (``interleaved``)
     in neighbouring pairs; without cos_sin nothing is rotated.  ``q_out`` may be
     q."""
-    import ctypes
-    cache = _kv_cache(k_cache, v_cache)
+    cache, heads, dim, dtype, dev = _kv_cache(k_cache, v_cache)
     if k.dim() != 3:
         raise ValueError(f"k must be [tokens, heads, dim] (got {tuple(k.shape)})")
     T = k.shape[0]
-    kv_shape = (T, cache.heads, cache.dim)
-    kh, vh = _heads(k, k_cache, kv_shape, "k"), _heads(v, k_cache, kv_shape, "v")
-    slot_p = _ints(slots, (T,), k_cache, "slots")
+    kh = _heads(k, dtype, (T, heads, dim), dev, "k")
+    vh = _heads(v, dtype, (T, heads, dim), dev, "v")
+    slot_p = _ints(slots, (T,), dev, "slots")
     pos_p = tab_p = None
     rot = ld = max_pos = 0
     if cos_sin is not None:
         if positions is None:
             raise ValueError("cos_sin needs positions")
-        pos_p = _ints(positions, (T,), k_cache, "positions")
+        pos_p = _ints(positions, (T,), dev, "positions")
         _mat(cos_sin, "cos_sin")
-        if cos_sin.dtype != torch.float32 or cos_sin.device != k_cache.device:
-            raise ValueError(f"cos_sin must be torch.float32 on {k_cache.device} "
+        if cos_sin.dtype != torch.float32 or cos_sin.get_device() != dev:
+            raise ValueError(f"cos_sin must be torch.float32 on cuda:{dev} "
                              f"(got {cos_sin.dtype} on {cos_sin.device})")
         max_pos, rot = cos_sin.shape
         tab_p, ld = cos_sin.data_ptr(), _ld(cos_sin)
@@ -761,16 +771,14 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         if q.dim() != 3:
             raise ValueError(f"q must be [tokens, heads, dim] (got {tuple(q.shape)})")
         hq = q.shape[1]
-        shape = (T, hq, cache.dim)
-        qh = _heads(q, k_cache, shape, "q")
+        qh = _heads(q, dtype, (T, hq, dim), dev, "q")
         if q_out is None:
-            q_out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        oh = _heads(q_out, k_cache, shape, "q_out")
+            q_out = torch.empty((T, hq, dim), dtype=dtype, device=q.device)
+        oh = _heads(q_out, dtype, (T, hq, dim), dev, "q_out")
     elif q_out is not None:
         raise ValueError("q_out needs q")
     st = lib.hxm_rope_append(qh, oh, hq, kh, vh, pos_p, tab_p, ld, max_pos, rot,
-                             int(interleaved), slot_p, ctypes.byref(cache), T, _DT[k.dtype],
-                             _stream(stream))
+                             int(interleaved), slot_p, cache, T, _DT[dtype], _stream(stream))
     if st:
         check(st, "hxm_rope_append")
     return q_out
@@ -788,29 +796,29 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``scale`` defaults to D ** -0.5; ``window`` keeps the last tokens only
     (0: all).  Returns out, or (out, lse) with the fp32 [B, Hq] logarithm of
     the softmax's sum."""
-    import ctypes
-    cache = _kv_cache(k_cache, v_cache)
+    cache, _, dim, dtype, dev = _kv_cache(k_cache, v_cache)
     if q.dim() != 3:
         raise ValueError(f"q must be [batch, heads, dim] (got {tuple(q.shape)})")
-    B, hq = q.shape[:2]
-    shape = (B, hq, cache.dim)
-    qh = _heads(q, k_cache, shape, "q")
+    B, hq, _ = q.shape
+    qh = _heads(q, dtype, (B, hq, dim), dev, "q")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    oh = _heads(out, k_cache, shape, "out")
+        out = torch.empty((B, hq, dim), dtype=dtype, device=q.device)
+    oh = _heads(out, dtype, (B, hq, dim), dev, "out")
     _mat(block_table, "block_table")
     if block_table.dtype != torch.int32:
         raise TypeError(f"block_table must be torch.int32 (got {block_table.dtype})")
-    if block_table.shape[0] != B or block_table.device != q.device:
-        raise ValueError(f"block_table must have {B} rows on {q.device} "
+    rows, table_pages = block_table.shape
+    if rows != B or block_table.get_device() != dev:
+        raise ValueError(f"block_table must have {B} rows on cuda:{dev} "
                          f"(got {tuple(block_table.shape)} on {block_table.device})")
-    lens_p = _ints(seq_lens, (B,), q, "seq_lens")
-    lse = torch.empty((B, hq), dtype=torch.float32, device=q.device) if return_lse else None
-    st = lib.hxm_paged_attention(qh, oh, hq, ctypes.byref(cache), block_table.data_ptr(),
-                                 _ld(block_table), block_table.shape[1], lens_p, B,
-                                 cache.dim ** -0.5 if scale is None else scale, window,
-                                 None if lse is None else lse.data_ptr(), _DT[q.dtype],
-                                 _stream(stream))
+    lens_p = _ints(seq_lens, (B,), dev, "seq_lens")
+    lse = lse_p = None
+    if return_lse:
+        lse = torch.empty((B, hq), dtype=torch.float32, device=q.device)
+        lse_p = lse.data_ptr()
+    st = lib.hxm_paged_attention(qh, oh, hq, cache, block_table.data_ptr(), _ld(block_table),
+                                 table_pages, lens_p, B, dim ** -0.5 if scale is None else scale,
+                                 window, lse_p, _DT[dtype], _stream(stream))
     if st:
         check(st, "hxm_paged_attention")
     return (out, lse) if return_lse else out
@@ -826,33 +834,31 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     y [M, N] is the projection's output and x [M, K] its input (f16 or bf16);
     A [adapters, R, K] and B [adapters, N, R] contiguous, R a multiple of 8 up
     to 256; scale fp32 [adapters].  ``out`` may be y."""
-    _on_current(y, "y")
+    dev = _on_current(y, "y")
     _mat(y, "y"), _mat(x, "x")
+    dtype = y.dtype
     _dtype(y, _HALVES, "y")
     M, N = y.shape
     K = x.shape[1]
-    for t, name in ((x, "x"), (A, "A"), (B, "B")):
-        if t.dtype != y.dtype or t.device != y.device:
-            raise ValueError(f"{name} must be {y.dtype} on {y.device} (got {t.dtype} on {t.device})")
-    if x.shape[0] != M:
-        raise ValueError(f"x must have {M} rows (got {x.shape[0]})")
-    if A.dim() != 3 or A.shape[2] != K or not A.is_contiguous():
-        raise ValueError(f"A must be contiguous [adapters, R, {K}] (got {tuple(A.shape)})")
-    L, R = A.shape[:2]
-    if B.shape != (L, N, R) or not B.is_contiguous():
-        raise ValueError(f"B must be contiguous {(L, N, R)} (got {tuple(B.shape)})")
-    index_p = _ints(index, (M,), y, "index")
+    _tensor(x, dtype, (M, K), dev, "x")
+    if A.dim() != 3:
+        raise ValueError(f"A must be [adapters, R, {K}] (got {tuple(A.shape)})")
+    L, R, _ = A.shape
+    _tensor(A, dtype, (L, R, K), dev, "A"), _tensor(B, dtype, (L, N, R), dev, "B")
+    if not A.is_contiguous() or not B.is_contiguous():
+        raise ValueError("A and B must be contiguous")
+    index_p = _ints(index, (M,), dev, "index")
+    scale_p = None
     if scale is not None:
-        if scale.device != y.device:
-            raise ValueError(f"scale must be on {y.device} (got {scale.device})")
-        scale = _f32_vec(scale, L, "scale")
+        scale = _tensor(scale, torch.float32, (L,), dev, "scale").contiguous()
+        scale_p = scale.data_ptr()
     if out is None:
-        out = torch.empty((M, N), dtype=y.dtype, device=y.device)
+        out = torch.empty((M, N), dtype=dtype, device=y.device)
     else:
-        _out(out, (M, N), (y.dtype,), y)
+        _out(out, (M, N), (dtype,), y)
     st = lib.hxm_lora_add(y.data_ptr(), _ld(y), x.data_ptr(), _ld(x), A.data_ptr(), B.data_ptr(),
-                          L, R, index_p, None if scale is None else scale.data_ptr(),
-                          out.data_ptr(), _ld(out), M, N, K, _DT[y.dtype], _stream(stream))
+                          L, R, index_p, scale_p, out.data_ptr(), _ld(out), M, N, K, _DT[dtype],
+                          _stream(stream))
     if st:
         check(st, "hxm_lora_add")
     return out
