@@ -3,8 +3,9 @@
 //   p = post(h);  y = residual_scale * x + block_scale * gate * p;  z = pre(y).
 //
 // Bound by memory: h and x are read once, y and z written once, 4 * rows * cols
-// elements against about ten operations each.  Done apart (norm, add, norm)
-// the same takes 8 * rows * cols.  As in the row kernels a row is held in
+// elements against about ten operations each (8192 x 4096 f16: 268 MB in 48 us, 5.6
+// TB/s; a copy of as much runs at 5.4).  Done apart (norm, add, norm) the same
+// takes 8 * rows * cols.  As in the row kernels a row is held in
 // registers by S waves: h and x in their storage type, y in fp32, so that z is
 // the norm of the y before its rounding; the norms' sums cross the waves
 // through LDS.  The kinds of the two norms are uniform branches, not template
@@ -45,7 +46,12 @@ struct RowStats {
 };
 
 // Registers: h, x and the fp32 y of VPL vectors a lane.
-template <typename T, int VPL, int S>
+//
+// EARLY: weights, biases and gate are loaded with h and x, not where they are used.
+// For calls of one workgroup a CU or fewer, whose time is their chain of loads (1 x 8192
+// bf16, LayerNorms and gate: 7.6 -> 6.6 us; 300 x 1000 f32: 6.1 -> 5.3); the registers it takes
+// cost larger ones more (2048 x 4096 bf16 14.4 -> 16.6), and 16 waves a row have none left.
+template <typename T, int VPL, int S, bool EARLY>
 __global__ __launch_bounds__(row_waves(S) * 64) void residual_norm_kernel(ResidualArgs a) {
   constexpr int N = RowVec<T>::N;
   constexpr int WAVES = row_waves(S);
@@ -128,19 +134,36 @@ __global__ __launch_bounds__(row_waves(S) * 64) void residual_norm_kernel(Residu
   if (gate && a.rows_per_gate)
     gate += static_cast<int64_t>(static_cast<uint32_t>(rv) / a.rows_per_gate) * a.ldg;
 
+  struct Params {
+    RawVec<T> post_w, post_b, gate, pre_w, pre_b;
+  };
+  auto load_post = [&](Params& p, int i) {
+    p.post_w = param(a.post.gamma, i, T(1)), p.post_b = param(a.post.beta, i, T(0));
+    p.gate = param(gate, i, T(1));
+  };
+  auto load_pre = [&](Params& p, int i) {
+    p.pre_w = param(a.pre.gamma, i, T(1)), p.pre_b = param(a.pre.beta, i, T(0));
+  };
+  Params early[EARLY ? VPL : 1];
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) load_post(early[i], i), load_pre(early[i], i);
+  }
+
   const RowStats ps = stats(a.post, 0, [&](int i, int j) { return tof(h[i][j]); });
   float y[VPL][N];
   T* yr = static_cast<T*>(a.y) + rv * a.ldy;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    const RawVec<T> w = param(a.post.gamma, i, T(1)), b = param(a.post.beta, i, T(0)),
-                    g = param(gate, i, T(1));
+    Params& q = early[EARLY ? i : 0];
+    if constexpr (!EARLY) load_post(q, i);
     const bool all = whole(i);
     RawVec<T> o;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float p = fmaf((tof(h[i][j]) - ps.mean) * ps.rstd, tof(w[j]), tof(b[j]));
-      const float v = fmaf(a.block_scale * tof(g[j]), p, a.residual_scale * tof(x[i][j]));
+      const float p =
+          fmaf((tof(h[i][j]) - ps.mean) * ps.rstd, tof(q.post_w[j]), tof(q.post_b[j]));
+      const float v = fmaf(a.block_scale * tof(q.gate[j]), p, a.residual_scale * tof(x[i][j]));
       y[i][j] = all || col0(i) + j < cols ? v : 0.0f;
       o[j] = fromf<T>(v);
     }
@@ -151,11 +174,12 @@ __global__ __launch_bounds__(row_waves(S) * 64) void residual_norm_kernel(Residu
   T* zr = static_cast<T*>(a.z) + rv * a.ldz;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    const RawVec<T> w = param(a.pre.gamma, i, T(1)), b = param(a.pre.beta, i, T(0));
+    Params& q = early[EARLY ? i : 0];
+    if constexpr (!EARLY) load_pre(q, i);
     RawVec<T> o;
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      o[j] = fromf<T>(fmaf((y[i][j] - zs.mean) * zs.rstd, tof(w[j]), tof(b[j])));
+      o[j] = fromf<T>(fmaf((y[i][j] - zs.mean) * zs.rstd, tof(q.pre_w[j]), tof(q.pre_b[j])));
     if (valid) store_at(zr, i, o);
   }
 }
@@ -268,8 +292,10 @@ hxm_status launch_residual(const ResidualArgs& a, hipStream_t stream) {
     kernel<<<static_cast<unsigned>(groups), threads, 0, stream>>>(a);
     st = check_launch("residual norm");
   };
-#define HXM_RESIDUAL(V, S) \
-  launch(residual_norm_kernel<T, V, S>, 64 * row_waves(S), row_waves(S) / (S))
+#define HXM_RESIDUAL(V, S)                                                                      \
+  ceil_div(a.rows, row_waves(S) / (S)) <= 256                                                  \
+      ? launch(residual_norm_kernel<T, V, S, (S < 16)>, 64 * row_waves(S), row_waves(S) / (S)) \
+      : launch(residual_norm_kernel<T, V, S, false>, 64 * row_waves(S), row_waves(S) / (S))
   if (nv <= 64) HXM_RESIDUAL(1, 1);
   else if (nv <= 128) HXM_RESIDUAL(2, 1);
   else if (nv <= 192) HXM_RESIDUAL(3, 1);

@@ -1,8 +1,9 @@
 // Rotary positions and the append to the paged key-value cache, in one launch:
 // q -> rotated q, k -> rotated k in its cache row, v -> its cache row.
 //
-// Bound by memory: every element of q, k and v is read once and written once;
-// a pair takes two products and two fmas.  A group of threads serves one token.
+// Bound by memory: every element of q, k and v is read once and written once
+// (8192 tokens, 32 + 8 heads of 128, bf16: 206 MB in 41 us, 5.0 TB/s; a copy of 1 GiB
+// runs at 5.3); a pair takes two products and two fmas.  A group of threads serves one token.
 // A thread keeps one chunk of the rotated dims (eight pairs, or four
 // neighbouring ones) and walks the heads with it, so it loads its cosines and
 // sines once per token and not once per head; the q heads, the k heads and then
@@ -262,9 +263,12 @@ extern "C" hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out
   a.rchunks = static_cast<int>(ceil_div(interleaved ? rot_dim : rot_dim / 2, kChunk));
   a.chunks = a.rchunks + static_cast<int>(ceil_div(dim - rot_dim, kChunk));
   // Threads of a token: one for each chunk it has, a power of two from 64 to
-  // a workgroup's 256 (a head has at most 32 chunks).
+  // a workgroup's 256, or 128 once the tokens fill the chip that way (a head has at
+  // most 33 chunks).  32 + 8 heads of 128: 8192 tokens 42.7 us with 256, 41.2 with 128, 46
+  // with 64; 64 tokens 5.2, 5.5, 6.8.
   a.tt = 64;
-  while (a.tt < 256 && a.tt < a.chunks * (a.hq + a.hkv)) a.tt *= 2;
+  const int most = tokens >= 2048 ? 128 : 256;
+  while (a.tt < most && a.tt < a.chunks * (a.hq + a.hkv)) a.tt *= 2;
   const int64_t groups = ceil_div(tokens, 256 / a.tt);
   if ((st = check_grid("rope append", groups, 256)) != HXM_OK) return st;
   const unsigned g = static_cast<unsigned>(groups);
