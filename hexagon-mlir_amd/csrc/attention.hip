@@ -43,24 +43,25 @@ namespace hxm {
 
 namespace {
 
-constexpr int kTile = 32;       // tokens of a wave's step
-constexpr int kHeads = 16;      // query heads of a workgroup
+constexpr int kTile = kAttnTile;  // tokens of a wave's step
+constexpr int kHeads = 16;        // query heads of a workgroup
 constexpr int kWaves = 4;
 constexpr int kUnit = kWaves * kTile;
-constexpr int64_t kMaxTokens = int64_t(1) << 30;  // of a sequence
+static_assert(kUnit == kAttnUnit, "a unit is one step of all waves");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;  // of the running maximum, in powers of two
 
-// Pieces a batch is cut into where it can be, one for each CU: what a workgroup has
-// under way (a tile of each wave) keeps its CU at its share of the memory's rate, fewer
-// pieces are fewer to join, and all run at once.  More at once only starve each
-// other: with three workgroups a CU, 8 x 32768 tokens, the first to end took 31 us and the
-// last 79; 32768 tokens of one sequence, 8 heads of 8, 32 us with 256 pieces, 42 with 768.
-constexpr int kGroups = 256;
-// Where sequences times heads are more than that, kFine times as many pieces level
-// what their lengths differ by (16 x 8192 tokens at most, 32 heads: 150 us with 2, 141 with
-// 3, 143 with 4 and more; 64 x 4096, 8 heads: 81.5, 80.7, 80.7).
-constexpr int kFine = 3;
+// The pieces (kAttnGroups and kAttnFine): one for each CU where the sequences allow it.  What a
+// workgroup has under way (a tile of each wave) keeps its CU at its share of the
+// memory's rate, fewer pieces are fewer to join, and all run at once.  More at once only
+// starve each other: with three workgroups a CU, 8 x 32768 tokens, the first to end took 31 us
+// and the last 79; 32768 tokens of one sequence, 8 heads of 8, 32 us with 256 pieces, 42
+// with 768.  Where sequences times heads are more than that, three times as many pieces
+// level what their lengths differ by (16 x 8192 tokens at most, 32 heads: 150 us with 2,
+// 141 with 3, 143 with 4 and more; 64 x 4096, 8 heads: 81.5, 80.7, 80.7).  A join costs
+// about what three units do, so four units are left whole (1 x 300 tokens, 32 heads: 7.8 us
+// whole, 9.2 in two).
+
 // Waves a SIMD, by the registers of a tile and the output: many short sequences
 // hide each other's start.
 constexpr int attn_waves(int dt) { return dt <= 64 ? 4 : dt <= 128 ? 2 : 1; }
@@ -147,56 +148,41 @@ struct Piece {
   bool over;          // longer than its table row
 };
 
-// Piece u of the batch, its sequences in order.  Every wave works it out from the
-// lengths, 64 sequences at a time: they are on the device, so the host cannot.
-//
-// Lengths count in units of kUnit tokens; a sequence of up to four is one
-// piece, since a join costs about what three units do (1 x 300 tokens, 32 heads: 7.8
-// us whole, 9.2 in two).  Longer ones are cut into equal pieces of at most `size`
-// units: with share = all units / kGroups, the least of share, 5/4, 3/2 and 2
-// shares that gives no more than kGroups pieces; where none does (many sequences), 1 / kFine
-// of a share, but eight units or more.  Then there are at most kFine * kGroups + batch * heads
-// pieces, fewer than 2 * kFine * kGroups of them parts of a sequence: one cut in c pieces
-// has more than (c - 1) * size units, so size * c is less than twice its units.
+// Piece u of the batch, its sequences in order, cut as host_logic.h says.  Every wave
+// works it out from the lengths, 64 sequences at a time: they are on the device, so
+// the host cannot.  Batches of more than 64 take the fine pieces without trying the others.
 __device__ __forceinline__ Piece find_piece(const AttnArgs& a, uint32_t u, int lane) {
   auto tokens = [&](int32_t len, int* lo) {
     const int n = len > a.capacity ? 0 : max(len, 0);
     *lo = a.window > 0 ? max(0, n - a.window) : 0;
     return n;
   };
-  // Zero past the last sequence; at most 2^23.
-  auto units = [&](int b, int32_t len) {
+  auto units = [&](int b, int32_t len) {  // zero past the last sequence
     int lo;
     const int n = tokens(len, &lo);
-    const uint32_t w = static_cast<uint32_t>(n - (lo & ~(kTile - 1)) + kUnit - 1) / kUnit;
-    return b < a.batch ? max(1u, w) : 0u;
+    return b < a.batch ? attn_units(n, lo) : 0u;
   };
   auto length = [&](int b) { return b < a.batch ? a.lens[b] : 0; };
   const int32_t len0 = length(lane);
   const uint32_t w0 = units(lane, len0);
   uint64_t total = wave_sum(w0);
   for (int b = 64; b < a.batch; b += 64) total += wave_sum(units(b + lane, length(b + lane)));
-  // (No sequence has more than 2^23 units: a larger share cuts nothing either.)
-  const uint32_t share = static_cast<uint32_t>(
-      min<uint64_t>((total * a.heads + kGroups - 1) / kGroups, uint64_t(1) << 24));
-  auto cut = [](uint32_t w, uint32_t size) {
-    return w <= 4u ? min(w, 1u) : (w + size - 1) / size;
-  };
-  uint32_t size = max(2u, share);
+  const uint32_t share = attn_share(total, a.heads);
+  uint32_t size = 0;
   bool fits = false;
   if (a.batch <= 64)
     for (uint32_t k = 0; k < 4 && !fits; ++k) {
-      size = max(2u, share + (k < 3 ? k : 4) * share / 4);
-      fits = wave_sum(cut(w0, size)) * a.heads <= static_cast<uint32_t>(kGroups);
+      size = attn_size(share, k);
+      fits = wave_sum(attn_cut(w0, size)) * a.heads <= kAttnGroups;
     }
-  if (!fits) size = max(8u, (share + kFine - 1) / kFine);
+  if (!fits) size = attn_fine_size(share);
   Piece r{};
   r.b = -1;
   uint32_t first = 0, slots = 0;  // pieces, and partial slots, of the sequences before
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int32_t len = b0 == 0 ? len0 : length(b0 + lane);
     const uint32_t w = units(b0 + lane, len);
-    const uint32_t c = cut(w, size), cs = c > 1 ? c : 0u;
+    const uint32_t c = attn_cut(w, size), cs = c > 1 ? c : 0u;
     const uint32_t upto = wave_scan(c, lane), upto_s = wave_scan(cs, lane);
     const uint64_t hit = __ballot(u < first + upto);
     if (hit) {
@@ -637,11 +623,7 @@ __global__ __launch_bounds__(kWaves * 64)
 
 template <typename T, int DT>
 hxm_status launch_attention(const AttnArgs& a, hipStream_t stream) {
-  // Pieces at most, by either rule of find_piece and by what a sequence can have.
-  const int64_t bh = static_cast<int64_t>(a.batch) * a.heads;
-  const int64_t units = ceil_div(a.capacity + kTile, kUnit);
-  const int64_t groups = std::max(std::min<int64_t>(kGroups, bh * (units / 2 + 1)),
-                                  std::min(kFine * kGroups + bh, bh * (units / 8 + 1)));
+  const int64_t groups = attn_grid(static_cast<int64_t>(a.batch) * a.heads, a.capacity);
   hxm_status st = check_grid("paged attention", groups, kWaves * 64);
   if (st != HXM_OK) return st;
   const unsigned n = static_cast<unsigned>(groups);
@@ -712,7 +694,7 @@ extern "C" hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* o
   a.vps = cache->v_page_stride, a.vhs = cache->v_head_stride, a.vts = cache->v_token_stride;
   a.table = block_table, a.lens = seq_lens, a.lse = lse;
   a.ld_table = ld_table;
-  a.capacity = std::min(table_pages * cache->page_size, kMaxTokens);
+  a.capacity = std::min(table_pages * cache->page_size, kAttnMaxTokens);
   a.pages = static_cast<uint32_t>(cache->pages);
   a.page_size = static_cast<uint32_t>(cache->page_size);
   a.page_div = fast_div(a.page_size);
@@ -727,7 +709,7 @@ extern "C" hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* o
   // Partial results of the sequences cut in pieces, and a counter for each
   // sequence and head, zero between launches.
   a.slot_rows = std::min(a.group, kHeads);
-  const int64_t parts = int64_t(2 * kFine * kGroups) * a.slot_rows * (a.dim + 2) * 4;
+  const int64_t parts = int64_t(2 * kAttnFine * kAttnGroups) * a.slot_rows * (a.dim + 2) * 4;
   const int64_t counts = batch * a.heads * 4;
   void* ws = nullptr;
   hipStream_t s = as_stream(stream);

@@ -169,19 +169,48 @@ inline FastDiv fast_div(uint32_t d) {
   return FastDiv{static_cast<uint32_t>((p + d - 1) / d), 31 + l};
 }
 
-// How paged attention splits its sequences over workgroups.  A sequence spans
-// span tokens, in units of 32 rounded up; with T the sum of all spans in a batch,
-// a piece is at least T * heads / target of them, a multiple of kAttnPieceStep
-// (each of a workgroup's four waves has the same number of steps) and no fewer
-// than kAttnPieceMin.  Pieces of all sequences and heads then number at most
-// target + batch * heads (each sequence rounds up once), and those of sequences
-// of two pieces or more at most 2 * target: such a sequence has fewer than twice
-// span / piece.
-constexpr int64_t kAttnPieceStep = 4, kAttnPieceMin = 8;
-constexpr int64_t attn_piece(int64_t total_units, int64_t heads, int64_t target) {
-  const int64_t want = ceil_div(total_units * heads, target);
-  const int64_t piece = ceil_div(want, kAttnPieceStep) * kAttnPieceStep;
-  return piece < kAttnPieceMin ? kAttnPieceMin : piece;
+// How paged attention cuts a batch into pieces, one for a workgroup.  Lengths count
+// in units of kAttnUnit tokens (of the window, from its first tile on; no sequence
+// is 0).  A sequence of up to kAttnWhole units is one piece.  Longer ones are cut
+// into equal pieces of at most `size` units: with share = all units / kAttnGroups,
+// the least of attn_size(share, 0 .. 3) that gives no more than kAttnGroups pieces over all
+// heads; where none does, attn_fine_size(share), which gives at most kAttnFine * kAttnGroups + batch
+// * heads.  Pieces of sequences cut in two or more then number at most 2 * kAttnFine *
+// kAttnGroups: one cut in c has more than (c - 1) * size units, so size * c is
+// less than twice its units.
+constexpr int64_t kAttnUnit = 128, kAttnTile = 32;
+constexpr uint32_t kAttnGroups = 256, kAttnFine = 3, kAttnWhole = 4, kAttnFineLeast = 8;
+constexpr int64_t kAttnMaxTokens = int64_t(1) << 30;  // of a sequence: 2^23 units
+constexpr uint32_t attn_units(int32_t n, int32_t lo) {  // of tokens [lo, n)
+  const int32_t from = lo & ~static_cast<int32_t>(kAttnTile - 1);
+  const uint32_t w =
+      (static_cast<uint32_t>(n - from) + static_cast<uint32_t>(kAttnUnit) - 1) / kAttnUnit;
+  return w > 1 ? w : 1;
+}
+// (No sequence has more than 2^23 units: a larger share cuts nothing either.)
+constexpr uint32_t attn_share(uint64_t units, uint64_t heads) {
+  const uint64_t s = (units * heads + kAttnGroups - 1) / kAttnGroups;
+  return s < (uint64_t(1) << 25) ? static_cast<uint32_t>(s) : uint32_t(1) << 25;
+}
+constexpr uint32_t attn_size(uint32_t share, uint32_t k) {  // share, 5/4, 3/2, 2 of it
+  const uint32_t s = share + (k < 3 ? k : 4) * share / 4;
+  return s > 2 ? s : 2;
+}
+constexpr uint32_t attn_fine_size(uint32_t share) {
+  const uint32_t s = (share + kAttnFine - 1) / kAttnFine;
+  return s > kAttnFineLeast ? s : kAttnFineLeast;
+}
+constexpr uint32_t attn_cut(uint32_t w, uint32_t size) {
+  return w <= kAttnWhole ? (w > 0 ? 1u : 0u) : (w + size - 1) / size;
+}
+// Workgroups that hold the pieces of any lengths: batch * heads = bh sequences' heads
+// of at most `capacity` tokens.
+inline int64_t attn_grid(int64_t bh, int64_t capacity) {
+  const int64_t units = ceil_div(capacity + kAttnTile, kAttnUnit);
+  const int64_t even = bh * (units / 2 + 1), fine = bh * (units / kAttnFineLeast + 1);
+  const int64_t g = kAttnGroups, f = kAttnFine * g + bh;
+  const int64_t a = even < g ? even : g, b = fine < f ? fine : f;
+  return a > b ? a : b;
 }
 
 // One entry of the tuning-cache file: "op M N K bm bn bk waves_m waves_n

@@ -4,9 +4,10 @@ Every cache row outside a sequence's tokens holds NaN, every table entry past
 its pages an invalid number.  Tolerances, from arithmetic alone, with A the
 mean of |v| under the exact probabilities and u = eps / 2 of the dtype:
 * out is rounded once: u |o|;
-* each probability is rounded once for the product with V: u A (the sum that
-  normalises adds the unrounded ones), and in f16 a subnormal one is off by
-  half of 2^-24, at least 2^7 below the scaled maximum: n 2^-32 max|v|;
+* each probability enters the product with V as two halves of the dtype, the second
+  the rounded rest of the first: 2 u^2 A at most (the sum that normalises adds the
+  unrounded ones), and in f16 a subnormal second half is off by half of 2^-24, at
+  least 2^7 below the scaled maximum: n 2^-32 max|v|;
 * scores: fp32 sums of dim products, (dim + 8) 2^-24 of scale sum|q k|, move a
   probability by that much relatively, and the mean of v by twice that of A;
 * the exponential, the rescalings and the chains of the fp32 sums, n / 16 terms
@@ -74,7 +75,7 @@ def check(out, lse, q, seqs, group, scale, window, name):
             p /= p.sum()
             want, A = p @ vh, p @ np.abs(vh)
             d = 2.0 ** -24 * ((dim + 8) * mag + n / 16 + 64)
-            tol = u * np.abs(want) + (u + 2 * d) * A + tiny
+            tol = u * np.abs(want) + (2 * u * u + 2 * d) * A + tiny
             if name == "f16":
                 tol = tol + n * 2.0 ** -32 * np.abs(vh).max()
             got = out[b, h].double().numpy()
@@ -132,6 +133,42 @@ def test_long(dev, name, lens):
     run_case(dev, name, lens, 2, 4, 128, 16, "nhd")
     run_case(dev, name, lens, 1, 1, 256, 40, "hnd")
     run_case(dev, name, lens, 4, 2, 64, 128, "hnd", window=1500)
+
+
+@pytest.mark.parametrize("batch", [63, 64, 65, 128, 200, 513])
+def test_many_sequences(dev, batch):
+    """Batches in and past one wave's lanes, of one long sequence among short ones, all
+    alike, and with rows of padding (no tokens) at the end."""
+    r = np.random.default_rng(batch)
+    lens = r.integers(0, 70, batch).tolist()
+    lens[batch // 2] = 2600
+    run_case(dev, "f16", lens, 2, 4, 64, 16, "hnd")
+    run_case(dev, "bf16", [640 if b < batch - 9 else 0 for b in range(batch)], 1, 2, 64, 32, "nhd")
+
+
+@pytest.mark.parametrize("hkv,group", [(32, 1), (8, 8), (64, 2), (2, 33), (300, 1)])
+def test_many_heads(dev, hkv, group):
+    run_case(dev, "bf16", [1000, 0, 2085, 1], hkv, group, 64, 16, "nhd")
+    run_case(dev, "f16", [700], hkv, group, 32, 16, "hnd", window=530)
+
+
+def test_calls_of_changing_sizes(dev):
+    """One stream, one workspace: larger calls after smaller ones and back, the same
+    results as before."""
+    cases = [([3000], 2, 4, 128), ([700] * 70, 4, 2, 64), ([2000, 0, 900], 8, 20, 64),
+             ([30] * 300, 2, 1, 64), ([9000, 5], 1, 16, 256)]
+    first = []
+    for turn in range(3):
+        for i, (lens, hkv, group, dim) in enumerate(cases[::-1] if turn == 1 else cases):
+            got = run_case(dev, "f16", lens, hkv, group, dim, 16, "hnd") if turn == 0 else None
+            if turn == 0:
+                first.append(got)
+                continue
+            i = len(cases) - 1 - i if turn == 1 else i
+            g = torch.Generator().manual_seed(dim + 16 + group)
+            q, kc, vc, table, ld, _ = build(g, "f16", lens, hkv, group, dim, 16, "hnd", dev)
+            out, lse = ops.paged_attention(q.to(dev), kc, vc, table, ld, return_lse=True)
+            assert torch.equal(out, first[i][0]) and torch.equal(lse, first[i][1])
 
 
 @pytest.mark.parametrize("name", ["f16", "bf16"])
