@@ -621,22 +621,46 @@ def _ints(t: torch.Tensor, shape, dev: int, name: str) -> int:
     """The address of a contiguous int32 tensor of this shape on this device."""
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be torch.int32 (got {t.dtype})")
-    if not _tensor(t, torch.int32, shape, dev, name).is_contiguous():
+    if t.shape != shape or t.get_device() != dev:
+        _tensor(t, torch.int32, shape, dev, name)
+    if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
+
+
+def _stream_on(stream, dev: int) -> int:
+    """_stream for a device known to be the current one."""
+    return _raw_stream(dev) if stream is None and _raw_stream is not None else _stream(stream)
+
+
+def _row_ld(t: torch.Tensor, rows: int, cols: int) -> int:
+    """The leading dimension of a [rows, cols] view; one row has none."""
+    return t.stride(0) if rows > 1 else cols
+
+
+def _param(t: Optional[torch.Tensor], dtype: torch.dtype, cols: int, dev: int, name: str,
+           what: str):
+    """(contiguous t, its address): [cols] of dtype on this device, or None."""
+    if t is None:
+        return None, 0
+    if t.numel() != cols or t.dtype != dtype or t.get_device() != dev:
+        raise ValueError(f"{name}_{what} must be {dtype} [{cols}] on cuda:{dev} "
+                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
+    t = t.contiguous()
+    return t, t.data_ptr()
 
 
 _NORMS = {"none": NORM_NONE, "rms": NORM_RMS, "layer": NORM_LAYER}
 
 
-def _row_norm(kind: str, weight, bias, eps: float, x: torch.Tensor, cols: int, name: str):
+def _row_norm(kind: str, weight, bias, eps: float, dtype: torch.dtype, cols: int, dev: int,
+              name: str):
     """The hxm_row_norm, and the tensors it points to (to be kept until the call)."""
     if kind not in _NORMS:
         raise ValueError(f"{name} must be one of {sorted(_NORMS)} (got {kind!r})")
-    w = _row_param(weight, x, cols, f"{name}_weight") if weight is not None else None
-    b = _row_param(bias, x, cols, f"{name}_bias") if bias is not None else None
-    return ROW_NORM.pack(_NORMS[kind], eps, 0 if w is None else w.data_ptr(),
-                         0 if b is None else b.data_ptr()), w, b
+    w, w_ptr = _param(weight, dtype, cols, dev, name, "weight")
+    b, b_ptr = _param(bias, dtype, cols, dev, name, "bias")
+    return ROW_NORM.pack(_NORMS[kind], eps, w_ptr, b_ptr), w, b
 
 
 def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
@@ -676,9 +700,10 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
         z_ptr, ldz = None, 0
     else:
         z, z2 = _rows_out(normed_out, h, cols)
-        z_ptr, ldz = z2.data_ptr(), _ld(z2)
-    post_n, *keep_post = _row_norm(post, post_weight, post_bias, post_eps, h, cols, "post")
-    pre_n, *keep_pre = _row_norm(pre, pre_weight, pre_bias, pre_eps, h, cols, "pre")
+        z_ptr, ldz = z2.data_ptr(), _row_ld(z2, rows, cols)
+    post_n, post_w, post_b = _row_norm(post, post_weight, post_bias, post_eps, dtype, cols, dev,
+                                       "post")
+    pre_n, pre_w, pre_b = _row_norm(pre, pre_weight, pre_bias, pre_eps, dtype, cols, dev, "pre")
     gate_ptr, ldg, G = None, 0, 0
     if gate is not None:
         if gate.dtype != dtype or gate.get_device() != dev:
@@ -690,10 +715,11 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
                              f"(got {tuple(gate.shape)})")
         gate = g2 if g2.stride(1) == 1 else g2.contiguous()
         gate_ptr, ldg, G = gate.data_ptr(), _ld(gate), gate.shape[0]
-    st = lib.hxm_residual_norm_rows(h2.data_ptr(), _ld(h2), x2.data_ptr(), _ld(x2), post_n,
-                                    gate_ptr, ldg, G, block_scale, residual_scale, pre_n,
-                                    y2.data_ptr(), _ld(y2), z_ptr, ldz, rows, cols, _DT[dtype],
-                                    _stream(stream))
+    st = lib.hxm_residual_norm_rows(h2.data_ptr(), _row_ld(h2, rows, cols), x2.data_ptr(),
+                                    _row_ld(x2, rows, cols), post_n, gate_ptr, ldg, G,
+                                    block_scale, residual_scale, pre_n, y2.data_ptr(),
+                                    _row_ld(y2, rows, cols), z_ptr, ldz, rows, cols, _DT[dtype],
+                                    _stream_on(stream, dev))
     if st:
         check(st, "hxm_residual_norm_rows")
     return y, z
@@ -704,7 +730,9 @@ _HALVES = (torch.float16, torch.bfloat16)
 
 def _heads(t: torch.Tensor, dtype: torch.dtype, shape, dev: int, name: str) -> bytes:
     """The hxm_heads of a [tokens, heads, dim] tensor."""
-    ts, hs, inner = _tensor(t, dtype, shape, dev, name).stride()
+    if t.dtype != dtype or t.shape != shape or t.get_device() != dev:
+        _tensor(t, dtype, shape, dev, name)
+    ts, hs, inner = t.stride()
     if inner != 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
     return HEADS.pack(t.data_ptr(), ts, hs)
@@ -773,12 +801,13 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         hq = q.shape[1]
         qh = _heads(q, dtype, (T, hq, dim), dev, "q")
         if q_out is None:
-            q_out = torch.empty((T, hq, dim), dtype=dtype, device=q.device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         oh = _heads(q_out, dtype, (T, hq, dim), dev, "q_out")
     elif q_out is not None:
         raise ValueError("q_out needs q")
     st = lib.hxm_rope_append(qh, oh, hq, kh, vh, pos_p, tab_p, ld, max_pos, rot,
-                             int(interleaved), slot_p, cache, T, _DT[dtype], _stream(stream))
+                             int(interleaved), slot_p, cache, T, _DT[dtype],
+                             _stream_on(stream, dev))
     if st:
         check(st, "hxm_rope_append")
     return q_out
@@ -802,7 +831,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     B, hq, _ = q.shape
     qh = _heads(q, dtype, (B, hq, dim), dev, "q")
     if out is None:
-        out = torch.empty((B, hq, dim), dtype=dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     oh = _heads(out, dtype, (B, hq, dim), dev, "out")
     _mat(block_table, "block_table")
     if block_table.dtype != torch.int32:
@@ -818,7 +847,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         lse_p = lse.data_ptr()
     st = lib.hxm_paged_attention(qh, oh, hq, cache, block_table.data_ptr(), _ld(block_table),
                                  table_pages, lens_p, B, dim ** -0.5 if scale is None else scale,
-                                 window, lse_p, _DT[dtype], _stream(stream))
+                                 window, lse_p, _DT[dtype], _stream_on(stream, dev))
     if st:
         check(st, "hxm_paged_attention")
     return (out, lse) if return_lse else out
@@ -853,12 +882,12 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
         scale = _tensor(scale, torch.float32, (L,), dev, "scale").contiguous()
         scale_p = scale.data_ptr()
     if out is None:
-        out = torch.empty((M, N), dtype=dtype, device=y.device)
+        out = torch.empty_like(y, memory_format=torch.contiguous_format)
     else:
         _out(out, (M, N), (dtype,), y)
-    st = lib.hxm_lora_add(y.data_ptr(), _ld(y), x.data_ptr(), _ld(x), A.data_ptr(), B.data_ptr(),
-                          L, R, index_p, scale_p, out.data_ptr(), _ld(out), M, N, K, _DT[dtype],
-                          _stream(stream))
+    st = lib.hxm_lora_add(y.data_ptr(), _row_ld(y, M, N), x.data_ptr(), _row_ld(x, M, K),
+                          A.data_ptr(), B.data_ptr(), L, R, index_p, scale_p, out.data_ptr(),
+                          _row_ld(out, M, N), M, N, K, _DT[dtype], _stream_on(stream, dev))
     if st:
         check(st, "hxm_lora_add")
     return out
