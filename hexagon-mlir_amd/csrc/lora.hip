@@ -158,6 +158,19 @@ __global__ __launch_bounds__(kWaves * 64) void lora_shrink_kernel(LoraArgs a) {
   }
 }
 
+// 2^-ex takes a row's largest |t|, top, to [1/2, 1); 0, infinities and NaN stay as
+// they are.
+__device__ __forceinline__ int row_exponent(float top) {
+  return top > 0.0f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) : 0;
+}
+template <typename T>
+__device__ __forceinline__ void split_halves(float v, T* hi, T* lo) {
+  *hi = fromf<T>(v);
+  // An infinite or NaN hi needs no remainder (it would be NaN).
+  const float rest = v - tof(*hi);
+  *lo = fromf<T>(rest == rest ? rest : 0.0f);
+}
+
 // t of a row, ranks 32 s + 8 g .. + 8, as two halves scaled by 2^-ex, and the factor
 // that takes the product back: the adapter's scale times 2^ex.
 template <typename T, int KS>
@@ -217,50 +230,161 @@ __device__ __forceinline__ void load_factors(const LoraArgs& a, int m0, const in
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(t[w][s][e]));
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    // 2^-ex takes the row's largest |t| to [1/2, 1); 0, infinities and NaN stay as
-    // they are.
-    int ex = 0;
-    if (top > 0.0f && top < __builtin_huge_valf()) ex = __builtin_amdgcn_frexp_expf(top);
+    const int ex = row_exponent(top);
     f[w].factor =
         live[w] ? __builtin_amdgcn_ldexpf(a.scale ? a.scale[id[w]] : 1.0f, ex) : 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_amdgcn_ldexpf(t[w][s][e], -ex);
-        f[w].hi[s][e] = fromf<T>(v);
-        // An infinite or NaN hi needs no remainder (it would be NaN).
-        const float rest = v - tof(f[w].hi[s][e]);
-        f[w].lo[s][e] = fromf<T>(rest == rest ? rest : 0.0f);
+        T hi, lo;
+        split_halves(__builtin_amdgcn_ldexpf(t[w][s][e], -ex), &hi, &lo);
+        f[w].hi[s][e] = hi, f[w].lo[s][e] = lo;
       }
   }
 }
 
-// Many rows: each row's factors made once, for the many workgroups that read them.  16 rows a
-// wave; halves [M][hi, lo][R] and the factors [M].  (Made by each workgroup from the planes they
-// were 67 MB of reads beside y's 90: 2048 rows, 4096 -> 11008, R 64, 9 us of 63; the
-// launch gives 4 of them back.)
-template <typename T, int KS>
-__global__ __launch_bounds__(kWaves * 64) void lora_halves_kernel(LoraArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-  const int m0 = (blockIdx.x * kWaves + wave) * kRows, m = m0 + c;
-  const int id = row_adapter(a, m);
-  const bool live = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.adapters);
-  RowFactors<T, KS> f[1];
-  load_factors<T, KS, 1>(a, m0, {id}, {live}, g, c, f);
-  if (m >= a.M) return;
-  T* halves = static_cast<T*>(a.halves) + static_cast<int64_t>(m) * 2 * a.R;
+// Many rows: t of 64 rows, a part of K; workgroup (tile, y, part) takes the tile's adapters y,
+// y + ways, .. in the order of their first rows.  A wave's 16 rows of x stay in
+// registers, 256 of K at a time; 16 RT ranks of an adapter's A lie in LDS for all
+// four waves, read in whole rows.  (Each wave reading its own operand of A, 16 rows of 64
+// bytes an instruction, took 18 us where this takes HXM_TODO: 2048 rows, 4096 -> 64.)
+constexpr int kManyTile = kRows * kWaves;
+constexpr int kManyK = 256;
+template <typename T, int RT, int NC>
+__global__ __launch_bounds__(kWaves * 64) void lora_shrink_many_kernel(LoraArgs a) {
+  using V = typename Mma<T>::V;
+  constexpr int U = kManyK / 32, CHUNKS = 2 * RT;  // 16-byte chunks of A a thread brings
+  constexpr int PITCH = kManyK / 8 + 1;            // of a rank's row in LDS, chunks
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int m0 = blockIdx.x * kManyTile, ways = gridDim.y;
+  const int all = row_adapter(a, m0 + lane);
+  const int64_t k_begin = static_cast<int64_t>(blockIdx.z) * a.k_per_split;
+  const int64_t k_end = min(a.K, k_begin + a.k_per_split);
+  const T* x = static_cast<const T*>(a.x) +
+               static_cast<int64_t>(min(m0 + wave * kRows + c, a.M - 1)) * a.ldx;
+  __shared__ __align__(16) v4u32_t la[RT * 16 * PITCH];
+  v4f32 acc[NC][RT];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int r = 32 * s + 8 * g;
-    if (r < a.R) {
-      *reinterpret_cast<typename Mma<T>::V*>(halves + r) = f[0].hi[s];
-      *reinterpret_cast<typename Mma<T>::V*>(halves + a.R + r) = f[0].lo[s];
+  for (int h = 0; h < NC; ++h)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) acc[h][r] = v4f32(0.0f);
+  uint64_t done = 0;
+  for (int64_t k0 = k_begin; k0 < k_end; k0 += kManyK) {
+    v4u32_t xv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = k0 + 32 * u + 8 * g;
+      xv[u] = *reinterpret_cast<const any4*>(x + (k < k_end ? k : 0));
+      xv[u] = k < k_end ? xv[u] : v4u32_t(0u);
     }
+    const int mine = __shfl(all, wave * kRows + c, 64);
+    int seen = 0;
+    for (uint64_t todo = __ballot(static_cast<uint32_t>(all) < static_cast<uint32_t>(a.adapters));
+         todo; ++seen) {
+      const int id = __builtin_amdgcn_readlane(all, __builtin_ctzll(todo));
+      const uint64_t same = __ballot(all == id);
+      todo &= ~same;
+      if (seen % ways != static_cast<int>(blockIdx.y)) continue;
+      done |= same;
+      const bool hit = mine == id;
+#pragma unroll
+      for (int h = 0; h < NC; ++h) {
+        if (16 * RT * h >= a.R) break;
+        v4u32_t st[CHUNKS];
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+          const int q = i * (kWaves * 64) + threadIdx.x, col = q % (kManyK / 8);
+          const int rank = min(16 * RT * h + q / (kManyK / 8), a.R - 1);
+          const int64_t k = k0 + 8 * col;
+          st[i] = *reinterpret_cast<const any4*>(
+              static_cast<const T*>(a.A) + (static_cast<int64_t>(id) * a.R + rank) * a.K +
+              (k < k_end ? k : 0));
+          st[i] = k < k_end ? st[i] : v4u32_t(0u);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+          const int q = i * (kWaves * 64) + threadIdx.x;
+          la[q / (kManyK / 8) * PITCH + q % (kManyK / 8)] = st[i];
+        }
+        __syncthreads();
+        if ((same >> (kRows * wave)) & 0xffff) {
+          v4f32 d[RT];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) d[r] = acc[h][r];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+              d[r] = Mma<T>::run(__builtin_bit_cast(V, la[(16 * r + c) * PITCH + 4 * u + g]),
+                                 __builtin_bit_cast(V, xv[u]), d[r]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) acc[h][r] = hit ? d[r] : acc[h][r];
+        }
+      }
+    }
+    if (!done) return;
   }
-  if (g == 0) a.factors[m] = f[0].factor;
+  // acc[h][r][i]: rank 16 (RT h + r) + 4g + i of row c.
+  if (!((done >> (kRows * wave + c)) & 1)) return;
+  float* t = a.t + (static_cast<int64_t>(blockIdx.z) * a.M + m0 + wave * kRows + c) * a.R;
+#pragma unroll
+  for (int h = 0; h < NC; ++h)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int rank = 16 * (RT * h + r) + 4 * g;
+      if (rank < a.R) *reinterpret_cast<v4f32*>(t + rank) = acc[h][r];
+    }
 }
-// A row's factors as lora_halves_kernel left them (zeros past the last rank).
+
+// Many rows: each row's factors made once, for the many workgroups that read them: halves
+// [M][hi, lo][R] and the factors [M].  A row is LANES neighbouring lanes, four ranks
+// each; the planes are added in order, eight loads under way at once (past the last plane,
+// its own again, which is not added).
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void lora_halves_kernel(LoraArgs a) {
+  constexpr int P = 8;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  const int m = static_cast<int>(min<int64_t>(at, a.M - 1));
+  const int r = threadIdx.x % LANES * 4, id = a.index[m];
+  const bool live = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.adapters);
+  const bool in = live && at < a.M && r < a.R;
+  const float* tp = a.t + (in ? static_cast<int64_t>(m) * a.R + r : 0);
+  v4f32 t = v4f32(0.0f);
+  for (int p0 = 0; p0 < a.splits; p0 += P) {
+    v4f32 v[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      v[i] = *reinterpret_cast<const v4f32*>(
+          tp + static_cast<int64_t>(min(p0 + i, a.splits - 1)) * a.M * a.R);
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (p0 + i < a.splits) t += v[i];
+  }
+  float top = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = in ? fmaxf(top, fabsf(t[e])) : 0.0f;
+#pragma unroll
+  for (int i = LANES / 2; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i, 64));
+  if (!in) return;
+  const int ex = row_exponent(top);
+  typedef T half4 __attribute__((ext_vector_type(4)));
+  half4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    T h, l;
+    split_halves(__builtin_amdgcn_ldexpf(t[e], -ex), &h, &l);
+    hi[e] = h, lo[e] = l;
+  }
+  T* halves = static_cast<T*>(a.halves) + static_cast<int64_t>(m) * 2 * a.R + r;
+  *reinterpret_cast<half4*>(halves) = hi;
+  *reinterpret_cast<half4*>(halves + a.R) = lo;
+  if (r == 0) a.factors[m] = __builtin_amdgcn_ldexpf(a.scale ? a.scale[id] : 1.0f, ex);
+}
+// A row's factors as lora_halves_kernel left them (zeros past the last rank; a row
+// without an adapter: whatever is there, and not used).
 template <typename T, int KS>
 __device__ __forceinline__ void load_halves(const LoraArgs& a, int m, int g,
                                             RowFactors<T, KS>& f) {
@@ -383,110 +507,144 @@ __global__ __launch_bounds__(kWaves * 64) void lora_expand_few_kernel(LoraArgs a
   if (here && left > 0) store_out<T>(a, m, n, left, mine, y, acc[0], acc[1], f[0].factor);
 }
 
-// Many rows: workgroup (columns, rows), a wave RW * 16 rows and 32 * NB columns at a time,
-// the adapters of its rows one after another; the waves walk the same columns, so
-// that the L1 serves three of four reads of the weights.  The next weights load as
-// soon as the products have used these, the next rows of y as soon as these are
-// stored, into the same registers (a copy from others would wait for the load).
+// Many rows: workgroup (64 rows, 32 NB columns), a wave 16 of the rows.  Everything a wave
+// needs of y is under way before its adapters are known; the columns' rows of B, one
+// block of memory, lie in LDS for the four waves, one adapter after another (the next
+// one's on their way during the products), and a row's y takes its sum in place when its
+// adapter's turn comes.
 //
-// Workgroups go to the XCDs in turn: XCD i takes the column groups i, i + 8, .. and
-// walks the rows with each, so that its L2 holds the group's weights.
-template <typename T, int KS, int RW, int NB>
-__global__ __launch_bounds__(kWaves * 64) void lora_expand_kernel(LoraArgs a) {
+// Tiles are numbered down the rows and each XCD (workgroups go to them in turn) takes a run of
+// them, so that its L2 holds the columns' weights.
+constexpr int expand_blocks(int ks) { return ks <= 4 ? 4 : 2; }  // of 32 columns each
+constexpr int expand_waves(int ks) { return ks <= 2 ? 4 : ks <= 4 ? 3 : 2; }
+template <typename T, int KS>
+__global__ __launch_bounds__(kWaves * 64)
+__attribute__((amdgpu_waves_per_eu(expand_waves(KS)))) void lora_expand_kernel(LoraArgs a) {
+  using V = typename Mma<T>::V;
+  constexpr int NB = expand_blocks(KS), COLS = 32 * NB;
+  constexpr int ROW = 4 * KS, PITCH = ROW + 1;  // 16-byte chunks of a row of B, and its pitch
+  constexpr int CHUNKS = COLS * ROW / (kWaves * 64);
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  const int turn = blockIdx.x / 8;
-  const int m0 = (turn % a.tiles * kWaves + wave) * (kRows * RW);
-  const int64_t n_begin =
-      (turn / a.tiles * 8 + static_cast<int64_t>(blockIdx.x % 8)) * a.n_per_group;
-  constexpr int STEP = 32 * NB;
-  if (n_begin >= a.N || m0 >= a.M) return;
-  const int n_end = static_cast<int>(min(a.N, n_begin + a.n_per_group));
-  int mine[RW];
-  uint64_t all = 0;
+  const uint32_t run = gridDim.x / 8, turn = blockIdx.x % 8 * run + blockIdx.x / 8;
+  const int col = turn / a.tiles;
+  const int m0 = (turn - col * a.tiles) * kManyTile, m = m0 + wave * kRows + c;
+  const int64_t n_begin = static_cast<int64_t>(col) * COLS;
+  if (n_begin >= a.N) return;
+  const int n0 = static_cast<int>(n_begin);
+  const int all = row_adapter(a, m0 + lane);
+  __shared__ __align__(16) v4u32_t lb[COLS * PITCH];
+  // y and then out of a wave: whole rows to and from memory, operands to the products.
+  constexpr int SEG = COLS / 8, SROW = SEG + 1, PER = 64 / SEG, NL = kRows / PER;
+  __shared__ __align__(16) RawVec<T> ly[kWaves][kRows * SROW];
+  const int lrow = lane / SEG, lcol = lane % SEG;
+  const int left = static_cast<int>(min<int64_t>(a.N - (n0 + 8 * lcol), 8));
+  RawVec<T> yl[NL];
+  auto row_at = [&](int j) { return m0 + wave * kRows + PER * j + lrow; };
 #pragma unroll
-  for (int w = 0; w < RW; ++w) {
-    mine[w] = row_adapter(a, m0 + 16 * w + c);
-    const bool live = static_cast<uint32_t>(mine[w]) < static_cast<uint32_t>(a.adapters);
-    all |= (__ballot(live) & 0xffffull) << (16 * w);
+  for (int j = 0; j < NL; ++j)
+    if (row_at(j) < a.M && left > 0) yl[j] = load_y<T>(a, row_at(j), n0 + 8 * lcol, left);
+  uint64_t todo =
+      __ballot(static_cast<uint32_t>(all) < static_cast<uint32_t>(a.adapters));
+  v4u32_t st[CHUNKS];
+  auto fetch = [&](int id) {
+    const T* B = static_cast<const T*>(a.B) + (static_cast<int64_t>(id) * a.N + n0) * a.R;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int q = i * (kWaves * 64) + threadIdx.x, r = q % ROW * 8, n = q / ROW;
+      const bool in = r < a.R && n < a.N - n0;
+      st[i] = *reinterpret_cast<const any4*>(B + (in ? n * a.R + r : 0));
+      st[i] = in ? st[i] : v4u32_t(0u);
+    }
+  };
+  // With ways, this workgroup's adapters alone, and the rows of no adapter in the first one.
+  const int way = blockIdx.y, ways = gridDim.y;
+  uint64_t rows = ~0ull;
+  if (ways > 1) {
+    rows = way == 0 ? ~todo : 0ull;
+    int seen = 0;
+    for (uint64_t left_ids = todo; left_ids; ++seen) {
+      const uint64_t same =
+          __ballot(all == __builtin_amdgcn_readlane(all, __builtin_ctzll(left_ids)));
+      left_ids &= ~same;
+      if (seen % ways == way) rows |= same;
+    }
+    if (!rows) return;
+    todo &= rows;
   }
-  auto first_of = [&](uint64_t todo) {
-    const int row = __builtin_ctzll(todo);
-    int id = __builtin_amdgcn_readlane(mine[0], row & 15);
-    if constexpr (RW == 2) id = row < 16 ? id : __builtin_amdgcn_readlane(mine[1], row & 15);
-    return id;
-  };
-  auto rows_of = [&](int id) {
-    uint64_t r = 0;
+  int id = -1;
+  if (todo) {
+    id = __builtin_amdgcn_readlane(all, __builtin_ctzll(todo));
+    fetch(id);
+  }
+  RowFactors<T, KS> f;
+  load_halves<T, KS>(a, m, g, f);
+  const int mine = __shfl(all, wave * kRows + c, 64);
+  RawVec<T> y[NB];
+  auto swap_in = [&] {
 #pragma unroll
-    for (int w = 0; w < RW; ++w) r |= (__ballot(mine[w] == id) & 0xffffull) << (16 * w);
-    return r;
+    for (int j = 0; j < NL; ++j) ly[wave][(PER * j + lrow) * SROW + lcol] = yl[j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < NB; ++k) y[k] = ly[wave][c * SROW + 4 * k + g];
   };
-  v4u32_t b[NB][2][KS];
-  RawVec<T> y[RW][NB];
-  auto load_weights = [&](int id, int n0) {
+  if (!todo) swap_in();
+  for (bool first = true; todo; first = false) {
+    const uint64_t same = __ballot(all == id);
+    const bool hit = mine == id;
+    todo &= ~same;
+    if (!first) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int q = i * (kWaves * 64) + threadIdx.x;
+      lb[q / ROW * PITCH + q % ROW] = st[i];
+    }
+    __syncthreads();
+    if (todo) {
+      id = __builtin_amdgcn_readlane(all, __builtin_ctzll(todo));
+      fetch(id);
+    }
+    if (first) swap_in();
+    if ((same >> (kRows * wave)) & 0xffff) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        v4f32 d[2] = {v4f32(0.0f), v4f32(0.0f)};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            // Columns 8 (c / 4) + 4u + c % 4 of the 32: a lane ends with 8 neighbours.
+            const V w = __builtin_bit_cast(
+                V, lb[(32 * k + 8 * (c >> 2) + 4 * u + (c & 3)) * PITCH + 4 * s + g]);
+            d[u] = Mma<T>::run(w, f.hi[s], d[u]);
+            d[u] = Mma<T>::run(w, f.lo[s], d[u]);
+          }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          y[k][e] = hit ? fromf<T>(fmaf(f.factor, d[e / 4][e % 4], tof(y[k][e]))) : y[k][e];
+      }
+    }
+  }
+  if (mine >= a.adapters)
 #pragma unroll
     for (int k = 0; k < NB; ++k)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) load_b<T, KS>(a, id, n0 + 32 * k, u, g, c, b[k][u]);
-  };
-  auto left_of = [&](int n0, int k) { return min(8, n_end - (n0 + 32 * k + 8 * g)); };
-  auto load_rows = [&](int n0) {
+      for (int e = 0; e < 8; ++e) y[k][e] = fromf<T>(__builtin_nanf(""));
+  __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int w = 0; w < RW; ++w)
+  for (int k = 0; k < NB; ++k) ly[wave][c * SROW + 4 * k + g] = y[k];
+  __builtin_amdgcn_wave_barrier();
+  // Plain stores: the next operator reads them.
 #pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        const int left = left_of(n0, k);
-        if (m0 + 16 * w + c < a.M && left > 0)
-          y[w][k] = load_y<T>(a, m0 + 16 * w + c, n0 + 32 * k + 8 * g, left);
-      }
-  };
-  int n0 = static_cast<int>(n_begin), id = -1;
-  load_rows(n0);
-  if (all) {
-    id = first_of(all);
-    load_weights(id, n0);
-  }
-  RowFactors<T, KS> f[RW];
-#pragma unroll
-  for (int w = 0; w < RW; ++w) load_halves<T, KS>(a, m0 + 16 * w + c, g, f[w]);
-  for (; n0 < n_end; n0 += STEP) {
-    v4f32 acc[RW][NB][2];
-#pragma unroll
-    for (int w = 0; w < RW; ++w)
-#pragma unroll
-      for (int k = 0; k < NB; ++k)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) acc[w][k][u] = v4f32(0.0f);
-    for (uint64_t todo = all; todo;) {
-      const int now = id;
-      todo &= ~rows_of(now);
-#pragma unroll
-      for (int w = 0; w < RW; ++w) {
-        const bool hit = mine[w] == now;
-#pragma unroll
-        for (int k = 0; k < NB; ++k)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const v4f32 d = times_b<T, KS>(b[k][u], f[w]);
-            acc[w][k][u] = hit ? d : acc[w][k][u];
-          }
-      }
-      // The next adapter of these columns, or the first of the next ones (past the
-      // last, of the last column).
-      id = first_of(todo ? todo : all);
-      load_weights(id, todo ? n0 : n0 + STEP);
-    }
-#pragma unroll
-    for (int w = 0; w < RW; ++w)
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        const int left = left_of(n0, k);
-        if (m0 + 16 * w + c < a.M && left > 0)
-          store_out<T>(a, m0 + 16 * w + c, n0 + 32 * k + 8 * g, left, mine[w], y[w][k],
-                       acc[w][k][0], acc[w][k][1], f[w].factor);
-      }
-    load_rows(n0 + STEP);
+  for (int j = 0; j < NL; ++j) {
+    const RawVec<T> v = ly[wave][(PER * j + lrow) * SROW + lcol];
+    const int of = __shfl(all, wave * kRows + PER * j + lrow, 64);
+    if (row_at(j) >= a.M || left <= 0 || (of < 0 && a.out == a.y) ||
+        !((rows >> (wave * kRows + PER * j + lrow)) & 1))
+      continue;
+    T* out = static_cast<T*>(a.out) + row_at(j) * a.ldo + n0 + 8 * lcol;
+    if (left >= 8) *reinterpret_cast<AnyVec<T>*>(out) = v;
+    else store_tail(out, 0, left, v);
   }
 }
 
@@ -494,9 +652,34 @@ template <typename T>
 hxm_status launch_lora(LoraArgs a, hipStream_t stream) {
   const bool few = a.M < kManyRows;
   hxm_status st = HXM_OK;
-  if (a.adapters > 0) {
-    // Few rows take all adapters of a tile at once, of which many rows have one or two.
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.M, kRows)), few ? std::min(kRows, a.M) : 4,
+  if (a.adapters > 0 && !few) {
+    const int64_t tiles = ceil_div(a.M, kManyTile);
+    // Workgroups for the adapters of a tile until there are four for each CU.
+    const dim3 grid(static_cast<unsigned>(tiles),
+                    static_cast<unsigned>(std::max<int64_t>(
+                        1, std::min<int64_t>(16, 256 / (tiles * a.splits)))),
+                    static_cast<unsigned>(a.splits));
+#define HXM_MANY(RT, NC) lora_shrink_many_kernel<T, RT, NC><<<grid, kWaves * 64, 0, stream>>>(a)
+    if (a.R <= 16) HXM_MANY(1, 1);
+    else if (a.R <= 32) HXM_MANY(2, 1);
+    else if (a.R <= 64) HXM_MANY(4, 1);
+    else if (a.R <= 128) HXM_MANY(4, 2);
+    else HXM_MANY(4, 4);
+#undef HXM_MANY
+    if ((st = check_launch("lora shrink")) != HXM_OK) return st;
+#define HXM_HALVES(LANES)                                                       \
+  lora_halves_kernel<T, LANES><<<static_cast<unsigned>(ceil_div(a.M, 256 / LANES)), 256, 0, \
+                                 stream>>>(a)
+    if (a.R <= 16) HXM_HALVES(4);
+    else if (a.R <= 32) HXM_HALVES(8);
+    else if (a.R <= 64) HXM_HALVES(16);
+    else if (a.R <= 128) HXM_HALVES(32);
+    else HXM_HALVES(64);
+#undef HXM_HALVES
+    if ((st = check_launch("lora halves")) != HXM_OK) return st;
+  } else if (a.adapters > 0) {
+    // All adapters of a tile at once.
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.M, kRows)), std::min(kRows, a.M),
                     static_cast<unsigned>(a.splits * ceil_div(a.R, 128)));
     if (a.R <= 16) lora_shrink_kernel<T, 1><<<grid, kWaves * 64, 0, stream>>>(a);
     else if (a.R <= 32) lora_shrink_kernel<T, 2><<<grid, kWaves * 64, 0, stream>>>(a);
@@ -506,25 +689,21 @@ hxm_status launch_lora(LoraArgs a, hipStream_t stream) {
   }
 #define HXM_LORA_EXPAND(KS)                                                                    \
   do {                                                                                         \
-    constexpr int RW = KS <= 2 ? 2 : 1, NB = 1;                                                \
     if (few) {                                                                                 \
       lora_expand_few_kernel<T, KS>                                                            \
           <<<dim3(static_cast<unsigned>(ceil_div(a.N, 32)),                                    \
                   static_cast<unsigned>(ceil_div(a.M, kRows))),                                \
              kWaves * 64, 0, stream>>>(a);                                                     \
     } else {                                                                                   \
-      /* Columns of a workgroup, in whole steps: what leaves four workgroups a CU. */          \
-      const int64_t tiles = ceil_div(a.M, kRows * RW * kWaves), step = 32 * NB;                \
-      const int64_t want = std::max<int64_t>(1, 1024 / tiles);                                 \
-      a.n_per_group = static_cast<int>(ceil_div(ceil_div(a.N, want), step) * step);            \
-      a.tiles = static_cast<int>(tiles);                                                       \
-      const int64_t groups = ceil_div(ceil_div(a.N, a.n_per_group), 8) * 8 * tiles;            \
+      a.tiles = static_cast<int>(ceil_div(a.M, kManyTile));                                    \
+      const int64_t groups =                                                                   \
+          ceil_div(a.tiles * ceil_div(a.N, 32 * expand_blocks(KS)), 8) * 8;                    \
       if ((st = check_grid("lora expand", groups, kWaves * 64)) != HXM_OK) return st;          \
-      lora_halves_kernel<T, KS>                                                                \
-          <<<static_cast<unsigned>(ceil_div(a.M, kRows * kWaves)), kWaves * 64, 0, stream>>>(  \
-              a);                                                                              \
-      lora_expand_kernel<T, KS, RW, NB>                                                        \
-          <<<static_cast<unsigned>(groups), kWaves * 64, 0, stream>>>(a);                      \
+      lora_expand_kernel<T, KS>                                                                \
+          <<<dim3(static_cast<unsigned>(groups),                                               \
+                  static_cast<unsigned>(std::max<int64_t>(                                     \
+                      1, std::min<int64_t>(16, 512 / groups)))),                          \
+             kWaves * 64, 0, stream>>>(a);                                                     \
     }                                                                                          \
   } while (0)
   if (a.R <= 32) HXM_LORA_EXPAND(1);
@@ -585,10 +764,12 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
   a.R = static_cast<int>(R), a.adapters = static_cast<int>(adapters);
   const int64_t piece = std::min(std::min(M, kLoraRows), (kLoraPlaneBytes / (R * 4)) & ~int64_t(15));
   // K split until about 512 workgroups, in 8 parts at most, each a step of all its waves
-  // or more.
-  const int64_t tiles = ceil_div(piece, kRows);
-  const int64_t step = 32 * kWaves * shrink_steps(R <= 16 ? 1 : R <= 64 ? 4 : 8);
-  const int64_t splits = std::min<int64_t>(std::min<int64_t>(8, ceil_div(512, tiles)), ceil_div(K, step));
+  // or more; many rows until 256 of 64 rows.
+  const bool few = piece < kManyRows;
+  const int64_t tiles = ceil_div(piece, few ? kRows : kManyTile);
+  const int64_t step = few ? 32 * kWaves * shrink_steps(R <= 16 ? 1 : R <= 64 ? 4 : 8) : kManyK;
+  const int64_t splits = std::min(std::min<int64_t>(few ? 8 : 16, ceil_div(few ? 512 : 512, tiles)),
+                                  ceil_div(K, step));
   a.k_per_split = static_cast<int>(ceil_div(ceil_div(K, splits), step) * step);
   a.splits = static_cast<int>(ceil_div(K, a.k_per_split));
   void* ws = nullptr;
