@@ -13,13 +13,15 @@
 //
 // Few rows are a matter of latency and of reading many adapters: each adapter of a
 // tile is a workgroup of the first launch and a wave of the second, every load under
-// way at once.  Many rows mostly share one adapter per tile: there a launch between makes
-// the second operand once, and the last walks the columns with 128 rows a workgroup.
-// One form for both, 16 rows and the adapters of a tile in turn, ran 10.9 us for 48 rows of 16
-// adapters, 4096 -> 4096, R 16, against 9.9; 64.6 for 2048 rows of 4, 4096 -> 11008, R 64, against
-// 59; 43 for 256 rows of 16 against 18.  Of the 59 about 20 are the first launch and 33 the
-// last, whose reads of y alone take 22, its weights from L2 10 and its products 7: they
-// hardly overlap.
+// way at once.  Many rows mostly share one adapter per tile: there a tile is 64 rows, whose waves share
+// the adapter's weights through LDS, read in whole rows, and a launch between makes the
+// second operand once.
+//
+// 48 rows of 16 adapters, 4096 -> 4096, R 16: 9.9 us, two launches of 4.7 and 5.4.  2048 rows of 4,
+// 4096 -> 11008, R 64, bf16: 37.5, of them 10 the first launch, 4 the second, and 23 the last,
+// which moves 90 MB of y and out (17 us at a large copy's rate).  With each wave reading its own operands of the
+// weights and of y, 16 rows of 64 bytes an instruction, they were 19, 5 and 39.  2048
+// rows of 16 mixed adapters, 4096 -> 4096, R 16: 52, sixteen turns for each tile.
 //
 // t enters the second product as two 16-bit halves, t = hi + lo: 22 bits of it
 // in f16, 16 in bf16, where one would round t to the weights' 11 or 8.  Rows
@@ -37,8 +39,8 @@ namespace {
 
 constexpr int kRows = 16;   // rows of an MFMA operand
 constexpr int kWaves = 4;
-// Rows from which the form for many is taken (R 16, 4096 -> 4096: 256 rows of 4 adapters 12.2 us
-// with it, 14.0 without; 512 rows of 16 mixed adapters 26.6 and 31).
+// Rows from which the form for many is taken (R 16, 4096 -> 4096: 256 rows of 4 adapters 10.8 us
+// with it, 14.0 without; 512 rows of 16 mixed adapters 24.5 and 31).
 constexpr int64_t kManyRows = 256;
 
 struct LoraArgs {
@@ -247,8 +249,7 @@ __device__ __forceinline__ void load_factors(const LoraArgs& a, int m0, const in
 // Many rows: t of 64 rows, a part of K; workgroup (tile, y, part) takes the tile's adapters y,
 // y + ways, .. in the order of their first rows.  A wave's 16 rows of x stay in
 // registers, 256 of K at a time; 16 RT ranks of an adapter's A lie in LDS for all
-// four waves, read in whole rows.  (Each wave reading its own operand of A, 16 rows of 64
-// bytes an instruction, took 18 us where this takes HXM_TODO: 2048 rows, 4096 -> 64.)
+// four waves, read in whole rows.
 constexpr int kManyTile = kRows * kWaves;
 constexpr int kManyK = 256;
 template <typename T, int RT, int NC>
@@ -546,15 +547,18 @@ __attribute__((amdgpu_waves_per_eu(expand_waves(KS)))) void lora_expand_kernel(L
     if (row_at(j) < a.M && left > 0) yl[j] = load_y<T>(a, row_at(j), n0 + 8 * lcol, left);
   uint64_t todo =
       __ballot(static_cast<uint32_t>(all) < static_cast<uint32_t>(a.adapters));
+  // Zeros past the last rank and the last column, put there when the loads have arrived.
+  auto inside = [&](int i) {
+    const int q = i * (kWaves * 64) + threadIdx.x;
+    return q % ROW * 8 < a.R && q / ROW < a.N - n0;
+  };
   v4u32_t st[CHUNKS];
   auto fetch = [&](int id) {
     const T* B = static_cast<const T*>(a.B) + (static_cast<int64_t>(id) * a.N + n0) * a.R;
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
-      const int q = i * (kWaves * 64) + threadIdx.x, r = q % ROW * 8, n = q / ROW;
-      const bool in = r < a.R && n < a.N - n0;
-      st[i] = *reinterpret_cast<const any4*>(B + (in ? n * a.R + r : 0));
-      st[i] = in ? st[i] : v4u32_t(0u);
+      const int q = i * (kWaves * 64) + threadIdx.x;
+      st[i] = *reinterpret_cast<const any4*>(B + (inside(i) ? q / ROW * a.R + q % ROW * 8 : 0));
     }
   };
   // With ways, this workgroup's adapters alone, and the rows of no adapter in the first one.
@@ -597,7 +601,7 @@ __attribute__((amdgpu_waves_per_eu(expand_waves(KS)))) void lora_expand_kernel(L
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       const int q = i * (kWaves * 64) + threadIdx.x;
-      lb[q / ROW * PITCH + q % ROW] = st[i];
+      lb[q / ROW * PITCH + q % ROW] = inside(i) ? st[i] : v4u32_t(0u);
     }
     __syncthreads();
     if (todo) {
@@ -634,7 +638,7 @@ __attribute__((amdgpu_waves_per_eu(expand_waves(KS)))) void lora_expand_kernel(L
 #pragma unroll
   for (int k = 0; k < NB; ++k) ly[wave][c * SROW + 4 * k + g] = y[k];
   __builtin_amdgcn_wave_barrier();
-  // Plain stores: the next operator reads them.
+  // Nontemporal, like the other row operators: 45 MB of them 2.8 us faster.
 #pragma unroll
   for (int j = 0; j < NL; ++j) {
     const RawVec<T> v = ly[wave][(PER * j + lrow) * SROW + lcol];
@@ -643,7 +647,7 @@ __attribute__((amdgpu_waves_per_eu(expand_waves(KS)))) void lora_expand_kernel(L
         !((rows >> (wave * kRows + PER * j + lrow)) & 1))
       continue;
     T* out = static_cast<T*>(a.out) + row_at(j) * a.ldo + n0 + 8 * lcol;
-    if (left >= 8) *reinterpret_cast<AnyVec<T>*>(out) = v;
+    if (left >= 8) store_any(out, v);
     else store_tail(out, 0, left, v);
   }
 }

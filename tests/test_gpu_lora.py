@@ -94,6 +94,73 @@ def test_many_rows(dev):
     run_case(dev, "f16", 2048, 128, 512, 16, mixed(2048, 6), 6)
 
 
+@pytest.mark.parametrize("R", [8, 16, 24, 32, 40, 64, 72, 128, 136, 200, 256])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_ranks_of_many_rows(dev, name, R):
+    """Tiles of 64 rows with one adapter, several, and none; K that ends inside a step of 256,
+    columns that end inside a block."""
+    run_case(dev, name, 300, 173, 520, R, mixed(300, 5, run=40), 5)
+    run_case(dev, name, 257, 264, 264, R, mixed(257, 9), 9, inplace=True)
+
+
+@pytest.mark.parametrize("M", [255, 256, 257, 320, 700])
+@pytest.mark.parametrize("N,K", [(1, 8), (31, 256), (129, 248), (136, 264), (1000, 2056)])
+def test_odd_sizes_of_many_rows(dev, M, N, K):
+    run_case(dev, "f16", M, N, K, 16, mixed(M, 30), 30)
+    run_case(dev, "bf16", M, N, K, 48, mixed(M, 2, run=90), 2, inplace=True, scaled=False)
+
+
+def test_bad_indexes_and_sick_weights_of_many_rows(dev):
+    run_case(dev, "f16", 260, 70, 64, 16, [-5, 3, 0, 2 ** 31 - 1, -2 ** 31] * 52, 3)
+    run_case(dev, "bf16", 320, 70, 64, 16, [-1] * 130 + [2] * 60 + [-1] * 130, 3, inplace=True)
+    g = torch.Generator().manual_seed(7)
+    M, N, K, R, L = 400, 160, 512, 16, 6
+    x, y = (torch.randn(M, w, generator=g).half().to(dev) for w in (K, N))
+    A, B = (torch.randn(L, a, b, generator=g).half().to(dev) * 0.1 for a, b in ((R, K), (N, R)))
+    index = torch.tensor(mixed(M, L, none=0.1), dtype=torch.int32, device=dev)
+    want = ops.lora_add(y, x, A, B, index)
+    A[2], B[4, 3] = float("nan"), float("inf")
+    sick = int((index == 0).nonzero()[0])
+    x[sick] = float("nan")
+    out = ops.lora_add(y, x, A, B, index)
+    for m, a in enumerate(index.tolist()):
+        if a == 2 or m == sick:
+            assert out[m].isnan().all(), m
+        elif a == 4:
+            assert not out[m, 3].isfinite() and torch.equal(out[m, 4:], want[m, 4:]), m
+        else:
+            assert torch.equal(out[m], want[m]), m
+
+
+def test_many_rows_captured_after_other_sizes(dev):
+    """One stream's workspace under calls of changing sizes, then a captured one."""
+    g = torch.Generator().manual_seed(8)
+    L, R, K, N = 4, 64, 1024, 640
+    A, B = (torch.randn(L, a, b, generator=g).bfloat16().to(dev) * 0.1
+            for a, b in ((R, K), (N, R)))
+    x, y = (torch.randn(600, w, generator=g).bfloat16().to(dev) for w in (K, N))
+    index = torch.tensor(mixed(600, L, run=50), dtype=torch.int32, device=dev)
+    s, graph, out = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.empty_like(y)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        want = ops.lora_add(y, x, A, B, index)
+        for m in (1, 300, 600, 17, 256):
+            part = ops.lora_add(y[:m], x[:m], A, B, index[:m])
+            if m >= 256:
+                assert torch.equal(part[:192], want[:192])
+    with torch.cuda.graph(graph, stream=s):
+        ops.lora_add(y, x, A, B, index, out=out)
+    for k in range(3):
+        x.normal_()
+        index.copy_(torch.tensor(mixed(600, L, seed=k, run=70), dtype=torch.int32))
+        want = ops.lora_add(y, x, A, B, index)
+        out.fill_(9)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), k
+
+
 def test_no_adapters_and_bad_indexes(dev):
     run_case(dev, "f16", 20, 100, 64, 16, [-1] * 20, 3)
     run_case(dev, "f16", 20, 100, 64, 16, [-5, 3, 0, 2 ** 31 - 1, -2 ** 31] * 4, 3)
