@@ -718,7 +718,7 @@ hxm_status launch_lora(LoraArgs a, hipStream_t stream) {
   return check_launch("lora expand");
 }
 
-// Rows of one pair of launches: a t plane of at most 64 MiB, at most 2^15 tiles.
+// Rows of one set of launches: a t plane of at most 64 MiB, at most 2^15 tiles of 16 rows.
 constexpr int64_t kLoraPlaneBytes = int64_t(64) << 20, kLoraRows = int64_t(1) << 19;
 
 }  // namespace
@@ -734,7 +734,7 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
   if (dtype != HXM_F16 && dtype != HXM_BF16)
     return fail(HXM_UNSUPPORTED_DTYPE, "unsupported-dtype: lora_add takes f16 or bf16 (got %d)",
                 dtype);
-  constexpr int64_t kMax = INT32_MAX / 4;
+  constexpr int64_t kMax = INT32_MAX / 4, kMaxN = int64_t(1) << 28;
   if (M < 0 || N < 0 || K < 1 || adapters < 0 || R < 1)
     return fail(HXM_INVALID_ARG, "invalid-argument: lora_add M=%lld N=%lld K=%lld adapters=%lld R=%lld",
                 (long long)M, (long long)N, (long long)K, (long long)adapters, (long long)R);
@@ -742,7 +742,7 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
     return fail(HXM_UNSUPPORTED_SHAPE,
                 "tile-alignment: lora_add K=%lld and R=%lld must be multiples of 8, R at most 256",
                 (long long)K, (long long)R);
-  if (M > kMax || N > kMax || K > kMax || adapters > kMax)
+  if (M > kMax || N > kMaxN || K > kMax || adapters > kMax)
     return fail(HXM_UNSUPPORTED_SHAPE, "tile-alignment: lora_add M=%lld N=%lld K=%lld too large",
                 (long long)M, (long long)N, (long long)K);
   if (!stride_ok(ldy) || !stride_ok(ldx) || !stride_ok(ldo) || ldy < N || ldx < K || ldo < N)
@@ -766,7 +766,11 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
   a.A = A, a.B = B, a.scale = scale;
   a.ldy = ldy, a.ldx = ldx, a.ldo = ldo, a.K = K, a.N = N;
   a.R = static_cast<int>(R), a.adapters = static_cast<int>(adapters);
-  const int64_t piece = std::min(std::min(M, kLoraRows), (kLoraPlaneBytes / (R * 4)) & ~int64_t(15));
+  // Rows of one set of launches: their planes fit the workspace, their tiles of 64 rows and
+  // 64 columns or more a grid.
+  const int64_t piece =
+      std::min({M, kLoraRows, (kLoraPlaneBytes / (R * 4)) & ~int64_t(15),
+                kManyTile * ((int64_t(1) << 23) / ceil_div(N, 64))});
   // K split until about 512 workgroups, in 8 parts at most, each a step of all its waves
   // or more; many rows until 256 of 64 rows.
   const bool few = piece < kManyRows;

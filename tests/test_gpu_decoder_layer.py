@@ -11,6 +11,7 @@ import numpy as np
 import pytest
 import torch
 
+import hxm
 import hxm.ops as ops
 from test_gpu_paged_attention import check as check_attention
 from test_gpu_rope_append import close, rotate64, table as rope_table
@@ -273,3 +274,45 @@ def test_padded_batch(dev):
         res.append([t[:n] for t in (y, z, qkv, q, a)] + [model.cache])
     for one, two in zip(*res):
         assert torch.equal(one.contiguous().view(torch.int16), two.contiguous().view(torch.int16))
+
+
+def test_capture_needs_its_workspace(dev):
+    """Without a call before it, a captured paged_attention or lora_add is refused and the
+    capture goes on; after one, it is recorded, and works when the buffers are new again."""
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(2, HQ, D, generator=g).half().to(dev)
+    kc, vc = (torch.randn(80, HKV, PAGE, D, generator=g).half().to(dev) for _ in range(2))
+    table = torch.randperm(80, generator=g).int().view(2, 40).to(dev)
+    lens = torch.tensor([640, 600], dtype=torch.int32, device=dev)
+    y, x = (torch.randn(300, w, generator=g).half().to(dev) for w in (256, H))
+    A, B = (torch.randn(2, a, b, generator=g).half().to(dev) * 0.1 for a, b in ((R, H), (256, R)))
+    index = (torch.arange(300, device=dev) % 3 - 1).int()
+    calls = [lambda out: ops.paged_attention(q, kc, vc, table, lens, out=out),
+             lambda out: ops.lora_add(y, x, A, B, index, out=out)]
+    outs = [torch.empty_like(q), torch.empty_like(y)]
+    want = [f(None).clone() for f in calls]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert hxm.lib.hxm_release_cache() == 0
+    for f, out in zip(calls, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            with pytest.raises(hxm.HxmError, match="workspace-budget"):
+                f(out)
+            out.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out == 3).all()
+    for f, out, w in zip(calls, outs, want):
+        with torch.cuda.stream(s):
+            f(out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            f(out)
+        for _ in range(3):
+            out.fill_(3)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, w)
