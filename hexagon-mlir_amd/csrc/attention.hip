@@ -13,16 +13,15 @@
 // are in, and running maximum, sum and output of a head live in one column
 // of lanes.
 //
-// Keys and values come in whole rows, 1 KiB of neighbouring bytes an
-// instruction in the order of a page, nontemporal: nothing is read twice.  (Keys
-// loaded in the operand's own layout, 64 bytes of 16 rows an instruction, read
-// every line in two halves, which the caches had to join: 8 x 32768 tokens, 8
-// heads of 128, 98 us and 91 nontemporal, against 88.)  A lane then holds 8
-// tokens x dim / 16 dims of V and transposes them in registers with byte permutes; K
-// becomes the left operand through the wave's own piece of LDS, where row t has its
-// 16-byte chunk q at q ^ t % 16 (of 8 chunks: q ^ t / 2 % 8, two rows to all 64
-// banks), so that neither side meets a bank twice.  The next tile's keys are on their way as soon as this one's are in
-// LDS, its values as soon as this one's are used.
+// Keys and values come in whole rows, 1 KiB of neighbouring bytes an instruction in the
+// order of a page, nontemporal: nothing is read twice.  (Keys loaded in the operand's own
+// layout, 64 bytes of 16 rows an instruction, read every line in two halves, which the
+// caches had to join: 8 x 32768 tokens, 8 heads of 128, 98 us and 91 nontemporal, against
+// 88.)  A lane then holds 8 tokens x dim / 16 dims of V and transposes them in registers
+// with byte permutes; K becomes the left operand through the wave's own piece of LDS, where
+// row t has its 16-byte chunk q at q ^ t % 16 (of 8 chunks: q ^ t / 2 % 8, two rows to all
+// 64 banks), so that neither side meets a bank twice.  The next tile's keys are on their
+// way as soon as this one's are in LDS, its values as soon as this one's are used.
 //
 // The running maximum moves only when a score passes it by more than 2^8 in
 // the exponent's base 2: exp2(s - m) stays far below fp32's limit, and the
@@ -51,11 +50,11 @@ static_assert(kUnit == kAttnUnit, "a unit is one step of all waves");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;  // of the running maximum, in powers of two
 
-// The pieces (kAttnGroups and kAttnFine): one for each CU where the sequences allow it.  What a
-// workgroup has under way (a tile of each wave) keeps its CU at its share of the
+// The pieces (kAttnGroups and kAttnFine): one for each CU where the sequences allow it.
+// What a workgroup has under way (a tile of each wave) keeps its CU at its share of the
 // memory's rate, fewer pieces are fewer to join, and all run at once.  More at once only
-// starve each other: with three workgroups a CU, 8 x 32768 tokens, the first to end took 31 us
-// and the last 79; 32768 tokens of one sequence, 8 heads of 8, 32 us with 256 pieces, 42
+// starve each other: with three workgroups a CU, 8 x 32768 tokens, the first to end took 31
+// us and the last 79; 32768 tokens of one sequence, 8 heads of 8, 32 us with 256 pieces, 42
 // with 768.  Where sequences times heads are more than that, three times as many pieces
 // level what their lengths differ by (16 x 8192 tokens at most, 32 heads: 150 us with 2,
 // 141 with 3, 143 with 4 and more; 64 x 4096, 8 heads: 81.5, 80.7, 80.7).  A join costs
@@ -279,8 +278,8 @@ __global__ __launch_bounds__(kWaves * 64)
 #pragma unroll
       for (int s = 0; s < DT / 128; ++s) {
         const int d = 128 * s + VC * c;
-        const v4u32_t x =
-            __builtin_nontemporal_load(reinterpret_cast<const any4*>(r + (D_FULL || d < D ? d : 0)));
+        const v4u32_t x = __builtin_nontemporal_load(
+            reinterpret_cast<const any4*>(r + (D_FULL || d < D ? d : 0)));
 #pragma unroll
         for (int y = 0; y < 4; ++y) vt[j][4 * s + y] = x[y];
       }

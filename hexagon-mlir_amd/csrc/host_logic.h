@@ -169,15 +169,15 @@ inline FastDiv fast_div(uint32_t d) {
   return FastDiv{static_cast<uint32_t>((p + d - 1) / d), 31 + l};
 }
 
-// How paged attention cuts a batch into pieces, one for a workgroup.  Lengths count
-// in units of kAttnUnit tokens (of the window, from its first tile on; no sequence
-// is 0).  A sequence of up to kAttnWhole units is one piece.  Longer ones are cut
-// into equal pieces of at most `size` units: with share = all units / kAttnGroups,
-// the least of attn_size(share, 0 .. 3) that gives no more than kAttnGroups pieces over all
-// heads; where none does, attn_fine_size(share), which gives at most kAttnFine * kAttnGroups + batch
-// * heads.  Pieces of sequences cut in two or more then number at most 2 * kAttnFine *
-// kAttnGroups: one cut in c has more than (c - 1) * size units, so size * c is
-// less than twice its units.
+// How paged attention cuts a batch into pieces, one for a workgroup.  Lengths count in
+// units of kAttnUnit tokens (of the window, from its first tile on; no sequence is 0).  A
+// sequence of up to kAttnWhole units is one piece.  Longer ones are cut into equal pieces
+// of at most `size` units: with share = all units / kAttnGroups, the least of
+// attn_size(share, 0 .. 3) that gives no more than kAttnGroups pieces over all heads; where
+// none does, attn_fine_size(share), which gives at most kAttnFine * kAttnGroups + batch *
+// heads.  Pieces of sequences cut in two or more then number at most 2 * kAttnFine *
+// kAttnGroups: one cut in c has more than (c - 1) * size units, so size * c is less than
+// twice its units.
 constexpr int64_t kAttnUnit = 128, kAttnTile = 32;
 constexpr uint32_t kAttnGroups = 256, kAttnFine = 3, kAttnWhole = 4, kAttnFineLeast = 8;
 constexpr int64_t kAttnMaxTokens = int64_t(1) << 30;  // of a sequence: 2^23 units

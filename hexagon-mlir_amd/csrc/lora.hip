@@ -11,17 +11,18 @@
 // keeps the results of its own adapter alone (chosen, not multiplied by zero: what
 // another adapter's weights hold does not reach it).
 //
-// Few rows are a matter of latency and of reading many adapters: each adapter of a
-// tile is a workgroup of the first launch and a wave of the second, every load under
-// way at once.  Many rows mostly share one adapter per tile: there a tile is 64 rows, whose waves share
+// Few rows are a matter of latency and of reading many adapters: each adapter of a tile is
+// a workgroup of the first launch and a wave of the second, every load under way at once.
+// Many rows mostly share one adapter per tile: there a tile is 64 rows, whose waves share
 // the adapter's weights through LDS, read in whole rows, and a launch between makes the
 // second operand once.
 //
-// 48 rows of 16 adapters, 4096 -> 4096, R 16: 9.9 us, two launches of 4.7 and 5.4.  2048 rows of 4,
-// 4096 -> 11008, R 64, bf16: 37.5, of them 10 the first launch, 4 the second, and 23 the last,
-// which moves 90 MB of y and out (17 us at a large copy's rate).  With each wave reading its own operands of the
-// weights and of y, 16 rows of 64 bytes an instruction, they were 19, 5 and 39.  2048
-// rows of 16 mixed adapters, 4096 -> 4096, R 16: 52, sixteen turns for each tile.
+// 48 rows of 16 adapters, 4096 -> 4096, R 16: 9.9 us, two launches of 4.7 and 5.4.  2048
+// rows of 4, 4096 -> 11008, R 64, bf16: 37.5, of them 10 the first launch, 4 the second,
+// and 23 the last, which moves 90 MB of y and out (17 us at a large copy's rate).  With
+// each wave reading its own operands of the weights and of y, 16 rows of 64 bytes an
+// instruction, they were 19, 5 and 39.  2048 rows of 16 mixed adapters, 4096 -> 4096, R 16:
+// 52, sixteen turns for each tile.
 //
 // t enters the second product as two 16-bit halves, t = hi + lo: 22 bits of it
 // in f16, 16 in bf16, where one would round t to the weights' 11 or 8.  Rows
@@ -39,8 +40,8 @@ namespace {
 
 constexpr int kRows = 16;   // rows of an MFMA operand
 constexpr int kWaves = 4;
-// Rows from which the form for many is taken (R 16, 4096 -> 4096: 256 rows of 4 adapters 10.8 us
-// with it, 14.0 without; 512 rows of 16 mixed adapters 24.5 and 31).
+// Rows from which the form for many is taken (R 16, 4096 -> 4096: 256 rows of 4 adapters
+// 10.8 us with it, 14.0 without; 512 rows of 16 mixed adapters 24.5 and 31).
 constexpr int64_t kManyRows = 256;
 
 struct LoraArgs {
@@ -246,10 +247,10 @@ __device__ __forceinline__ void load_factors(const LoraArgs& a, int m0, const in
   }
 }
 
-// Many rows: t of 64 rows, a part of K; workgroup (tile, y, part) takes the tile's adapters y,
-// y + ways, .. in the order of their first rows.  A wave's 16 rows of x stay in
-// registers, 256 of K at a time; 16 RT ranks of an adapter's A lie in LDS for all
-// four waves, read in whole rows.
+// Many rows: t of 64 rows, a part of K; workgroup (tile, y, part) takes the tile's adapters
+// y, y + ways, .. in the order of their first rows.  A wave's 16 rows of x stay in
+// registers, 256 of K at a time; 16 RT ranks of an adapter's A lie in LDS for all four
+// waves, read in whole rows.
 constexpr int kManyTile = kRows * kWaves;
 constexpr int kManyK = 256;
 template <typename T, int RT, int NC>
@@ -514,9 +515,11 @@ __global__ __launch_bounds__(kWaves * 64) void lora_expand_few_kernel(LoraArgs a
 // one's on their way during the products), and a row's y takes its sum in place when its
 // adapter's turn comes.
 //
-// Tiles are numbered down the rows and each XCD (workgroups go to them in turn) takes a run of
-// them, so that its L2 holds the columns' weights.
+// Tiles are numbered down the rows and each XCD (workgroups go to them in turn) takes a run
+// of them, so that its L2 holds the columns' weights.
 constexpr int expand_blocks(int ks) { return ks <= 4 ? 4 : 2; }  // of 32 columns each
+// Waves a SIMD that the registers allow without spills (108 of them at R 64: five waves
+// spill some and run 58 us where four run 41).
 constexpr int expand_waves(int ks) { return ks <= 2 ? 4 : ks <= 4 ? 3 : 2; }
 template <typename T, int KS>
 __global__ __launch_bounds__(kWaves * 64)
@@ -561,7 +564,8 @@ __attribute__((amdgpu_waves_per_eu(expand_waves(KS)))) void lora_expand_kernel(L
       st[i] = *reinterpret_cast<const any4*>(B + (inside(i) ? q / ROW * a.R + q % ROW * 8 : 0));
     }
   };
-  // With ways, this workgroup's adapters alone, and the rows of no adapter in the first one.
+  // With ways, this workgroup's adapters alone, and the rows of no adapter in the first
+  // one.
   const int way = blockIdx.y, ways = gridDim.y;
   uint64_t rows = ~0ull;
   if (ways > 1) {
@@ -658,7 +662,9 @@ hxm_status launch_lora(LoraArgs a, hipStream_t stream) {
   hxm_status st = HXM_OK;
   if (a.adapters > 0 && !few) {
     const int64_t tiles = ceil_div(a.M, kManyTile);
-    // Workgroups for the adapters of a tile until there are four for each CU.
+    // A tile's adapters go to workgroups of their own while there are CUs without any
+    // (256 rows of one adapter a tile, R 16: 10.8 us, 13.5 with four a CU, most of which
+    // find no adapter; 256 rows of 16 mixed ones 18.2 and 20.8).
     const dim3 grid(static_cast<unsigned>(tiles),
                     static_cast<unsigned>(std::max<int64_t>(
                         1, std::min<int64_t>(16, 256 / (tiles * a.splits)))),
@@ -703,10 +709,12 @@ hxm_status launch_lora(LoraArgs a, hipStream_t stream) {
       const int64_t groups =                                                                   \
           ceil_div(a.tiles * ceil_div(a.N, 32 * expand_blocks(KS)), 8) * 8;                    \
       if ((st = check_grid("lora expand", groups, kWaves * 64)) != HXM_OK) return st;          \
+      /* Ways until two workgroups a CU (256 rows of 16 mixed adapters 18.2 us, 25.5        */ \
+      /* without). */                                                                          \
       lora_expand_kernel<T, KS>                                                                \
           <<<dim3(static_cast<unsigned>(groups),                                               \
                   static_cast<unsigned>(std::max<int64_t>(                                     \
-                      1, std::min<int64_t>(16, 512 / groups)))),                          \
+                      1, std::min<int64_t>(16, 512 / groups)))),                               \
              kWaves * 64, 0, stream>>>(a);                                                     \
     }                                                                                          \
   } while (0)
@@ -736,7 +744,8 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
                 dtype);
   constexpr int64_t kMax = INT32_MAX / 4, kMaxN = int64_t(1) << 28;
   if (M < 0 || N < 0 || K < 1 || adapters < 0 || R < 1)
-    return fail(HXM_INVALID_ARG, "invalid-argument: lora_add M=%lld N=%lld K=%lld adapters=%lld R=%lld",
+    return fail(HXM_INVALID_ARG,
+                "invalid-argument: lora_add M=%lld N=%lld K=%lld adapters=%lld R=%lld",
                 (long long)M, (long long)N, (long long)K, (long long)adapters, (long long)R);
   if (K % 8 != 0 || R % 8 != 0 || R > 256)
     return fail(HXM_UNSUPPORTED_SHAPE,
@@ -772,7 +781,8 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
       std::min({M, kLoraRows, (kLoraPlaneBytes / (R * 4)) & ~int64_t(15),
                 kManyTile * ((int64_t(1) << 23) / ceil_div(N, 64))});
   // K split until about 512 workgroups, in 8 parts at most, each a step of all its waves
-  // or more; many rows until 256 of 64 rows.
+  // or more; many rows, tiles of 64, in 16 parts (2048 rows, R 64: 21.0 us with 512
+  // workgroups in sight, 22.9 with 256).
   const bool few = piece < kManyRows;
   const int64_t tiles = ceil_div(piece, few ? kRows : kManyTile);
   const int64_t step = few ? 32 * kWaves * shrink_steps(R <= 16 ? 1 : R <= 64 ? 4 : 8) : kManyK;

@@ -47,9 +47,9 @@ struct RowStats {
 
 // Registers: h, x and the fp32 y of VPL vectors a lane.
 //
-// EARLY: weights, biases and gate are loaded with h and x, not where they are used.
-// For calls of one workgroup a CU or fewer, whose time is their chain of loads (1 x 8192
-// bf16, LayerNorms and gate: 7.6 -> 6.6 us; 300 x 1000 f32: 6.1 -> 5.3); the registers it takes
+// EARLY: weights, biases and gate are loaded with h and x, not where they are used. For
+// calls of one workgroup a CU or fewer, whose time is their chain of loads (1 x 8192 bf16,
+// LayerNorms and gate: 7.6 -> 6.6 us; 300 x 1000 f32: 6.1 -> 5.3); the registers it takes
 // cost larger ones more (2048 x 4096 bf16 14.4 -> 16.6), and 16 waves a row have none left.
 template <typename T, int VPL, int S, bool EARLY>
 __global__ __launch_bounds__(row_waves(S) * 64) void residual_norm_kernel(ResidualArgs a) {
@@ -352,7 +352,8 @@ extern "C" hxm_status hxm_residual_norm_rows(
   // 2^40 elements in a row or between rows keep every byte offset below 2^63.
   constexpr int64_t kMax = int64_t(1) << 40;
   if (rows < 0 || cols < 1 || cols > kMax || gate_rows < 0)
-    return fail(HXM_INVALID_ARG, "invalid-argument: residual_norm rows=%lld cols=%lld gate_rows=%lld",
+    return fail(HXM_INVALID_ARG,
+                "invalid-argument: residual_norm rows=%lld cols=%lld gate_rows=%lld",
                 (long long)rows, (long long)cols, (long long)gate_rows);
   if (rows > INT32_MAX)
     return fail(HXM_UNSUPPORTED_SHAPE, "tile-alignment: residual_norm rows=%lld too many",
@@ -366,7 +367,8 @@ extern "C" hxm_status hxm_residual_norm_rows(
   auto bad_ld = [&](int64_t ld) { return ld < cols || ld > kMax; };
   if (bad_ld(ldh) || bad_ld(ldx) || bad_ld(ldy) || (has_z && bad_ld(ldz)) ||
       (gate_rows > 0 && bad_ld(ldg)))
-    return fail(HXM_INVALID_ARG, "invalid-argument: residual_norm leading dimension below cols=%lld",
+    return fail(HXM_INVALID_ARG,
+                "invalid-argument: residual_norm leading dimension below cols=%lld",
                 (long long)cols);
   if (gate_rows > 0 && rows % gate_rows != 0)
     return fail(HXM_INVALID_ARG,
@@ -383,7 +385,8 @@ extern "C" hxm_status hxm_residual_norm_rows(
         const bool same = out[o] == in[i] && (ldo[o] == ldi[i] || rows == 1);
         if (!same && !rows_disjoint(out[o], ldo[o], in[i], ldi[i], rows, cols, eb))
           return fail(HXM_INVALID_ARG,
-                      "invalid-argument: residual_norm an output overlaps an input without being it");
+                      "invalid-argument: residual_norm an output overlaps an input without "
+                      "being it");
       }
     if (has_z && !rows_disjoint(y, ldy, z, ldz, rows, cols, eb))
       return fail(HXM_INVALID_ARG, "invalid-argument: residual_norm y and z overlap");

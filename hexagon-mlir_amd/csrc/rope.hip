@@ -1,14 +1,13 @@
 // Rotary positions and the append to the paged key-value cache, in one launch:
 // q -> rotated q, k -> rotated k in its cache row, v -> its cache row.
 //
-// Bound by memory: every element of q, k and v is read once and written once
-// (8192 tokens, 32 + 8 heads of 128, bf16: 206 MB in 41 us, 5.0 TB/s; a copy of 1 GiB
-// runs at 5.3); a pair takes two products and two fmas.  A group of threads serves one token.
-// A thread keeps one chunk of the rotated dims (eight pairs, or four
-// neighbouring ones) and walks the heads with it, so it loads its cosines and
-// sines once per token and not once per head; the q heads, the k heads and then
-// the v chunks are one sequence of 16-byte loads and stores, at any element
-// address.
+// Bound by memory: every element of q, k and v is read once and written once (8192 tokens,
+// 32 + 8 heads of 128, bf16: 206 MB in 41 us, 5.0 TB/s; a copy of 1 GiB runs at 5.3); a
+// pair takes two products and two fmas.  A group of threads serves one token. A thread
+// keeps one chunk of the rotated dims (eight pairs, or four neighbouring ones) and walks
+// the heads with it, so it loads its cosines and sines once per token and not once per
+// head; the q heads, the k heads and then the v chunks are one sequence of 16-byte loads
+// and stores, at any element address.
 #include "device_util.h"
 #include "hxm_internal.h"
 #include "row_vec.h"

@@ -20,10 +20,11 @@
  *     stream is capturing a HIP graph).  There is no silent fallback: a
  *     refused call computes nothing.
  *   - HIP graphs: the compute entries (matmul, GEMM, GEMV, row ops, the
- *     decoder-layer operators) may be captured; the tuners, the resident-weight cache and hxm_release_cache
- *     allocate or synchronise and may not.  A compute entry that uses the
- *     per-stream workspace (f32 operands, a [K,N] B, a K split, paged
- *     attention, adapters) needs it already large enough: one call of the shape on the stream before the
+ *     decoder-layer operators) may be captured; the tuners, the
+ *     resident-weight cache and hxm_release_cache allocate or synchronise and
+ *     may not.  A compute entry that uses the per-stream workspace (f32
+ *     operands, a [K,N] B, a K split, paged attention, adapters) needs it
+ *     already large enough: one call of the shape on the stream before the
  *     capture grows it (it is kept until hxm_release_cache, also past a later
  *     growth once a graph has captured it).  Such a graph holds the workspace
  *     of the stream it was captured on: it must not run at the same time as
@@ -558,13 +559,13 @@ typedef struct hxm_heads {
  * rotated q[t] (q_heads heads; q.data == q_out.data with equal strides is in
  * place; q_heads 0: keys only); cache row slots[t] = page * page_size + offset
  * receives the rotated k[t] and v[t].  A slot outside [0, pages * page_size),
- * -1 by custom, marks padding: it stores nothing (q is rotated all the same).  The slots of
- * one call must otherwise be distinct (of two tokens in one slot either may
- * end there, element by element).  A position outside [0, max_pos) makes the
+ * -1 by custom, marks padding: it stores nothing (q is rotated all the same).
+ * The slots of one call must otherwise be distinct (of two tokens in one slot
+ * either may end there, element by element).  A position outside [0, max_pos) makes the
  * rotated dims of that token NaN.  cos_sin: fp32 [max_pos, rot_dim]
  * (ld_cos_sin); rot_dim even, 0 to dim (0: an append without rotation,
- * positions and cos_sin unused).  The cache must
- * not overlap the other tensors.  dtype F16 or BF16, one for all. */
+ * positions and cos_sin unused).  The cache must not overlap the other
+ * tensors.  dtype F16 or BF16, one for all. */
 hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q_heads,
                            const hxm_heads* k, const hxm_heads* v, const int32_t* positions,
                            const float* cos_sin, int64_t ld_cos_sin, int64_t max_pos,
@@ -586,9 +587,10 @@ hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q
  * tokens, or n beyond table_pages * page_size or 2^30, makes that sequence's
  * outputs NaN.  dtype F16 or BF16, one for q, cache and out; scores, the softmax's
  * maximum and sum and the output's sum are fp32, the probabilities enter the
- * product with V with 22 bits (f16) or 16 (bf16).  out may be q itself.  A long cache is split over workgroups and
- * joined in a fixed order: results do not depend on how the workgroups are
- * scheduled.  Uses the per-stream workspace. */
+ * product with V with 22 bits (f16) or 16 (bf16).  out may be q itself.  A
+ * long cache is split over workgroups and joined in a fixed order: results do
+ * not depend on how the workgroups are scheduled.  batch * q_heads up to
+ * 2^24.  Uses the per-stream workspace. */
 hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
                                const hxm_kv_cache* cache, const int32_t* block_table,
                                int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
@@ -602,10 +604,11 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * int32 [M]: -1 (any negative) leaves out[m] = y[m]; an index >= adapters makes
  * the row NaN.  Rows of one adapter need not be neighbours, but runs of them
  * are what large calls are fast at.  out may be y itself (same ld); any other
- * overlap of out with y or x is refused.  x A^T accumulates in fp32 and enters the second
- * product with 22 bits (f16) or 16 bits (bf16) of precision; one rounding to dtype.
- * dtype F16 or BF16, one for all; K a multiple of 8, R a multiple of 8 up to
- * 256.  Uses the per-stream workspace. */
+ * overlap of out with y or x is refused (A, B, index and scale must not overlap
+ * it either).  x A^T accumulates in fp32 and enters the second product with 22
+ * bits (f16) or 16 bits (bf16) of precision; one rounding to dtype.  dtype F16
+ * or BF16, one for all; K a multiple of 8, R a multiple of 8 up to 256.  Uses
+ * the per-stream workspace. */
 hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, const void* A,
                         const void* B, int64_t adapters, int64_t R, const int32_t* index,
                         const float* scale, void* out, int64_t ldo, int64_t M, int64_t N,

@@ -68,7 +68,8 @@ RESIDUAL = [
     (dict(ldh=63), INVALID), (dict(ldx=63), INVALID), (dict(ldy=63), INVALID),
     (dict(ldz=63), INVALID), (dict(ldg=63), INVALID), (dict(ldh=(1 << 40) + 1), INVALID),
     (dict(gate_rows=3), INVALID),
-    (dict(y=16 * MB + 2), INVALID), (dict(z=17 * MB - 2), INVALID), (dict(y=23 * MB + 128), INVALID),
+    (dict(y=16 * MB + 2), INVALID), (dict(z=17 * MB - 2), INVALID),
+    (dict(y=23 * MB + 128), INVALID),
     (dict(y=16 * MB, ldy=65), INVALID), (dict(y=23 * MB), INVALID),
 ]
 

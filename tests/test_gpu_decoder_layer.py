@@ -100,7 +100,8 @@ def check_norm(h, x, w, y, z):
     near(y, h + x, c * mag, "y")
     s = h + x
     r = 1 / np.sqrt((s * s).mean(1, keepdims=True) + EPS)
-    err = c * (np.abs(w) * r * mag + np.abs(s * r * w) * r * np.sqrt((mag ** 2).mean(1, keepdims=True)))
+    rms = np.sqrt((mag ** 2).mean(1, keepdims=True))
+    err = c * (np.abs(w) * r * mag + np.abs(s * r * w) * r * rms)
     near(z, s * r * w, err, "z")
 
 
@@ -115,7 +116,8 @@ def check_lora(y, x, A, B, index, alpha, out):
         A64, B64, s = f64(A[a]), f64(B[a]), float(alpha[a])
         t, tm = A64 @ x64[m], np.abs(A64) @ np.abs(x64[m])
         err = ((K + 2 * R + 32) * 2.0 ** -24 * tm + 2.0 ** -21 * np.abs(t).max())
-        near(out[m], y64[m] + s * (B64 @ t), s * (np.abs(B64) @ err) + 2.0 ** -23 * np.abs(y64[m]), m)
+        near(out[m], y64[m] + s * (B64 @ t),
+             s * (np.abs(B64) @ err) + 2.0 ** -23 * np.abs(y64[m]), m)
 
 
 def check_rope(q0, k, v, kc, vc, slots, positions, cos_sin, q):
