@@ -61,9 +61,11 @@ constexpr float kSlack = 8.0f;  // of the running maximum, in powers of two
 // about what three units do, so four units are left whole (1 x 300 tokens, 32 heads: 7.8 us
 // whole, 9.2 in two).
 
-// Waves a SIMD, by the registers of a tile and the output: many short sequences
-// hide each other's start.
-constexpr int attn_waves(int dt) { return dt <= 64 ? 4 : dt <= 128 ? 2 : 1; }
+// Waves a SIMD, by the registers of a tile and the output: many short sequences hide each
+// other's start.  Rows located one by one need a few registers more, and spill with 128.
+constexpr int attn_waves(int dt, bool p8) {
+  return dt <= 64 ? (p8 ? 4 : 3) : dt <= 128 ? 2 : 1;
+}
 
 struct AttnArgs {
   const void* q;
@@ -210,7 +212,7 @@ __device__ __forceinline__ Piece find_piece(const AttnArgs& a, uint32_t u, int l
 // page each, whose number and address the scalar unit works out.
 template <typename T, int DT, bool D_FULL, bool P8>
 __global__ __launch_bounds__(kWaves * 64)
-    __attribute__((amdgpu_waves_per_eu(attn_waves(DT)))) void paged_attention_kernel(AttnArgs a) {
+    __attribute__((amdgpu_waves_per_eu(attn_waves(DT, P8)))) void paged_attention_kernel(AttnArgs a) {
   using F = Frag<T>;
   using V8 = typename F::V;
   constexpr int KK = DT / 32;       // K steps of the first product
