@@ -18,11 +18,12 @@
 // second operand once.
 //
 // 48 rows of 16 adapters, 4096 -> 4096, R 16: 9.9 us, two launches of 4.7 and 5.4.  2048
-// rows of 4, 4096 -> 11008, R 64, bf16: 37.5, of them 10 the first launch, 4 the second,
+// rows of 4, 4096 -> 11008, R 64, bf16: 36.6, of them 10 the first launch, 4 the second,
 // and 23 the last, which moves 90 MB of y and out (17 us at a large copy's rate).  With
 // each wave reading its own operands of the weights and of y, 16 rows of 64 bytes an
 // instruction, they were 19, 5 and 39.  2048 rows of 16 mixed adapters, 4096 -> 4096, R 16:
-// 52, sixteen turns for each tile.
+// 44, sixteen turns for each tile (52 before conversions and selects took two elements
+// each).
 //
 // t enters the second product as two 16-bit halves, t = hi + lo: 22 bits of it
 // in f16, 16 in bf16, where one would round t to the weights' 11 or 8.  Rows
@@ -41,7 +42,7 @@ namespace {
 constexpr int kRows = 16;   // rows of an MFMA operand
 constexpr int kWaves = 4;
 // Rows from which the form for many is taken (R 16, 4096 -> 4096: 256 rows of 4 adapters
-// 10.8 us with it, 14.0 without; 512 rows of 16 mixed adapters 24.5 and 31).
+// 10.8 us with it, 14.0 without; 512 rows of 16 mixed adapters 22.8 and 31).
 constexpr int64_t kManyRows = 256;
 
 struct LoraArgs {
@@ -627,9 +628,13 @@ __attribute__((amdgpu_waves_per_eu(expand_waves(KS)))) void lora_expand_kernel(L
             d[u] = Mma<T>::run(w, f.hi[s], d[u]);
             d[u] = Mma<T>::run(w, f.lo[s], d[u]);
           }
+        typedef float v8f32 __attribute__((ext_vector_type(8)));
+        v8f32 v;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          y[k][e] = hit ? fromf<T>(fmaf(f.factor, d[e / 4][e % 4], tof(y[k][e]))) : y[k][e];
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(f.factor, d[e / 4][e % 4], tof(y[k][e]));
+        // Conversions and selects of two elements each.
+        const v4u32_t sum = __builtin_bit_cast(v4u32_t, __builtin_convertvector(v, RawVec<T>));
+        y[k] = __builtin_bit_cast(RawVec<T>, hit ? sum : __builtin_bit_cast(v4u32_t, y[k]));
       }
     }
   }
