@@ -10,6 +10,7 @@ the GPU; a CPU tensor is an error, never a silent fallback.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Sequence
 
 import torch
@@ -628,9 +629,21 @@ def _ints(t: torch.Tensor, shape, dev: int, name: str) -> int:
     return t.data_ptr()
 
 
-def _stream_on(stream, dev: int) -> int:
-    """_stream for a device known to be the current one."""
-    return _raw_stream(dev) if stream is None and _raw_stream is not None else _stream(stream)
+def _on_stream(op):
+    """An operator whose outputs and contiguous copies belong to the stream it runs on:
+    with ``stream`` given, the whole call is made with that stream the current one."""
+    @functools.wraps(op)
+    def call(*args, stream=None, **kwargs):
+        if stream is None:
+            return op(*args, **kwargs)
+        with torch.cuda.stream(stream):
+            return op(*args, **kwargs)
+    return call
+
+
+def _current_stream(dev: int) -> int:
+    """_stream() for a device known to be the current one."""
+    return _raw_stream(dev) if _raw_stream is not None else _stream()
 
 
 def _row_ld(t: torch.Tensor, rows: int, cols: int) -> int:
@@ -663,6 +676,7 @@ def _row_norm(kind: str, weight, bias, eps: float, dtype: torch.dtype, cols: int
     return ROW_NORM.pack(_NORMS[kind], eps, w_ptr, b_ptr), w, b
 
 
+@_on_stream
 def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
                   post_weight: Optional[torch.Tensor] = None,
                   post_bias: Optional[torch.Tensor] = None, post_eps: float = 1e-6,
@@ -670,7 +684,7 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
                   pre_bias: Optional[torch.Tensor] = None, pre_eps: float = 1e-6,
                   gate: Optional[torch.Tensor] = None, block_scale: float = 1.0,
                   residual_scale: float = 1.0, out: Optional[torch.Tensor] = None,
-                  normed_out: Optional[torch.Tensor] = None, stream=None):
+                  normed_out: Optional[torch.Tensor] = None):
     """The norms around a block fused with its gate and the residual
     (hxm_residual_norm_rows): returns (y, z),
 
@@ -719,7 +733,7 @@ def residual_norm(h: torch.Tensor, x: torch.Tensor, *, post: str = "none",
                                     _row_ld(x2, rows, cols), post_n, gate_ptr, ldg, G,
                                     block_scale, residual_scale, pre_n, y2.data_ptr(),
                                     _row_ld(y2, rows, cols), z_ptr, ldz, rows, cols, _DT[dtype],
-                                    _stream_on(stream, dev))
+                                    _current_stream(dev))
     if st:
         check(st, "hxm_residual_norm_rows")
     return y, z
@@ -758,11 +772,12 @@ def _kv_cache(k: torch.Tensor, v: torch.Tensor):
                           vt), heads, dim, dtype, dev)
 
 
+@_on_stream
 def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
                 k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
                 positions: Optional[torch.Tensor] = None,
                 cos_sin: Optional[torch.Tensor] = None, *, interleaved: bool = False,
-                q_out: Optional[torch.Tensor] = None, stream=None) -> Optional[torch.Tensor]:
+                q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Rotary positions and the append to a paged cache in one launch
     (hxm_rope_append): returns the rotated q and stores the rotated k and v.
 
@@ -807,16 +822,17 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         raise ValueError("q_out needs q")
     st = lib.hxm_rope_append(qh, oh, hq, kh, vh, pos_p, tab_p, ld, max_pos, rot,
                              int(interleaved), slot_p, cache, T, _DT[dtype],
-                             _stream_on(stream, dev))
+                             _current_stream(dev))
     if st:
         check(st, "hxm_rope_append")
     return q_out
 
 
+@_on_stream
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     block_table: torch.Tensor, seq_lens: torch.Tensor, *,
                     scale: Optional[float] = None, window: int = 0,
-                    out: Optional[torch.Tensor] = None, return_lse: bool = False, stream=None):
+                    out: Optional[torch.Tensor] = None, return_lse: bool = False):
     """Attention of one new token per sequence over a paged cache
     (hxm_paged_attention): q [B, Hq, D] f16 / bf16 against the caches [pages,
     Hkv, page_size, D] (any strides; Hq a multiple of Hkv).  ``block_table``
@@ -847,15 +863,16 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         lse_p = lse.data_ptr()
     st = lib.hxm_paged_attention(qh, oh, hq, cache, block_table.data_ptr(), _ld(block_table),
                                  table_pages, lens_p, B, dim ** -0.5 if scale is None else scale,
-                                 window, lse_p, _DT[dtype], _stream_on(stream, dev))
+                                 window, lse_p, _DT[dtype], _current_stream(dev))
     if st:
         check(st, "hxm_paged_attention")
     return (out, lse) if return_lse else out
 
 
+@_on_stream
 def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
              index: torch.Tensor, scale: Optional[torch.Tensor] = None,
-             out: Optional[torch.Tensor] = None, *, stream=None) -> torch.Tensor:
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Low-rank adapters of many requests beside a projection they share
     (hxm_lora_add): out[m] = y[m] + scale[a] * (x[m] @ A[a].T) @ B[a].T with
     a = ``index``[m] (int32 [M]; -1: out[m] = y[m]).
@@ -887,7 +904,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
         _out(out, (M, N), (dtype,), y)
     st = lib.hxm_lora_add(y.data_ptr(), _row_ld(y, M, N), x.data_ptr(), _row_ld(x, M, K),
                           A.data_ptr(), B.data_ptr(), L, R, index_p, scale_p, out.data_ptr(),
-                          _row_ld(out, M, N), M, N, K, _DT[dtype], _stream_on(stream, dev))
+                          _row_ld(out, M, N), M, N, K, _DT[dtype], _current_stream(dev))
     if st:
         check(st, "hxm_lora_add")
     return out

@@ -318,3 +318,70 @@ def test_capture_needs_its_workspace(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, w)
+
+
+def test_stream_argument(dev):
+    """With stream=, copies of parameters that are not contiguous and new outputs belong to that
+    stream: a call does not wait for, nor race with, what the current stream still does."""
+    g = torch.Generator().manual_seed(11)
+    wide = torch.randn(H, 2, generator=g).half().to(dev)
+    h, x = (torch.randn(40, H, generator=g).half().to(dev) for _ in range(2))
+    q = torch.randn(2, HQ, D, generator=g).half().to(dev)
+    kc, vc = (torch.randn(8, HKV, PAGE, D, generator=g).half().to(dev) for _ in range(2))
+    table = torch.arange(8, dtype=torch.int32, device=dev).view(2, 4)
+    lens = torch.tensor([60, 33], dtype=torch.int32, device=dev)
+    none = torch.full_like(lens, -1)
+    A, B = (torch.randn(2, a, b, generator=g).half().to(dev) * 0.1 for a, b in ((R, H), (H, R)))
+    scale = torch.rand(2, 3, generator=g).to(dev)[:, 1]
+    index = (torch.arange(40, device=dev) % 3 - 1).int()
+    calls = [lambda s: ops.residual_norm(h, x, pre_weight=wide[:, 1], post="rms",
+                                         post_weight=wide[:, 0], gate=wide.t(), stream=s)[1],
+             lambda s: ops.rope_append(q, kc[:2, :, 0], vc[:2, :, 0], kc, vc,
+                                       none, stream=s),
+             lambda s: ops.paged_attention(q, kc, vc, table, lens, stream=s),
+             lambda s: ops.lora_add(h, x, A, B, index, scale, stream=s)]
+    want = [f(None).clone() for f in calls]
+    s = torch.cuda.Stream()
+    big = torch.randn(4096, 4096, device=dev)
+    for f, w in zip(calls, want):
+        f(s)                                     # workspaces, before the current stream is busy
+        torch.cuda.synchronize()
+        for _ in range(20):
+            big @ big
+        with torch.cuda.stream(s):
+            same = torch.equal(f(s), w)          # waits for s alone
+        assert same
+        torch.cuda.synchronize()
+
+
+def test_host_threads(dev):
+    """Four host threads, each with a stream, a model and a batch of its own, give what one
+    thread gives."""
+    import threading
+
+    def loop(seed, stream):
+        lens = [90 + 7 * seed, 0, 300 - 40 * seed, 1]
+        with torch.cuda.stream(stream):
+            model, batch = Model(dev, seed=seed), Batch(dev, lens, seed=seed)
+            prefill(model, batch, lens, 1, seed=seed)
+            g = torch.Generator().manual_seed(seed)
+            outs = [model.step(torch.randn(len(lens), H, generator=g).half().to(dev), batch.index,
+                               *batch.advance()) for _ in range(5)]
+            stream.synchronize()
+        return outs
+
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    want = [loop(i, streams[0]) for i in range(4)]
+    got = [None] * 4
+
+    def run(i):
+        torch.cuda.set_device(0)
+        got[i] = loop(i, streams[i])
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert a is not None and all(torch.equal(x, y) for x, y in zip(a, b))
