@@ -58,9 +58,8 @@ struct LoraArgs {
   const float* scale;
   int64_t ldy, ldx, ldo, K, N;
   int M, R, adapters, splits;
-  int tiles;        // of rows, of the second launch
+  int tiles;        // of 64 rows, of the last launch
   int k_per_split;  // a multiple of what a workgroup's waves take together
-  int n_per_group;  // columns of a workgroup of the second launch
 };
 
 template <typename T>
@@ -791,7 +790,7 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
   const bool few = piece < kManyRows;
   const int64_t tiles = ceil_div(piece, few ? kRows : kManyTile);
   const int64_t step = few ? 32 * kWaves * shrink_steps(R <= 16 ? 1 : R <= 64 ? 4 : 8) : kManyK;
-  const int64_t splits = std::min(std::min<int64_t>(few ? 8 : 16, ceil_div(few ? 512 : 512, tiles)),
+  const int64_t splits = std::min(std::min<int64_t>(few ? 8 : 16, ceil_div(512, tiles)),
                                   ceil_div(K, step));
   a.k_per_split = static_cast<int>(ceil_div(ceil_div(K, splits), step) * step);
   a.splits = static_cast<int>(ceil_div(K, a.k_per_split));

@@ -132,6 +132,30 @@ def test_bad_indexes_and_sick_weights_of_many_rows(dev):
             assert torch.equal(out[m], want[m]), m
 
 
+def test_rows_beyond_one_set_of_launches(dev):
+    """65536 rows of rank 256 fill one set's planes: the next set starts at row 65536, and takes
+    the form for few rows where 100 are left."""
+    R, K, N, L = 256, 16, 24, 3
+    for M in (65536 + 100, 65536 + 300):
+        g = torch.Generator().manual_seed(M)
+        x, y = (torch.randn(M, w, generator=g).half().to(dev) for w in (K, N))
+        A, B = (torch.randn(L, a, b, generator=g).half().to(dev) / 16 for a, b in ((R, K), (N, R)))
+        index = (torch.arange(M, device=dev) // 1000 % (L + 1) - 1).int()
+        out = ops.lora_add(y, x, A, B, index)
+        for a in range(-1, L):
+            rows = index == a
+            want = y[rows].double()
+            err = torch.zeros_like(want)
+            if a >= 0:
+                t = x[rows].double() @ A[a].double().t()
+                tm = x[rows].double().abs() @ A[a].double().abs().t()
+                want = want + t @ B[a].double().t()
+                e = (K + 2 * R + 32) * 2.0 ** -24 * tm + HALVES["f16"] * t.abs().amax(1, True)
+                err = e @ B[a].double().abs().t() + 2.0 ** -23 * y[rows].double().abs()
+            tol = 2.0 ** -11 * (want.abs() + err) + 2.0 ** -25 + err
+            assert ((out[rows].double() - want).abs() <= (tol if a >= 0 else 0)).all(), (M, a)
+
+
 def test_many_rows_captured_after_other_sizes(dev):
     """One stream's workspace under calls of changing sizes, then a captured one."""
     g = torch.Generator().manual_seed(8)
