@@ -150,8 +150,9 @@ struct Piece {
 };
 
 // Piece u of the batch, its sequences in order, cut as host_logic.h says.  Every wave
-// works it out from the lengths, 64 sequences at a time: they are on the device, so
-// the host cannot.  Batches of more than 64 take the fine pieces without trying the others.
+// works it out from the lengths, 64 sequences at a time, all loaded at once: they are on
+// the device, so the host cannot.  Batches of more than 64 take the fine pieces without
+// trying the others.
 __device__ __forceinline__ Piece find_piece(const AttnArgs& a, uint32_t u, int lane) {
   auto tokens = [&](int32_t len, int* lo) {
     const int n = len > a.capacity ? 0 : max(len, 0);
@@ -164,34 +165,48 @@ __device__ __forceinline__ Piece find_piece(const AttnArgs& a, uint32_t u, int l
     return b < a.batch ? attn_units(n, lo) : 0u;
   };
   auto length = [&](int b) { return b < a.batch ? a.lens[b] : 0; };
-  const int32_t len0 = length(lane);
-  const uint32_t w0 = units(lane, len0);
-  uint64_t total = wave_sum(w0);
-  for (int b = 64; b < a.batch; b += 64) total += wave_sum(units(b + lane, length(b + lane)));
+  Piece r{};
+  r.b = -1;
+  if (a.batch > kAttnCutBatch) {  // a whole sequence each
+    if (u >= static_cast<uint32_t>(a.batch)) return r;
+    const int32_t len = a.lens[u];
+    r.b = static_cast<int>(u), r.n = tokens(len, &r.lo), r.over = len > a.capacity;
+    r.pieces = 1, r.begin = r.lo & ~(kTile - 1), r.end = r.n;
+    return r;
+  }
+  constexpr int CHUNKS = kAttnCutBatch / 64;
+  int32_t len[CHUNKS];
+  uint32_t w[CHUNKS];
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) len[i] = 64 * i < a.batch ? length(64 * i + lane) : 0;
+  uint64_t total = 0;
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    w[i] = units(64 * i + lane, len[i]);
+    if (64 * i < a.batch) total += wave_sum(w[i]);
+  }
   const uint32_t share = attn_share(total, a.heads);
   uint32_t size = 0;
   bool fits = false;
   if (a.batch <= 64)
     for (uint32_t k = 0; k < 4 && !fits; ++k) {
       size = attn_size(share, k);
-      fits = wave_sum(attn_cut(w0, size)) * a.heads <= kAttnGroups;
+      fits = wave_sum(attn_cut(w[0], size)) * a.heads <= kAttnGroups;
     }
   if (!fits) size = attn_fine_size(share);
-  Piece r{};
-  r.b = -1;
   uint32_t first = 0, slots = 0;  // pieces, and partial slots, of the sequences before
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int32_t len = b0 == 0 ? len0 : length(b0 + lane);
-    const uint32_t w = units(b0 + lane, len);
-    const uint32_t c = attn_cut(w, size), cs = c > 1 ? c : 0u;
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    if (64 * i >= a.batch) break;
+    const uint32_t c = attn_cut(w[i], size), cs = c > 1 ? c : 0u;
     const uint32_t upto = wave_scan(c, lane), upto_s = wave_scan(cs, lane);
     const uint64_t hit = __ballot(u < first + upto);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      const int32_t len_l = static_cast<int32_t>(lane_u32(static_cast<uint32_t>(len), l));
+      const int32_t len_l = static_cast<int32_t>(lane_u32(static_cast<uint32_t>(len[i]), l));
       const uint32_t pieces = lane_u32(c, l);
-      const int step = static_cast<int>((lane_u32(w, l) + pieces - 1) / pieces) * kUnit;
-      r.b = b0 + l;
+      const int step = static_cast<int>((lane_u32(w[i], l) + pieces - 1) / pieces) * kUnit;
+      r.b = 64 * i + l;
       r.n = tokens(len_l, &r.lo);
       r.over = len_l > a.capacity;
       r.pieces = static_cast<int>(pieces);
@@ -624,7 +639,7 @@ __global__ __launch_bounds__(kWaves * 64)
 
 template <typename T, int DT>
 hxm_status launch_attention(const AttnArgs& a, hipStream_t stream) {
-  const int64_t groups = attn_grid(static_cast<int64_t>(a.batch) * a.heads, a.capacity);
+  const int64_t groups = attn_grid(a.batch, a.heads, a.capacity);
   hxm_status st = check_grid("paged attention", groups, kWaves * 64);
   if (st != HXM_OK) return st;
   const unsigned n = static_cast<unsigned>(groups);

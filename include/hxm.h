@@ -588,9 +588,9 @@ hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q
  * outputs NaN.  dtype F16 or BF16, one for q, cache and out; scores, the softmax's
  * maximum and sum and the output's sum are fp32, the probabilities enter the
  * product with V with 22 bits (f16) or 16 (bf16).  out may be q itself.  A
- * long cache is split over workgroups and joined in a fixed order: results do
- * not depend on how the workgroups are scheduled.  batch * q_heads up to
- * 2^24.  Uses the per-stream workspace. */
+ * long cache is split over workgroups (in batches of up to 256 sequences) and
+ * joined in a fixed order: results do not depend on how the workgroups are
+ * scheduled.  batch * q_heads up to 2^24.  Uses the per-stream workspace. */
 hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
                                const hxm_kv_cache* cache, const int32_t* block_table,
                                int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,

@@ -122,7 +122,12 @@ static void check_cut(const std::vector<int32_t>& lens, int64_t heads, int32_t w
     lo[b] = window > 0 ? std::max(0, n[b] - window) : 0;
     w[b] = hxm::attn_units(n[b], lo[b]);
     total += w[b];
-    CHECK(total < (uint64_t(1) << 32) || batch > 512, "units of 64 sequences pass 32 bits");
+    CHECK(total < (uint64_t(1) << 32) || batch > 256, "units of 64 sequences pass 32 bits");
+  }
+  const int64_t grid = hxm::attn_grid(static_cast<int64_t>(batch), heads, capacity);
+  if (static_cast<int64_t>(batch) > hxm::kAttnCutBatch) {  // a sequence a piece
+    CHECK(grid == static_cast<int64_t>(batch) * heads, "grid of a batch that is not cut");
+    return;
   }
   const uint32_t share = hxm::attn_share(total, heads);
   uint32_t size = 0;
@@ -139,7 +144,6 @@ static void check_cut(const std::vector<int32_t>& lens, int64_t heads, int32_t w
     }
   if (!fits) size = hxm::attn_fine_size(share);
   const uint64_t pieces = pieces_of();
-  const int64_t grid = hxm::attn_grid(static_cast<int64_t>(batch) * heads, capacity);
   CHECK(static_cast<int64_t>(pieces * heads) <= grid, "%llu pieces of %lld heads, grid %lld",
         (unsigned long long)pieces, (long long)heads, (long long)grid);
   uint64_t slots = 0;
@@ -168,7 +172,7 @@ static void check_attention() {
   for (int64_t heads : {1, 2, 3, 8, 32, 64, 128, 255, 256, 257, 1000, 65535}) {
     for (int32_t len : {0, 1, 31, 32, 33, 127, 128, 129, 512, 513, 640, 1024, 4096, 32768, 1 << 20,
                         1 << 30})
-      for (int64_t batch : {1, 2, 7, 63, 64, 65, 130}) {
+      for (int64_t batch : {1, 2, 7, 63, 64, 65, 130, 255, 256, 257}) {
         if (batch * heads > (1 << 24)) continue;
         check_cut(std::vector<int32_t>(batch, len), heads, 0, len > 0 ? len : 32);
         check_cut(std::vector<int32_t>(batch, len), heads, 1000, int64_t(1) << 30);
@@ -177,10 +181,10 @@ static void check_attention() {
         check_cut(one, heads, 0, int64_t(1) << 30);
       }
   }
-  check_cut(std::vector<int32_t>(1 << 16, 1 << 12), 256, 0, 1 << 12);
-  check_cut(std::vector<int32_t>(1 << 14, 1 << 30), 1024, 0, int64_t(1) << 30);
+  check_cut(std::vector<int32_t>(256, 1 << 12), 65535, 0, 1 << 12);
+  check_cut(std::vector<int32_t>(256, 1 << 30), 65535, 0, int64_t(1) << 30);
   for (int i = 0; i < 4000; ++i) {
-    const int64_t batch = pick(1, pick(0, 3) ? 80 : 400), heads = pick(1, pick(0, 1) ? 16 : 200);
+    const int64_t batch = pick(1, pick(0, 3) ? 80 : 300), heads = pick(1, pick(0, 1) ? 16 : 200);
     const int64_t top = int64_t(1) << pick(0, pick(0, 3) ? 15 : 30);
     std::vector<int32_t> lens(batch);
     const bool skew = pick(0, 1);

@@ -135,7 +135,7 @@ def test_long(dev, name, lens):
     run_case(dev, name, lens, 4, 2, 64, 128, "hnd", window=1500)
 
 
-@pytest.mark.parametrize("batch", [63, 64, 65, 128, 200, 513])
+@pytest.mark.parametrize("batch", [63, 64, 65, 128, 200, 255, 256, 257, 513])
 def test_many_sequences(dev, batch):
     """Batches in and past one wave's lanes, of one long sequence among short ones, all
     alike, and with rows of padding (no tokens) at the end."""
