@@ -520,7 +520,8 @@ typedef struct hxm_row_norm {
  * pre->kind HXM_NORM_NONE, z is not computed (z NULL).  y or z may be h or x
  * itself (same pointer and ld); any other overlap of an output with h, x or
  * the other output is refused (gamma, beta and gate must not overlap the
- * outputs either).  rows up to 2^31 - 1. */
+ * outputs either).  rows: as many as a launch holds, 2^26 of up to 64 vectors
+ * of 16 bytes, fewer of longer ones. */
 hxm_status hxm_residual_norm_rows(const void* h, int64_t ldh, const void* x, int64_t ldx,
                                   const hxm_row_norm* post, const void* gate, int64_t ldg,
                                   int64_t gate_rows, float block_scale, float residual_scale,
