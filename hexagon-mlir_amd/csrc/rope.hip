@@ -2,7 +2,7 @@
 // q -> rotated q, k -> rotated k in its cache row, v -> its cache row.
 //
 // Bound by memory: every element of q, k and v is read once and written once (8192 tokens,
-// 32 + 8 heads of 128, bf16: 206 MB in 41 us, 5.0 TB/s; a copy of 1 GiB runs at 5.3); a
+// 32 + 8 heads of 128, bf16: 206 MB in 40 us, 5.1 TB/s; a copy of 1 GiB runs at 5.3); a
 // pair takes two products and two fmas.  A group of threads serves one token. A thread
 // keeps one chunk of the rotated dims (eight pairs, or four neighbouring ones) and walks
 // the heads with it, so it loads its cosines and sines once per token and not once per
@@ -42,10 +42,14 @@ template <typename T>
 __device__ __forceinline__ RawVec<T> load_n(const T* p, int n) {
   return n == kChunk ? load_any(p) : load_tail(p, 0, n, T(0));
 }
-template <typename T>
+// Rows of the cache go past the caches, which then keep the inputs of large calls (8192
+// tokens, 32 + 8 heads of 128: 41.2 -> 40.4 us; 16 + 16 heads of 64: 26.2 -> 20.9; 1024
+// tokens 7.2 -> 6.9); q stays in them for the attention that follows (nontemporal too,
+// 42.2, 25.6 and 5.9).
+template <bool CACHED, typename T>
 __device__ __forceinline__ void store_n(T* p, RawVec<T> v, int n) {
-  // Plain stores: the attention that follows reads both.
-  if (n == kChunk) *reinterpret_cast<AnyVec<T>*>(p) = v;
+  if (n == kChunk && !CACHED) store_any(p, v);
+  else if (n == kChunk) *reinterpret_cast<AnyVec<T>*>(p) = v;
   else store_tail(p, 0, n, v);
 }
 // n of M floats (M a multiple of 4, n at least 1), the rest unspecified.
@@ -122,10 +126,12 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
             x[e] = fromf<T>(fmaf(u, cs[e], -(w * sn[e])));
             y[e] = fromf<T>(fmaf(w, cs[e], u * sn[e]));
           }
-          store_n(dst + lo + half, y, n);
+          if (isq) store_n<true>(dst + lo + half, y, n);
+          else store_n<false>(dst + lo + half, y, n);
         }
       }
-      store_n(dst + lo, x, n);
+      if (isq) store_n<true>(dst + lo, x, n);
+      else store_n<false>(dst + lo, x, n);
     }
   }
   if (!stored) return;
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
   for (int j = i; j < a.hkv * vch; j += a.tt) {
     const int hv = j / vch, d = (j - hv * vch) * kChunk;
     const T* src = static_cast<const T*>(a.v.p) + t * a.v.ts + hv * a.v.hs + d;
-    store_n(vc + hv * a.vhs + d, load_any(src), kChunk);
+    store_n<false>(vc + hv * a.vhs + d, load_any(src), kChunk);
   }
 }
 
