@@ -19,7 +19,7 @@
 //
 // 48 rows of 16 adapters, 4096 -> 4096, R 16: 9.9 us, two launches of 4.7 and 5.4.  2048
 // rows of 4, 4096 -> 11008, R 64, bf16: 36.6, of them 10 the first launch, 4 the second,
-// and 23 the last, which moves 90 MB of y and out (17 us at a large copy's rate).  With
+// and 22 the last, which moves 90 MB of y and out (17 us at a large copy's rate).  With
 // each wave reading its own operands of the weights and of y, 16 rows of 64 bytes an
 // instruction, they were 19, 5 and 39.  2048 rows of 16 mixed adapters, 4096 -> 4096, R 16:
 // 44, sixteen turns for each tile (52 before conversions and selects took two elements

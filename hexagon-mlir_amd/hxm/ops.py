@@ -859,7 +859,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lens_p = _ints(seq_lens, (B,), dev, "seq_lens")
     lse = lse_p = None
     if return_lse:
-        lse = torch.empty((B, hq), dtype=torch.float32, device=q.device)
+        lse = torch.empty(B, hq, dtype=torch.float32, device=q.device)
         lse_p = lse.data_ptr()
     st = lib.hxm_paged_attention(qh, oh, hq, cache, block_table.data_ptr(), _ld(block_table),
                                  table_pages, lens_p, B, dim ** -0.5 if scale is None else scale,
