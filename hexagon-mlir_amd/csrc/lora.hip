@@ -27,9 +27,13 @@
 //
 // t enters the second product as two 16-bit halves, t = hi + lo: 22 bits of it
 // in f16, 16 in bf16, where one would round t to the weights' 11 or 8.  Rows
-// are scaled by a power of two first, so that no t over- or underflows in f16; it
-// comes back in fp32 with the adapter's scale.
+// are scaled by a power of two first, which comes back in fp32 with the adapter's scale: in
+// f16 the largest |t| goes to [2^14, 2^15), as high as it can, so that the smallest lo,
+// 2^-24, is 2^-38 of it or less (22 bits of a rank down to 2^-17 of the row's largest; with the
+// largest in [1/2, 1) lo was subnormal for nearly all of them, and a rank 2^-20 of the largest
+// kept 5 bits).  bf16 has fp32's exponents and needs no room.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_util.h"
 #include "hxm_internal.h"
@@ -161,10 +165,12 @@ __global__ __launch_bounds__(kWaves * 64) void lora_shrink_kernel(LoraArgs a) {
   }
 }
 
-// 2^-ex takes a row's largest |t|, top, to [1/2, 1); 0, infinities and NaN stay as
-// they are.
+// 2^-ex takes a row's largest |t|, top, to [2^14, 2^15) in f16 (hi of at most 2^15 stays
+// finite) and to [1/2, 1) in bf16; 0, infinities and NaN stay as they are.
+template <typename T>
 __device__ __forceinline__ int row_exponent(float top) {
-  return top > 0.0f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) : 0;
+  constexpr int kUp = std::is_same<T, _Float16>::value ? 15 : 0;
+  return top > 0.0f && top < __builtin_huge_valf() ? __builtin_amdgcn_frexp_expf(top) - kUp : 0;
 }
 template <typename T>
 __device__ __forceinline__ void split_halves(float v, T* hi, T* lo) {
@@ -233,7 +239,7 @@ __device__ __forceinline__ void load_factors(const LoraArgs& a, int m0, const in
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(t[w][s][e]));
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const int ex = row_exponent(top);
+    const int ex = row_exponent<T>(top);
     f[w].factor =
         live[w] ? __builtin_amdgcn_ldexpf(a.scale ? a.scale[id[w]] : 1.0f, ex) : 0.0f;
 #pragma unroll
@@ -371,7 +377,7 @@ __global__ __launch_bounds__(256) void lora_halves_kernel(LoraArgs a) {
 #pragma unroll
   for (int i = LANES / 2; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i, 64));
   if (!in) return;
-  const int ex = row_exponent(top);
+  const int ex = row_exponent<T>(top);
   typedef T half4 __attribute__((ext_vector_type(4)));
   half4 hi, lo;
 #pragma unroll

@@ -607,9 +607,10 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * are what large calls are fast at.  out may be y itself (same ld); any other
  * overlap of out with y or x is refused (A, B, index and scale must not overlap
  * it either).  x A^T accumulates in fp32 and enters the second product with 22
- * bits (f16) or 16 bits (bf16) of precision; one rounding to dtype.  dtype F16
- * or BF16, one for all; K a multiple of 8, R a multiple of 8 up to 256.  Uses
- * the per-stream workspace. */
+ * bits (f16; a rank below 2^-17 of its row's largest to 2^-39 of that) or 16
+ * bits (bf16) of precision; one rounding to dtype.  dtype F16 or BF16, one for
+ * all; K a multiple of 8, R a multiple of 8 up to 256.  Uses the per-stream
+ * workspace. */
 hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, const void* A,
                         const void* B, int64_t adapters, int64_t R, const int32_t* index,
                         const float* scale, void* out, int64_t ldo, int64_t M, int64_t N,

@@ -293,3 +293,37 @@ def test_refusals(dev):
     with pytest.raises(hxm.HxmError, match="overlaps"):
         ops.lora_add(**{**ok, "x": big[:4], "out": big[:4, :48]})
     assert ops.lora_add(mk(0, 48), mk(0, 64), ok["A"], ok["B"], ok["index"][:0]).shape == (0, 48)
+
+
+# What a rank is off by as two halves of a row scaled to [2^14, 2^15): two roundings of the
+# dtype, and in f16 half of the smallest subnormal, 2^-25, at least 2^14 below the largest.
+SPLIT = {"f16": (2.0 ** -21, 2.0 ** -39), "bf16": (2.0 ** -15, 0.0)}
+
+
+@pytest.mark.parametrize("M", [5, 300])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_ranks_far_apart(dev, name, M):
+    """t falls by 2^20 from a row's first rank to its last while B grows by as much, so that
+    every rank adds about the same to the output: each keeps its own precision."""
+    R, N, L = 16, 200, 2
+    K = 8 * R
+    g = torch.Generator().manual_seed(M)
+    dt, t = TDT[name], torch.finfo(TDT[name])
+    e = 20.0 * torch.arange(R) / (R - 1)
+    x = (torch.randn(M, R, 8, generator=g) * 2.0 ** (-e / 2)[:, None]).reshape(M, K).to(dt)
+    A = torch.zeros(L, R, R, 8)                       # rank r reads its own eight columns
+    A[:, range(R), range(R)] = torch.randn(L, R, 8, generator=g) * 2.0 ** (-e / 2)[:, None]
+    A = A.view(L, R, K).to(dt)
+    B = (torch.randn(L, N, R, generator=g) * 2.0 ** (e - 10)).to(dt)
+    index = torch.arange(M, dtype=torch.int32) % L
+    out = ops.lora_add(torch.zeros(M, N, dtype=dt, device=dev), x.to(dev), A.to(dev), B.to(dev),
+                       index.to(dev)).double().cpu().numpy()
+    half, floor = SPLIT[name]
+    for m, a in enumerate(index.tolist()):
+        A64, B64, x64 = (v.double().numpy() for v in (A[a], B[a], x[m]))
+        tt, tm = A64 @ x64, np.abs(A64) @ np.abs(x64)
+        want = B64 @ tt
+        err = (K + 2 * R + 32) * 2.0 ** -24 * tm + half * np.abs(tt) + floor * np.abs(tt).max()
+        tol = t.eps / 2 * np.abs(want) + t.smallest_normal * t.eps / 2 + np.abs(B64) @ err
+        bad = ~(np.abs(out[m] - want) <= tol)
+        assert not bad.any(), (m, np.argwhere(bad)[:4].tolist(), out[m][bad][:4], want[bad][:4])
