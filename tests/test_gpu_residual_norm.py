@@ -214,3 +214,17 @@ def test_refusals(dev):
     wide = torch.zeros(6, 64, dtype=torch.float16, device=dev)
     y, z = ops.residual_norm(h, wide[:, :32], out=wide[:, 32:])      # other columns: disjoint
     assert y.data_ptr() == wide.data_ptr() + 64
+
+
+@pytest.mark.parametrize("cols,rows", [(300, 1028), (1000, 1028), (1536, 1028), (2043, 1028),
+                                       (4096, 260), (6100, 260), (8192, 260), (12000, 260),
+                                       (16384, 260)])
+@pytest.mark.parametrize("name", ["f16", "bf16", "f32"])
+def test_more_than_a_workgroup_a_cu(dev, name, cols, rows):
+    """Past 256 workgroups parameters are loaded where they are used: every width that takes
+    a row in registers of 1, 4 or 8 waves, at the last row count before the change and past it."""
+    cols = max(1, cols // 2) if name == "f32" else cols
+    run_case(dev, name, rows, cols, "rms", "layer", 4)
+    run_case(dev, name, rows, cols, "layer", "rms", 1, alias="y=x")
+    run_case(dev, name, rows - 4, cols, "none", "rms", rows - 4, bias=False, alias="y=h z=x")
+    run_case(dev, name, rows - 3, cols, "layer", "none", 0)
