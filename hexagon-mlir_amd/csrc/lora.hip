@@ -94,74 +94,74 @@ __device__ __forceinline__ int row_adapter(const LoraArgs& a, int m) {
 constexpr int shrink_steps(int rt) { return rt <= 1 ? 8 : rt <= 4 ? 4 : 2; }
 
 // t of 16 rows, RT * 16 ranks, a part of K.  Workgroup (tile, y, ranks and part) takes the
-// tile's adapters y, y + ways, .. in the order of their first rows; its waves
-// take steps of K in turn and are summed in order.
+// tile's adapter y in the order of their first rows (a tile has no more of them than rows, nor
+// the grid fewer); its waves take steps of K in turn and are summed in order.
 template <typename T, int RT>
 __global__ __launch_bounds__(kWaves * 64) void lora_shrink_kernel(LoraArgs a) {
   using V = typename Mma<T>::V;
   constexpr int U = shrink_steps(RT);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-  const int m0 = blockIdx.x * kRows, ways = gridDim.y;
+  const int m0 = blockIdx.x * kRows;
   const int split = blockIdx.z % a.splits, r0 = blockIdx.z / a.splits * (RT * 16);
   const int mine = row_adapter(a, m0 + c);
-  const bool live = static_cast<uint32_t>(mine) < static_cast<uint32_t>(a.adapters);
+  uint64_t todo = __ballot(static_cast<uint32_t>(mine) < static_cast<uint32_t>(a.adapters)) &
+                  0xffffull;
+  int row0 = 0, id = -1;
+  uint64_t same = 0;
+  for (int y = 0; todo && y <= static_cast<int>(blockIdx.y); ++y) {
+    row0 = __builtin_ctzll(todo);
+    id = __builtin_amdgcn_readlane(mine, row0);
+    same = __ballot(mine == id);
+    todo &= ~same;
+    if (y < static_cast<int>(blockIdx.y)) same = 0;
+  }
+  if (!same) return;
   const int64_t k_begin = static_cast<int64_t>(split) * a.k_per_split;
   const int64_t k_end = min(a.K, k_begin + a.k_per_split);
   __shared__ __align__(16) float sum[kWaves][RT * 16][kRows + 1];
-  int seen = 0;
-  bool dirty = false;
-  for (uint64_t todo = __ballot(live) & 0xffffull; todo; ++seen) {
-    const int row0 = __builtin_ctzll(todo);
-    const int id = __builtin_amdgcn_readlane(mine, row0);
-    const uint64_t same = __ballot(mine == id);
-    todo &= ~same;
-    if (seen % ways != static_cast<int>(blockIdx.y)) continue;
-    // Rows of another adapter are read as row0; their results are not kept.
-    const T* x = static_cast<const T*>(a.x) +
-                 static_cast<int64_t>(m0 + (mine == id ? c : row0)) * a.ldx;
-    const T* A = static_cast<const T*>(a.A) + static_cast<int64_t>(id) * a.R * a.K;
-    v4f32 acc[RT];
+  // Rows of another adapter are read as row0; their results are not kept.
+  const T* x = static_cast<const T*>(a.x) +
+               static_cast<int64_t>(m0 + (mine == id ? c : row0)) * a.ldx;
+  const T* A = static_cast<const T*>(a.A) + static_cast<int64_t>(id) * a.R * a.K;
+  v4f32 acc[RT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) acc[r] = v4f32(0.0f);
-    for (int64_t k0 = k_begin + wave * (32 * U); k0 < k_end; k0 += 32 * U * kWaves) {
-      v4u32_t xv[U], av[U][RT];
+  for (int r = 0; r < RT; ++r) acc[r] = v4f32(0.0f);
+  for (int64_t k0 = k_begin + wave * (32 * U); k0 < k_end; k0 += 32 * U * kWaves) {
+    v4u32_t xv[U], av[U][RT];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t k = k0 + 32 * u + 8 * g;
-        const int64_t kc = k < k_end ? k : 0;
-        xv[u] = *reinterpret_cast<const any4*>(x + kc);
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = k0 + 32 * u + 8 * g;
+      const int64_t kc = k < k_end ? k : 0;
+      xv[u] = *reinterpret_cast<const any4*>(x + kc);
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-          av[u][r] = *reinterpret_cast<const any4*>(
-              A + static_cast<int64_t>(min(r0 + r * 16 + c, a.R - 1)) * a.K + kc);
-      }
+      for (int r = 0; r < RT; ++r)
+        av[u][r] = *reinterpret_cast<const any4*>(
+            A + static_cast<int64_t>(min(r0 + r * 16 + c, a.R - 1)) * a.K + kc);
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool in = k0 + 32 * u + 8 * g < k_end;
-        xv[u] = in ? xv[u] : v4u32_t(0u);
+    for (int u = 0; u < U; ++u) {
+      const bool in = k0 + 32 * u + 8 * g < k_end;
+      xv[u] = in ? xv[u] : v4u32_t(0u);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          av[u][r] = in ? av[u][r] : v4u32_t(0u);
-          acc[r] = Mma<T>::run(__builtin_bit_cast(V, av[u][r]), __builtin_bit_cast(V, xv[u]),
-                               acc[r]);
-        }
+      for (int r = 0; r < RT; ++r) {
+        av[u][r] = in ? av[u][r] : v4u32_t(0u);
+        acc[r] = Mma<T>::run(__builtin_bit_cast(V, av[u][r]), __builtin_bit_cast(V, xv[u]),
+                             acc[r]);
       }
     }
-    if (dirty) __syncthreads();
-    dirty = true;
-    // acc[r][i]: rank 16r + 4g + i of row c.
+  }
+  // acc[r][i]: rank 16r + 4g + i of row c.
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[wave][16 * r + 4 * g + i][c] = acc[r][i];
-    __syncthreads();
-    const int ranks = min(RT * 16, a.R - r0);
-    for (int e = threadIdx.x; e < kRows * ranks; e += kWaves * 64) {
-      const int row = e / ranks, r = e - row * ranks;
-      if (!((same >> row) & 1)) continue;
-      const float v = (sum[0][r][row] + sum[1][r][row]) + (sum[2][r][row] + sum[3][r][row]);
-      a.t[(static_cast<int64_t>(split) * a.M + m0 + row) * a.R + r0 + r] = v;
-    }
+    for (int i = 0; i < 4; ++i) sum[wave][16 * r + 4 * g + i][c] = acc[r][i];
+  __syncthreads();
+  const int ranks = min(RT * 16, a.R - r0);
+  for (int e = threadIdx.x; e < kRows * ranks; e += kWaves * 64) {
+    const int row = e / ranks, r = e - row * ranks;
+    if (!((same >> row) & 1)) continue;
+    const float v = (sum[0][r][row] + sum[1][r][row]) + (sum[2][r][row] + sum[3][r][row]);
+    a.t[(static_cast<int64_t>(split) * a.M + m0 + row) * a.R + r0 + r] = v;
   }
 }
 
@@ -187,70 +187,57 @@ struct RowFactors {
   typename Mma<T>::V hi[KS], lo[KS];
   float factor;
 };
-// For rows m0 + 16 w + c, w < RW.  The planes are added in order, P of all rows' loads
-// under way at once (past the last plane, its own again, which is not added).
-template <typename T, int KS, int RW>
-__device__ __forceinline__ void load_factors(const LoraArgs& a, int m0, const int (&id)[RW],
-                                             const bool (&live)[RW], int g, int c,
-                                             RowFactors<T, KS> (&f)[RW]) {
-  constexpr int P = RW * KS >= 4 ? 1 : 4 / (RW * KS);
-  float t[RW][KS][8];
+// For row m0 + c.  The planes are added in order, P of their loads under way at once (past
+// the last plane, its own again, which is not added).
+template <typename T, int KS>
+__device__ __forceinline__ void load_factors(const LoraArgs& a, int m0, int id, bool live, int g,
+                                             int c, RowFactors<T, KS>& f) {
+  constexpr int P = KS >= 4 ? 1 : 4 / KS;
+  float t[KS][8];
 #pragma unroll
-  for (int w = 0; w < RW; ++w)
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) t[w][s][e] = 0.0f;
-  auto inside = [&](int w, int s) { return live[w] && 32 * s + 8 * g < a.R; };
+    for (int e = 0; e < 8; ++e) t[s][e] = 0.0f;
+  auto inside = [&](int s) { return live && 32 * s + 8 * g < a.R; };
   if (a.adapters > 0)
     for (int p0 = 0; p0 < a.splits; p0 += P) {
-      v4f32 v[P][RW][KS][2];
+      v4f32 v[P][KS][2];
 #pragma unroll
       for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int w = 0; w < RW; ++w)
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            // A row without an adapter, or ranks past the last, read the plane's start.
-            const int64_t at = static_cast<int64_t>(min(p0 + i, a.splits - 1)) * a.M * a.R +
-                               (inside(w, s) ? static_cast<int64_t>(m0 + 16 * w + c) * a.R +
-                                                   32 * s + 8 * g
-                                             : 0);
-            const v4f32* tp = reinterpret_cast<const v4f32*>(a.t + at);
-            v[i][w][s][0] = tp[0], v[i][w][s][1] = tp[1];
-          }
+        for (int s = 0; s < KS; ++s) {
+          // A row without an adapter, or ranks past the last, read the plane's start.
+          const int64_t at =
+              static_cast<int64_t>(min(p0 + i, a.splits - 1)) * a.M * a.R +
+              (inside(s) ? static_cast<int64_t>(m0 + c) * a.R + 32 * s + 8 * g : 0);
+          const v4f32* tp = reinterpret_cast<const v4f32*>(a.t + at);
+          v[i][s][0] = tp[0], v[i][s][1] = tp[1];
+        }
 #pragma unroll
       for (int i = 0; i < P; ++i)
         if (p0 + i < a.splits)
 #pragma unroll
-          for (int w = 0; w < RW; ++w)
+          for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                t[w][s][e] += inside(w, s) ? v[i][w][s][e / 4][e % 4] : 0.0f;
+            for (int e = 0; e < 8; ++e) t[s][e] += inside(s) ? v[i][s][e / 4][e % 4] : 0.0f;
     }
+  float top = 0.0f;
 #pragma unroll
-  for (int w = 0; w < RW; ++w) {
-    float top = 0.0f;
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(t[s][e]));
+  top = fmaxf(top, __shfl_xor(top, 16, 64));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  const int ex = row_exponent<T>(top);
+  f.factor = live ? __builtin_amdgcn_ldexpf(a.scale ? a.scale[id] : 1.0f, ex) : 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(t[w][s][e]));
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const int ex = row_exponent<T>(top);
-    f[w].factor =
-        live[w] ? __builtin_amdgcn_ldexpf(a.scale ? a.scale[id[w]] : 1.0f, ex) : 0.0f;
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        T hi, lo;
-        split_halves(__builtin_amdgcn_ldexpf(t[w][s][e], -ex), &hi, &lo);
-        f[w].hi[s][e] = hi, f[w].lo[s][e] = lo;
-      }
-  }
+    for (int e = 0; e < 8; ++e) {
+      T hi, lo;
+      split_halves(__builtin_amdgcn_ldexpf(t[s][e], -ex), &hi, &lo);
+      f.hi[s][e] = hi, f.lo[s][e] = lo;
+    }
 }
 
 // Many rows: t of 64 rows, a part of K; workgroup (tile, y, part) takes the tile's adapters
@@ -490,7 +477,7 @@ __global__ __launch_bounds__(kWaves * 64) void lora_expand_few_kernel(LoraArgs a
   RawVec<T> y;
   if (here && left > 0) y = load_y<T>(a, m, n, left);
   v4f32 acc[2] = {v4f32(0.0f), v4f32(0.0f)};
-  RowFactors<T, KS> f[1];
+  RowFactors<T, KS> f;
 #pragma unroll
   for (int i0 = 0; i0 < PER; i0 += BATCH) {
     v4u32_t w[BATCH][2][KS];
@@ -500,19 +487,19 @@ __global__ __launch_bounds__(kWaves * 64) void lora_expand_few_kernel(LoraArgs a
 #pragma unroll
         for (int u = 0; u < 2; ++u) load_b<T, KS>(a, ids[i0 + i], n0, u, g, c, w[i][u]);
     if (i0 == 0)
-      load_factors<T, KS, 1>(a, blockIdx.y * kRows, {mine}, {live && here}, g, c, f);
+      load_factors<T, KS>(a, blockIdx.y * kRows, mine, live && here, g, c, f);
 #pragma unroll
     for (int i = 0; i < BATCH; ++i)
       if (i0 + i < count) {
         const bool hit = mine == ids[i0 + i];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const v4f32 d = times_b<T, KS>(w[i][u], f[0]);
+          const v4f32 d = times_b<T, KS>(w[i][u], f);
           acc[u] = hit ? d : acc[u];
         }
       }
   }
-  if (here && left > 0) store_out<T>(a, m, n, left, mine, y, acc[0], acc[1], f[0].factor);
+  if (here && left > 0) store_out<T>(a, m, n, left, mine, y, acc[0], acc[1], f.factor);
 }
 
 // Many rows: workgroup (64 rows, 32 NB columns), a wave 16 of the rows.  Everything a wave
@@ -698,7 +685,7 @@ hxm_status launch_lora(LoraArgs a, hipStream_t stream) {
 #undef HXM_HALVES
     if ((st = check_launch("lora halves")) != HXM_OK) return st;
   } else if (a.adapters > 0) {
-    // All adapters of a tile at once.
+    // All adapters of a tile at once, each a workgroup.
     const dim3 grid(static_cast<unsigned>(ceil_div(a.M, kRows)), std::min(kRows, a.M),
                     static_cast<unsigned>(a.splits * ceil_div(a.R, 128)));
     if (a.R <= 16) lora_shrink_kernel<T, 1><<<grid, kWaves * 64, 0, stream>>>(a);
