@@ -155,6 +155,19 @@ inline bool strides_disjoint(const int64_t* n, const int64_t* s, int dims, int64
   return true;
 }
 
+// Whether two such arrays at the same strides (at most 3 dims), at byte addresses a and b,
+// share no element: the step from one to the other is one more stride, with an extent of
+// two.  (Heads of q between heads of k in a fused projection, keys and values of a cache
+// side by side: spans that meet, and rows that do not.)  eb: bytes of an element.
+inline bool twins_disjoint(uintptr_t a, uintptr_t b, const int64_t* n, const int64_t* s, int dims,
+                           int64_t width, int64_t eb) {
+  const uintptr_t step = a < b ? b - a : a - b;
+  if (dims < 0 || dims > 3 || step % eb != 0) return false;
+  int64_t n2[4] = {2}, s2[4] = {static_cast<int64_t>(step / eb)};
+  for (int i = 0; i < dims; ++i) n2[i + 1] = n[i], s2[i + 1] = s[i];
+  return strides_disjoint(n2, s2, dims + 1, width);
+}
+
 // Division of n < 2^31 by a fixed d in [1, 2^31): with l = ceil(log2 d) and
 // m = ceil(2^(31+l) / d), n / d = (n m) >> (31 + l): m d - 2^(31+l) < d <= 2^l, so
 // the product is off by less than 2^(31+l) / d.  m fits 32 bits (2^(l-1) < d);

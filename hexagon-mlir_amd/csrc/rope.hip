@@ -165,10 +165,19 @@ bool heads_same(const hxm_heads* out, const hxm_heads* in, int64_t tokens, int64
 
 bool heads_apart(const hxm_heads* out, int64_t out_heads, const hxm_heads* in, int64_t in_heads,
                  int64_t tokens, int64_t dim) {
-  return matrices_disjoint(reinterpret_cast<uintptr_t>(out->data), out->token_stride,
-                           reinterpret_cast<uintptr_t>(in->data), in->token_stride, tokens,
-                           (out_heads - 1) * out->head_stride + dim,
-                           (in_heads - 1) * in->head_stride + dim, 2);
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out->data),
+                  i = reinterpret_cast<uintptr_t>(in->data);
+  if (matrices_disjoint(o, out->token_stride, i, in->token_stride, tokens,
+                        (out_heads - 1) * out->head_stride + dim,
+                        (in_heads - 1) * in->head_stride + dim, 2))
+    return true;
+  // Heads of one between heads of the other.  A stride along one token or one head is none.
+  if ((tokens > 1 && out->token_stride != in->token_stride) ||
+      (out_heads > 1 && in_heads > 1 && out->head_stride != in->head_stride))
+    return false;
+  const int64_t n[2] = {tokens, out_heads > in_heads ? out_heads : in_heads};
+  const int64_t s[2] = {out->token_stride, out_heads > 1 ? out->head_stride : in->head_stride};
+  return twins_disjoint(o, i, n, s, 2, dim, 2);
 }
 
 hxm_status check_kv_cache(const char* op, const hxm_kv_cache* c, bool written) {

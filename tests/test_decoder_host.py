@@ -202,3 +202,41 @@ def test_host_tensors_are_refused():
                  lambda: hxm.ops.lora_add(t[:, 0], t[:, 0], t, t, i)):
         with pytest.raises((ValueError, RuntimeError)):
             call()
+
+
+def interleaved(heads, tokens=5, **kw):
+    """A fused projection whose heads hold q, k and v side by side ([tokens, heads, 3, 64]),
+    q turned in place."""
+    at = lambda i: (16 * MB + 128 * i, heads * 192, 192)  # noqa: E731
+    return rope(**{**dict(q=at(0), q_out=at(0), q_heads=heads, k=at(1), v=at(2), heads=heads,
+                          ks=(heads * 1024, 1024, 64), vs=(heads * 1024, 1024, 64),
+                          tokens=tokens), **kw})
+
+
+@no_gpu
+@pytest.mark.parametrize("tokens", [1, 5])
+@pytest.mark.parametrize("heads", [1, 2, 8])
+def test_rope_append_in_place_between_the_heads_of_k_and_v(heads, tokens):
+    assert interleaved(heads, tokens) == _lib.HXM_NO_DEVICE, hxm.last_error()
+    # k a dim short of q's end, and (where there is a next head) past its start.
+    for off in (63, 129):
+        st = interleaved(heads, tokens, k=(16 * MB + 2 * off, heads * 192, 192),
+                         v=(19 * MB, heads * 192, 192))
+        if off == 63 or heads * tokens > 1:
+            _refused(st, INVALID, "overlaps")
+        else:
+            assert st == _lib.HXM_NO_DEVICE
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_overlap_logic_under_asan_and_ubsan(tmp_path):
+    exe = tmp_path / "overlap_logic_check"
+    src = os.path.join(ROOT, "tests", "sanitize", "overlap_logic_check.cpp")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fno-omit-frame-pointer",
+                    "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-Wall", "-Werror", src, "-o", str(exe)], check=True, timeout=300)
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=1:abort_on_error=0",
+               UBSAN_OPTIONS="print_stacktrace=1:halt_on_error=1")
+    env.pop("LD_PRELOAD", None)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and "overlap logic ok" in r.stdout, r.stdout + r.stderr

@@ -216,3 +216,26 @@ def test_refusals(dev):
     e = mk(0, hkv, D)
     assert ops.rope_append(mk(0, hq, D), e, e, ok["k_cache"], ok["v_cache"], ok["slots"][:0],
                            ok["positions"][:0], ok["cos_sin"]).shape == (0, hq, D)
+
+
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_in_place_between_the_heads_of_k_and_v(dev, T, interleaved):
+    """A fused projection whose heads hold q, k and v side by side, q turned in place."""
+    H, D, page = 6, 64, 16
+    g = torch.Generator().manual_seed(T)
+    qkv = torch.randn(T, H, 3, D, generator=g).half()
+    fused = qkv.to(dev)
+    q, k, v = fused.unbind(2)
+    kc, vc = make_cache(T // page + 1, H, page, D, "nhd", torch.float16, dev)
+    slots = torch.randperm((T // page + 1) * page, generator=g)[:T].int()
+    pos = torch.randint(0, 512, (T,), generator=g).int()
+    cs = table(512, D)
+    out = ops.rope_append(q, k, v, kc, vc, slots.to(dev), pos.to(dev), cs.to(dev),
+                          interleaved=interleaved, q_out=q)
+    assert out is q
+    c, s = cs[pos.long()], slots.long()
+    close(fused[:, :, 0], *rotate64(qkv[:, :, 0], c, D, interleaved), "f16")
+    assert torch.equal(fused[:, :, 1:].cpu(), qkv[:, :, 1:])
+    close(kc.transpose(1, 2)[s // page, s % page], *rotate64(qkv[:, :, 1], c, D, interleaved), "f16")
+    assert torch.equal(vc.transpose(1, 2)[s // page, s % page].cpu(), qkv[:, :, 2])
