@@ -180,6 +180,27 @@ bool heads_apart(const hxm_heads* out, int64_t out_heads, const hxm_heads* in, i
   return twins_disjoint(o, i, n, s, 2, dim, 2);
 }
 
+// Keys and values apart: whole buffers, parts of each page, or rows side by side at equal
+// strides.
+static bool keys_values_apart(const hxm_kv_cache* c) {
+  const uintptr_t k = reinterpret_cast<uintptr_t>(c->k), v = reinterpret_cast<uintptr_t>(c->v);
+  auto page_span = [&](int64_t head_stride, int64_t token_stride) {
+    const __int128 span = static_cast<__int128>(c->heads - 1) * head_stride +
+                          static_cast<__int128>(c->page_size - 1) * token_stride + c->dim;
+    return span < INT64_MAX ? static_cast<int64_t>(span) : INT64_MAX;
+  };
+  if (matrices_disjoint(k, c->k_page_stride, v, c->v_page_stride, c->pages,
+                        page_span(c->k_head_stride, c->k_token_stride),
+                        page_span(c->v_head_stride, c->v_token_stride), 2))
+    return true;
+  const int64_t n[3] = {c->pages, c->heads, c->page_size};
+  const int64_t ks[3] = {c->k_page_stride, c->k_head_stride, c->k_token_stride},
+                vs[3] = {c->v_page_stride, c->v_head_stride, c->v_token_stride};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && ks[i] != vs[i]) return false;
+  return twins_disjoint(k, v, n, ks, 3, c->dim, 2);
+}
+
 hxm_status check_kv_cache(const char* op, const hxm_kv_cache* c, bool written) {
   if (!c || !c->k || !c->v)
     return fail(HXM_INVALID_ARG, "invalid-argument: %s null cache", op);
@@ -206,6 +227,8 @@ hxm_status check_kv_cache(const char* op, const hxm_kv_cache* c, bool written) {
     if (written && !strides_disjoint(n, st, 3, c->dim))
       return fail(HXM_INVALID_ARG, "invalid-argument: %s cache rows share elements", op);
   }
+  if (written && !keys_values_apart(c))
+    return fail(HXM_INVALID_ARG, "invalid-argument: %s keys and values share elements", op);
   return HXM_OK;
 }
 

@@ -565,8 +565,9 @@ typedef struct hxm_heads {
  * either may end there, element by element).  A position outside [0, max_pos) makes the
  * rotated dims of that token NaN.  cos_sin: fp32 [max_pos, rot_dim]
  * (ld_cos_sin); rot_dim even, 0 to dim (0: an append without rotation,
- * positions and cos_sin unused).  The cache must not overlap the other
- * tensors.  dtype F16 or BF16, one for all. */
+ * positions and cos_sin unused).  Keys and values of the cache must share no
+ * element (refused where their strides do not show it), nor the cache any with
+ * the other tensors.  dtype F16 or BF16, one for all. */
 hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q_heads,
                            const hxm_heads* k, const hxm_heads* v, const int32_t* positions,
                            const float* cos_sin, int64_t ld_cos_sin, int64_t max_pos,

@@ -240,3 +240,49 @@ def test_overlap_logic_under_asan_and_ubsan(tmp_path):
     env.pop("LD_PRELOAD", None)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300, env=env)
     assert r.returncode == 0 and "overlap logic ok" in r.stdout, r.stdout + r.stderr
+
+
+KV = dict(pages=4, page_size=16, heads=2, dim=64)
+
+
+@no_gpu
+@pytest.mark.parametrize("v_cache, ks, vs", [
+    (24 * MB, (2048, 1024, 64), (2048, 1024, 64)),               # one cache for both
+    (24 * MB, (2048, 1024, 64), (2048, 64, 128)),                # in two layouts
+    (24 * MB + 2, (2048, 1024, 64), (2048, 1024, 64)),
+    (24 * MB + 2 * 1024, (2048, 1024, 64), (2048, 1024, 64)),    # values at the next head's keys
+    (24 * MB + 2 * 2048, (2048, 1024, 64), (2048, 1024, 64)),    # at the next page's
+    (24 * MB - 2 * 2048, (2048, 1024, 64), (2048, 1024, 64)),
+    (24 * MB + 2 * 2040, (4096, 1024, 64), (4096, 1024, 64)),    # eight elements into the page
+])
+def test_rope_append_refuses_keys_and_values_in_one_place(v_cache, ks, vs):
+    _refused(rope(**KV, v_cache=v_cache, ks=ks, vs=vs), INVALID, "keys and values")
+    # Attention only reads them.
+    assert attention(**KV, v_cache=v_cache, ks=ks, vs=vs) == _lib.HXM_NO_DEVICE
+
+
+@no_gpu
+@pytest.mark.parametrize("at, ks, vs", [
+    (8192, (2048, 1024, 64), (2048, 1024, 64)),                  # [2, pages, heads, page, dim]
+    (-8192, (2048, 1024, 64), (2048, 1024, 64)),
+    (2048, (4096, 1024, 64), (4096, 1024, 64)),                  # [pages, 2, heads, page, dim]
+    (-2048, (4096, 64, 128), (4096, 64, 128)),                   # [pages, 2, page, heads, dim]
+    (2048, (4096, 1024, 64), (4096, 64, 128)),                   # each half in its own layout
+    (1024, (4096, 2048, 64), (4096, 2048, 64)),                  # [pages, heads, 2, page, dim]
+    (64, (4096, 2048, 128), (4096, 2048, 128)),                  # [pages, heads, page, 2, dim]
+    (64, (4096, 128, 256), (4096, 128, 256)),                    # [pages, page, heads, 2, dim]
+    (128, (4096, 64, 256), (4096, 64, 256)),                     # [pages, page, 2, heads, dim]
+    (3 * 2048, (4 * 2048, 1024, 64), (4 * 2048, 1024, 64)),      # of [pages, layers, 2, ..]
+    (3 * 2048, (4096, 1024, 64), (4096, 1024, 64)),              # values a page further
+])
+def test_rope_append_takes_keys_and_values_side_by_side(at, ks, vs):
+    assert rope(**KV, v_cache=24 * MB + 2 * at, ks=ks, vs=vs) == _lib.HXM_NO_DEVICE, \
+        hxm.last_error()
+
+
+@no_gpu
+def test_rope_append_spans_past_64_bits():
+    far = (1 << 40, 1 << 40, 1 << 40)
+    one = dict(pages=1, page_size=1 << 30, heads=1, ks=far, vs=far)
+    assert rope(**one, k=(18 * MB, 64, 64), v=(19 * MB, 64, 64)) == _lib.HXM_NO_DEVICE
+    _refused(rope(**one, v_cache=24 * MB), INVALID, "keys and values")
