@@ -512,9 +512,11 @@ def _rows_out(out: Optional[torch.Tensor], x: torch.Tensor, cols: int):
     """The output of a row op: new, or the caller's of x's shape and dtype
     (rows of it may be strided, its last dimension contiguous)."""
     if out is None:
-        out = torch.empty_like(x)
-        if out.dim() == 2:
+        if x.dim() == 2:
+            out = torch.empty_like(x)
             return out, out
+        # Not x's own strides: its dimensions may be permuted.
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif tuple(out.shape) != tuple(x.shape) or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"out must be {x.dtype} {tuple(x.shape)} on {x.device} "
                          f"(got {out.dtype} {tuple(out.shape)} on {out.device})")

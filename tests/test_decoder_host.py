@@ -286,3 +286,14 @@ def test_rope_append_spans_past_64_bits():
     one = dict(pages=1, page_size=1 << 30, heads=1, ks=far, vs=far)
     assert rope(**one, k=(18 * MB, 64, 64), v=(19 * MB, 64, 64)) == _lib.HXM_NO_DEVICE
     _refused(rope(**one, v_cache=24 * MB), INVALID, "keys and values")
+
+
+@pytest.mark.parametrize("shape, order", [((4, 3, 8), (1, 0, 2)), ((2, 5, 3, 16), (2, 0, 1, 3)),
+                                          ((4, 3, 8), (0, 1, 2)), ((8,), (0,)), ((0, 3, 8), (1, 0, 2))])
+def test_new_outputs_of_permuted_rows(shape, order):
+    """The output that a row operator makes itself has evenly strided rows, whatever
+    the order of its input's dimensions."""
+    x = torch.zeros(shape, dtype=torch.float16).permute(order)
+    out, rows = hxm.ops._rows_out(None, x, shape[-1])
+    assert out.shape == x.shape and out.dtype == x.dtype
+    assert rows.data_ptr() == out.data_ptr() and rows.shape == (x.numel() // shape[-1], shape[-1])

@@ -228,3 +228,18 @@ def test_more_than_a_workgroup_a_cu(dev, name, cols, rows):
     run_case(dev, name, rows, cols, "layer", "rms", 1, alias="y=x")
     run_case(dev, name, rows - 4, cols, "none", "rms", rows - 4, bias=False, alias="y=h z=x")
     run_case(dev, name, rows - 3, cols, "layer", "none", 0)
+
+
+def test_permuted_rows(dev):
+    """Sequences first or tokens first: rows of a permuted tensor, new outputs."""
+    import torch.nn.functional as F
+
+    g = torch.Generator().manual_seed(12)
+    h, x = (torch.randn(7, 5, 96, generator=g).half().to(dev).transpose(0, 1) for _ in range(2))
+    for a, b in zip(ops.residual_norm(h, x, post="rms", pre_eps=EPS),
+                    ops.residual_norm(h.contiguous(), x.contiguous(), post="rms", pre_eps=EPS)):
+        assert a.shape == h.shape and torch.equal(a, b)
+    assert torch.equal(ops.softmax(h), ops.softmax(h.contiguous()))
+    assert torch.equal(ops.rms_norm(h, (96,)), ops.rms_norm(h.contiguous(), (96,)))
+    torch.testing.assert_close(ops.layer_norm(h, (96,)).float(), F.layer_norm(h.float(), (96,)),
+                               rtol=1e-2, atol=2e-3)
