@@ -680,9 +680,13 @@ extern "C" hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* o
                 "invalid-argument: paged_attention batch=%lld, %lld query heads over %lld, "
                 "window=%lld",
                 (long long)batch, (long long)q_heads, (long long)cache->heads, (long long)window);
-  // 2^24 sequences times heads keep every count of pieces in 32 bits.
+  // 2^24 sequences times heads keep every count of pieces in 32 bits.  A launch holds one
+  // workgroup fewer, the pieces of sequences that are cut among them (attn_grid).
   constexpr int64_t kMaxBatchHeads = int64_t(1) << 24;
-  if (q_heads > 65535 || batch > kMaxBatchHeads || batch * q_heads > kMaxBatchHeads)
+  constexpr int64_t kMaxGroups = 0xffffffffLL / (kWaves * 64);
+  if (q_heads > 65535 || batch > kMaxBatchHeads || batch * q_heads > kMaxBatchHeads ||
+      batch * cache->heads * ceil_div(q_heads / cache->heads, kHeads) >
+          kMaxGroups - (batch > kAttnCutBatch ? 0 : kAttnFine * kAttnGroups))
     return fail(HXM_UNSUPPORTED_SHAPE, "tile-alignment: paged_attention batch=%lld, %lld heads",
                 (long long)batch, (long long)q_heads);
   if ((st = check_heads("paged_attention", "q", q, batch, q_heads, cache->dim, false)) != HXM_OK ||

@@ -592,7 +592,9 @@ hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q
  * product with V with 22 bits (f16) or 16 (bf16).  out may be q itself.  A
  * long cache is split over workgroups (in batches of up to 256 sequences) and
  * joined in a fixed order: results do not depend on how the workgroups are
- * scheduled.  batch * q_heads up to 2^24.  Uses the per-stream workspace. */
+ * scheduled.  batch * q_heads up to 2^24, and batch * cache->heads (times
+ * ceil(q_heads / cache->heads / 16)) below 2^24, or 2^24 - 768 where sequences
+ * are split.  Uses the per-stream workspace. */
 hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
                                const hxm_kv_cache* cache, const int32_t* block_table,
                                int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,

@@ -297,3 +297,21 @@ def test_new_outputs_of_permuted_rows(shape, order):
     out, rows = hxm.ops._rows_out(None, x, shape[-1])
     assert out.shape == x.shape and out.dtype == x.dtype
     assert rows.data_ptr() == out.data_ptr() and rows.shape == (x.numel() // shape[-1], shape[-1])
+
+
+@no_gpu
+def test_paged_attention_refuses_more_workgroups_than_a_launch_holds():
+    """2^32 - 1 work-items, 256 to a sequence and head, and 768 workgroups for the pieces of
+    sequences that are cut."""
+    most = (2 ** 32 - 1) // 256
+    one = dict(q_heads=1, heads=1, ks=(1024, 1024, 64), vs=(1024, 1024, 64), q=(16 * MB, 64, 64),
+               out=(1 << 40, 64, 64))
+    assert attention(**one, batch=most) == _lib.HXM_NO_DEVICE
+    _refused(attention(**one, batch=most + 1), SHAPE)
+    two = dict(heads=1, ks=(1024, 1024, 64), vs=(1024, 1024, 64), q_heads=16, q=(16 * MB, 1024, 64),
+               out=(1 << 40, 1024, 64))
+    assert attention(**two, batch=1 << 20) == _lib.HXM_NO_DEVICE   # sixteen heads share one
+    wide = dict(q_heads=65535, heads=65535, ks=(65535 * 1024, 1024, 64), vs=(65535 * 1024, 1024, 64),
+                q=(16 * MB, 65535 * 64, 64), out=(1 << 40, 65535 * 64, 64))
+    assert attention(**wide, batch=255) == _lib.HXM_NO_DEVICE
+    _refused(attention(**wide, batch=256), SHAPE)
