@@ -589,12 +589,14 @@ hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q
  * tokens, or n beyond table_pages * page_size or 2^30, makes that sequence's
  * outputs NaN.  dtype F16 or BF16, one for q, cache and out; scores, the softmax's
  * maximum and sum and the output's sum are fp32, the probabilities enter the
- * product with V with 22 bits (f16) or 16 (bf16).  out may be q itself.  A
- * long cache is split over workgroups (in batches of up to 256 sequences) and
- * joined in a fixed order: results do not depend on how the workgroups are
- * scheduled.  batch * q_heads up to 2^24, and batch * cache->heads (times
- * ceil(q_heads / cache->heads / 16)) below 2^24, or 2^24 - 768 where sequences
- * are split.  Uses the per-stream workspace. */
+ * product with V as two 16-bit halves: 22 bits (f16; one below 2^-10 of the
+ * largest to 2^-32 of that) or 16 (bf16).  Where V is infinite the halves make
+ * its dim infinite or NaN.  out may be q itself; out and lse must overlap nothing
+ * else.  A long cache is split over workgroups (in batches of up to 256
+ * sequences) and joined in a fixed order: results do not depend on how the
+ * workgroups are scheduled.  batch * q_heads up to 2^24, and batch *
+ * cache->heads (times ceil(q_heads / cache->heads / 16)) below 2^24, or 2^24 -
+ * 768 where sequences are split.  Uses the per-stream workspace. */
 hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
                                const hxm_kv_cache* cache, const int32_t* block_table,
                                int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
@@ -611,7 +613,8 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * overlap of out with y or x is refused (A, B, index and scale must not overlap
  * it either).  x A^T accumulates in fp32 and enters the second product with 22
  * bits (f16; a rank below 2^-17 of its row's largest to 2^-39 of that) or 16
- * bits (bf16) of precision; one rounding to dtype.  dtype F16 or BF16, one for
+ * bits (bf16) of precision, as two 16-bit halves (which make a column whose B
+ * is infinite infinite or NaN); one rounding to dtype.  dtype F16 or BF16, one for
  * all; K a multiple of 8, R a multiple of 8 up to 256.  Uses the per-stream
  * workspace. */
 hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, const void* A,

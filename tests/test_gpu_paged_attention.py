@@ -360,3 +360,22 @@ def test_refusals(dev):
     assert out.shape == (0, 4, D) and lse.shape == (0, 4)
     out = ops.paged_attention(**{**ok, "block_table": mk(B, 0, dt=torch.int32)})
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("lens", [[40, 70], [3000, 70]])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_infinite_and_nan_values_keep_to_their_dims(dev, name, lens):
+    """An infinite or NaN value of a live token: its sequence, key head and dim are not finite,
+    all else is as without it."""
+    g = torch.Generator().manual_seed(11)
+    q, kc, vc, table, ln, _ = build(g, name, lens, 2, 3, 64, 16, "hnd", dev)
+    q = q.to(dev)
+    want, wl = ops.paged_attention(q, kc, vc, table, ln, return_lse=True)
+    t = lens[0] - 3
+    row = vc[table[0, t // 16], 1, t % 16]
+    row[5], row[9], row[40] = float("inf"), -float("inf"), float("nan")
+    out, lse = ops.paged_attention(q, kc, vc, table, ln, return_lse=True)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[0, 3:, [5, 9, 40]] = True
+    assert not out[hit].isfinite().any() and out[0, 3:, 40].isnan().all()
+    assert torch.equal(out[~hit], want[~hit]) and torch.equal(lse, wl)
