@@ -3,7 +3,9 @@
 // Bound by memory: the keys and values of a sequence are read once per key
 // head, 4 * dim bytes a token, against 4 * dim * group operations.  The group of
 // query heads that shares a key head is the 16-wide side of the MFMAs (padded
-// with zeros), so one read serves the whole group.
+// with zeros), so one read serves a group of up to 16.  Larger ones are read once for every
+// 16 of them, by workgroups apart (8 x 32768 tokens, 2 heads of 128: groups of 16 take 41 us,
+// 17 and 32 64, 48 94).
 //
 // A wave takes 32 tokens at a time, in two steps whose data stays in registers.
 // S^T = K Q^T, K the left operand, leaves lane (g, c) = (lane / 16, lane % 16)
@@ -14,10 +16,12 @@
 // of lanes.
 //
 // Keys and values come in whole rows, 1 KiB of neighbouring bytes an instruction in the
-// order of a page, nontemporal: nothing is read twice.  (Keys loaded in the operand's own
-// layout, 64 bytes of 16 rows an instruction, read every line in two halves, which the
-// caches had to join: 8 x 32768 tokens, 8 heads of 128, 98 us and 91 nontemporal, against
-// 88.)  A lane then holds 8 tokens x dim / 16 dims of V and transposes them in registers
+// order of a page, nontemporal: a workgroup reads nothing twice.  (Keys loaded in the operand's
+// own layout, 64 bytes of 16 rows an instruction, read every line in two halves, which the
+// caches have to join.  With that layout and three pieces a CU, 8 x 32768 tokens, 8 heads of
+// 128, took 98 us where this takes 86, 32 x 4096, 4 heads of 256, 65 and 49; but 16 windows of
+// 1000 tokens, one head of 64, took 8.6 and take 10.2, 1 x 2000 tokens 9.8 and 11.3: a tile's
+// way through LDS is longer than its own loads.)  A lane then holds 8 tokens x dim / 16 dims of V and transposes them in registers
 // with byte permutes; K becomes the left operand through the wave's own piece of LDS, where
 // row t has its 16-byte chunk q at q ^ t % 16 (of 8 chunks: q ^ t / 2 % 8, two rows to all
 // 64 banks), so that neither side meets a bank twice.  The next tile's keys are on their
@@ -30,7 +34,8 @@
 // one half alone added as much to the error as the output's own rounding, and the
 // second costs no time that shows: 98.3 against 98.5 us).  f16 ones are scaled by
 // 2^7 on the way, so that with those 8 binary orders of headroom they stay below
-// 65504 and the smallest normal one is 2^-21 of the largest.
+// 65504 and the smallest normal one is 2^-21 of the largest; the second half, 2^-24 at least, is
+// off by up to 2^-32 of the largest, which is more than 22 bits leave of one below 2^-10 of it.
 #include <algorithm>
 #include <type_traits>
 
@@ -58,8 +63,10 @@ constexpr float kSlack = 8.0f;  // of the running maximum, in powers of two
 // with 768.  Where sequences times heads are more than that, three times as many pieces
 // level what their lengths differ by (16 x 8192 tokens at most, 32 heads: 150 us with 2,
 // 141 with 3, 143 with 4 and more; 64 x 4096, 8 heads: 81.5, 80.7, 80.7).  A join costs
-// about what three units do, so four units are left whole (1 x 300 tokens, 32 heads: 7.8 us
-// whole, 9.2 in two).
+// about what three units do, so four units are left whole (1 x 300 tokens, 32 heads: 8.8 us
+// whole, 10.3 in two; 8 x 500, 8 heads, 10.0 and 10.8); of longer ones pieces of two units are worth it (the least piece two or
+// four units, and four or eight left whole: 1 x 700 tokens, 8 heads, 10.8 and 12.2 us; 1 x 2000
+// 11.3 and 13.3; 32 x 1000, one head, 10.9 and 14.5; 8 x 32768 the same).
 
 // Waves a SIMD, by the registers of a tile and the output: many short sequences hide each
 // other's start.  Rows located one by one need a few registers more, and spill with 128.
@@ -152,7 +159,9 @@ struct Piece {
 // Piece u of the batch, its sequences in order, cut as host_logic.h says.  Every wave
 // works it out from the lengths, 64 sequences at a time, all loaded at once: they are on
 // the device, so the host cannot.  Batches of more than 64 take the fine pieces without
-// trying the others.
+// trying the others, which took 13 us instead of 15.4 for 256 x 600 tokens, one head, 12.3 for
+// 13.7 (128 x 600, two) and 149 for 152 (256 x 2048, eight), and 15 for 11.6 where few tokens
+// are many sequences' (65 x 1024, one head) and 30 for 25 (200 x 2048, one).
 __device__ __forceinline__ Piece find_piece(const AttnArgs& a, uint32_t u, int lane) {
   auto tokens = [&](int32_t len, int* lo) {
     const int n = len > a.capacity ? 0 : max(len, 0);
@@ -222,9 +231,12 @@ __device__ __forceinline__ Piece find_piece(const AttnArgs& a, uint32_t u, int l
   return r;
 }
 
-// D_FULL: dim == DT, no dims to mask.  P8: page_size a multiple of 8, and 8 rows
-// of a page within 2^31 bytes: the tile's four groups of 8 tokens then have one
-// page each, whose number and address the scalar unit works out.
+// D_FULL: dim == DT, no dims to mask (masked all the same: 8 x 32768 tokens, 8 heads of 128,
+// 85.4 us for 84; 32 x 4096, 4 heads of 256, 50.6 for 49.4).  P8: page_size a multiple of 8, and
+// 8 rows of a page within 2^31 bytes: the tile's four groups of 8 tokens then have one
+// page each, whose number and address the scalar unit works out (rows located one by one over
+// the same pages of 16 take 94 us for 84, 58.4 for 51.5 at 64 x 4096, 8 heads of 64, and 144
+// for 49.4 at 256 dims, where one wave a SIMD waits for each table entry).
 template <typename T, int DT, bool D_FULL, bool P8>
 __global__ __launch_bounds__(kWaves * 64)
     __attribute__((amdgpu_waves_per_eu(attn_waves(DT, P8)))) void paged_attention_kernel(AttnArgs a) {

@@ -17,8 +17,8 @@
 // the adapter's weights through LDS, read in whole rows, and a launch between makes the
 // second operand once.
 //
-// 48 rows of 16 adapters, 4096 -> 4096, R 16: 9.9 us, two launches of 4.7 and 5.4.  2048
-// rows of 4, 4096 -> 11008, R 64, bf16: 36.6, of them 10 the first launch, 4 the second,
+// 48 rows of 16 adapters, 4096 -> 4096, R 16: 9.8 us, two launches of 4.4 and 5.5.  2048
+// rows of 4, 4096 -> 11008, R 64, bf16: 36.4, of them 10 the first launch, 4 the second,
 // and 22 the last, which moves 90 MB of y and out (17 us at a large copy's rate).  With
 // each wave reading its own operands of the weights and of y, 16 rows of 64 bytes an
 // instruction, they were 19, 5 and 39.  2048 rows of 16 mixed adapters, 4096 -> 4096, R 16:
@@ -511,8 +511,10 @@ __global__ __launch_bounds__(kWaves * 64) void lora_expand_few_kernel(LoraArgs a
 // Tiles are numbered down the rows and each XCD (workgroups go to them in turn) takes a run
 // of them, so that its L2 holds the columns' weights.
 constexpr int expand_blocks(int ks) { return ks <= 4 ? 4 : 2; }  // of 32 columns each
-// Waves a SIMD that the registers allow without spills (108 of them at R 64: five waves
-// spill some and run 58 us where four run 41).
+// Waves a SIMD that the compiler keeps its registers to.  R 256 needs two (2048 rows of 2,
+// 4096 -> 4096: 61.4 us, 65.6 with one); up to R 128 the kernel takes no more registers than
+// these leave it and one wave more or fewer is the same (R 64: 36.4 to 36.6 with
+// 3, 4 or 5; R 128, 4096 -> 4096, 38.2 with 2 or 3).
 constexpr int expand_waves(int ks) { return ks <= 2 ? 4 : ks <= 4 ? 3 : 2; }
 template <typename T, int KS>
 __global__ __launch_bounds__(kWaves * 64)
@@ -778,8 +780,8 @@ extern "C" hxm_status hxm_lora_add(const void* y, int64_t ldy, const void* x, in
       std::min({M, kLoraRows, (kLoraPlaneBytes / (R * 4)) & ~int64_t(15),
                 kManyTile * ((int64_t(1) << 23) / ceil_div(N, 64))});
   // K split until about 512 workgroups, in 8 parts at most, each a step of all its waves
-  // or more; many rows, tiles of 64, in 16 parts (2048 rows, R 64: 21.0 us with 512
-  // workgroups in sight, 22.9 with 256).
+  // or more; many rows, tiles of 64, in 16 parts (2048 rows, 4096 -> 11008, R 64: 36.4 us with
+  // 512 workgroups in sight, 37.6 with 256; 8192 rows, R 32: 56.4 and 63.8).
   const bool few = piece < kManyRows;
   const int64_t tiles = ceil_div(piece, few ? kRows : kManyTile);
   const int64_t step = few ? 32 * kWaves * shrink_steps(R <= 16 ? 1 : R <= 64 ? 4 : 8) : kManyK;

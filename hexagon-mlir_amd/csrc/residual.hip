@@ -186,7 +186,10 @@ __global__ __launch_bounds__(row_waves(S) * 64) void residual_norm_kernel(Residu
 
 // Rows too long for the registers: 16 waves re-read h and x in every pass and
 // compute y again.  y and z are written in the last pass alone, each element by
-// the thread that has read it, so that they may be h or x.
+// the thread that has read it, so that they may be h or x.  Every statistic is a pass:
+// 512 x 32768 f32, 268 MB, takes 69 us with an RMSNorm after, 77 with one on either side and
+// 101 with LayerNorms, where the same bytes in rows of half the length, held in registers,
+// take 43 to 45.
 template <typename T>
 __global__ __launch_bounds__(1024) void residual_norm_stream_kernel(ResidualArgs a) {
   constexpr int N = RowVec<T>::N, S = 16;
