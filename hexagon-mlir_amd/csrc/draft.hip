@@ -1,0 +1,342 @@
+// Which of a sequence's drafted tokens the target's probabilities keep, and the token that
+// follows them.
+//
+// Bound by the read of one row of the vocabulary per sequence (two with the draft's
+// probabilities): the tests themselves need one probability per drafted token.  A
+// sequence's row is cut into chunks, a workgroup each.  Every one of them walks the tree by
+// itself (a lane a node, all tests at once), sums its chunk of what is left in the row
+// where the walk ends, and the last to arrive looks for the chunk that holds the drawn
+// point, and for the token in it.  Nobody waits.
+//
+// Sums and products are in 64 bits: probabilities have 24, a product of two is exact, and
+// the sum of a row is off by about 2^-53 of itself per term, so that the drawn token is
+// that of exact arithmetic but for a point within that of a border between two tokens.
+#include <algorithm>
+
+#include "device_util.h"
+#include "hxm_internal.h"
+#include "row_vec.h"
+
+namespace hxm {
+
+namespace {
+
+constexpr int kMaxNodes = 64;
+constexpr int kThreads = 256;
+// Elements of a chunk at the least, and workgroups of a launch that the rows are cut for.
+constexpr int64_t kLeastChunk = 4096, kGroups = 1024;
+
+struct VerifyArgs {
+  const int32_t* tokens;
+  const int32_t* parents;
+  const void* target;
+  const void* draft;
+  const float* uniform;
+  int64_t ldt, ldd, vocab;
+  int32_t *path, *counts, *next;
+  double* sums;       // [batch][chunks]
+  uint32_t* arrived;  // [batch], zero between launches
+  int batch, nodes, chunks;
+  int64_t chunk;      // elements
+};
+
+// Probabilities below zero, and those that are no numbers, count as zero.
+template <typename T>
+__device__ __forceinline__ double prob(T v) {
+  return static_cast<double>(fmaxf(tof(v), 0.0f));
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Where the walk of a sequence ends.
+struct End {
+  int node;        // the last one kept, -1: no sequence
+  int count;       // kept ones
+  uint64_t kept;   // a bit each
+  uint64_t tried;  // its children that were tried, none kept
+  int token;       // lane i: node i's token
+};
+template <typename T, bool DRAFT>
+__device__ __forceinline__ End walk(const VerifyArgs& a, int b, int lane) {
+  const bool in = lane < a.nodes;
+  const int64_t at = static_cast<int64_t>(b) * a.nodes + (in ? lane : 0);
+  const int token = a.tokens[at];
+  int parent = a.parents ? a.parents[at] : lane - 1;
+  const double u = a.uniform[at];
+  // No child: past the nodes, of no earlier node, or of a token that is none.
+  const bool child = in && parent >= 0 && parent < lane && token >= 0 && token < a.vocab;
+  End r{-1, 0, 0, 0, token};
+  if (__builtin_amdgcn_readfirstlane(parent) != -1) return r;
+  double p = 0.0, q = 1.0;
+  if (child) {
+    const int64_t row = static_cast<int64_t>(b) * a.nodes + parent;
+    p = prob(static_cast<const T*>(a.target)[row * a.ldt + token]);
+    if (DRAFT) q = prob(static_cast<const T*>(a.draft)[row * a.ldd + token]);
+  }
+  if (!child) parent = -1;
+  // Brothers in order: what the older ones of other tokens leave (they were not kept), and
+  // whether one of them had this token.
+  double left = 1.0;
+  bool again = false, older = false;
+  for (int j = 1; j < a.nodes; ++j) {
+    const int pj = __builtin_amdgcn_readlane(parent, j);
+    if (pj < 0) continue;
+    const bool brother = child && lane > j && parent == pj;
+    older |= brother;
+    if (!DRAFT) {
+      const int tj = __builtin_amdgcn_readlane(token, j);
+      const bool fresh_j = __builtin_amdgcn_readlane(static_cast<int>(again), j) == 0;
+      const double p_j = lane_f64(p, j);
+      again |= brother && token == tj;
+      if (brother && fresh_j) left -= p_j;
+    }
+  }
+  const bool ok = child && (DRAFT ? !older : !again) && u * q * left < p;
+  const uint64_t oks = __ballot(ok), firsts = __ballot(child && !older);
+  int node = 0;
+  r.kept = 1, r.count = 1;
+  while (true) {
+    const uint64_t children = __ballot(child && parent == node);
+    const uint64_t good = children & oks;
+    if (!good) {
+      r.tried = DRAFT ? children & firsts : children;
+      break;
+    }
+    node = __builtin_ctzll(good);
+    r.kept |= uint64_t(1) << node;
+    ++r.count;
+  }
+  r.node = node;
+  return r;
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+template <typename T, bool DRAFT>
+__global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
+  constexpr int E = RowVec<T>::N;
+  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x;
+  __shared__ double totals[kThreads / 64];
+  __shared__ int32_t tried[kMaxNodes];
+  __shared__ int ntried, last;
+  __shared__ double found_before;
+  __shared__ int found;
+
+  const End end = walk<T, DRAFT>(a, b, lane);
+  if (chunk == 0 && wave == 0) {
+    if (lane < a.nodes) {
+      // The kept nodes in front, in their order, then -1.
+      const bool kept = (end.kept >> lane) & 1;
+      const uint64_t below = (uint64_t(1) << lane) - 1;
+      const int at = kept ? __builtin_popcountll(end.kept & below)
+                          : end.count + __builtin_popcountll(~end.kept & below);
+      a.path[static_cast<int64_t>(b) * a.nodes + at] = kept ? lane : -1;
+    }
+    if (lane == 0) a.counts[b] = end.count;
+    if (lane == 0 && end.node < 0) a.next[b] = -1;
+  }
+  if (end.node < 0) return;
+  // Tokens that are gone from the row (a one-hot draft's), by their order.
+  if (wave == 0) {
+    if ((end.tried >> lane) & 1)
+      tried[__builtin_popcountll(end.tried & ((uint64_t(1) << lane) - 1))] = end.token;
+    if (lane == 0) ntried = __builtin_popcountll(end.tried);
+  }
+  __syncthreads();
+  const int64_t row = static_cast<int64_t>(b) * a.nodes + end.node;
+  const T* p = static_cast<const T*>(a.target) + row * a.ldt;
+  const T* q = DRAFT && end.tried ? static_cast<const T*>(a.draft) + row * a.ldd : nullptr;
+  const int gone = DRAFT ? 0 : ntried;
+  // What the row leaves of element v (whole: of all of them).
+  auto weigh = [&](T pv, T qv, int64_t v, bool whole) {
+    double w = prob(pv);
+    if (DRAFT && q && !whole) w = fmax(w - prob(qv), 0.0);
+    if (!DRAFT && !whole)
+      for (int i = 0; i < gone; ++i) w = tried[i] == v ? 0.0 : w;
+    return w;
+  };
+  const int64_t lo = chunk * a.chunk, hi = min(a.vocab, lo + a.chunk);
+  auto sum_of = [&](int64_t from, int64_t to, bool whole) {
+    double s = 0.0;
+    for (int64_t v = from + tid * E; v < to; v += kThreads * E) {
+      const int m = static_cast<int>(min(static_cast<int64_t>(E), to - v));
+      const RawVec<T> pv = m == E ? load_any(p + v) : load_tail(p, v, to, T(0));
+      RawVec<T> qv = pv;
+      if (DRAFT && q) qv = m == E ? load_any(q + v) : load_tail(q, v, to, T(0));
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < m) s += weigh(pv[e], qv[e], v + e, whole);
+    }
+    s = wave_sum(s);
+    __syncthreads();
+    if (lane == 0) totals[wave] = s;
+    __syncthreads();
+    double t = 0.0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) t += totals[i];
+    return t;
+  };
+  const double mine = sum_of(lo, hi, false);
+  double* sums = a.sums + static_cast<int64_t>(b) * a.chunks;
+  if (tid == 0) {
+    __hip_atomic_store(sums + chunk, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t before =
+        __hip_atomic_fetch_add(a.arrived + b, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    last = before == static_cast<uint32_t>(a.chunks - 1);
+    if (last) __hip_atomic_store(a.arrived + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return;
+
+  // The chunk where the sum of those up to it passes the drawn point: lanes of the first
+  // wave, 64 chunks at a time.
+  auto load_sum = [&](int i) {
+    return i < a.chunks
+               ? __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+               : 0.0;
+  };
+  auto scan = [&](double v) {  // over lanes 0 .. lane
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const double o = __shfl_up(v, m, 64);
+      if (lane >= m) v += o;
+    }
+    return v;
+  };
+  double total = 0.0;
+  for (int i = 0; i < a.chunks; i += 64) total += wave_sum(load_sum(i + lane));
+  bool whole = false;
+  if (!(total > 0.0)) {
+    // Nothing is left (the target's probabilities lie below the draft's everywhere, by
+    // their rounding): the whole row.
+    whole = true;
+    total = sum_of(0, a.vocab, true);
+  }
+  if (!(total > 0.0) || !(total < __builtin_huge_val())) {
+    if (tid == 0) a.next[b] = -1;
+    return;
+  }
+  const double point = static_cast<double>(a.uniform[static_cast<int64_t>(b) * a.nodes]) * total;
+  int64_t from = 0, to = a.vocab;
+  double before = 0.0;
+  if (!whole) {
+    if (wave == 0) {
+      double run = 0.0, start = 0.0;
+      int at = -1, some = 0;
+      double some_before = 0.0;
+      for (int i = 0; i < a.chunks && at < 0; i += 64) {
+        const double v = load_sum(i + lane), upto = run + scan(v);
+        const uint64_t past = __ballot(i + lane < a.chunks && v > 0.0 && upto > point);
+        const uint64_t any = __ballot(v > 0.0);
+        if (past) {
+          const int k = __builtin_ctzll(past);
+          at = i + k, start = lane_f64(upto - v, k);
+        }
+        if (any) {
+          const int k = 63 - __builtin_clzll(any);
+          some = i + k, some_before = lane_f64(upto - v, k);
+        }
+        run = lane_f64(upto, 63);
+      }
+      // (The sums round: the last chunk that has any where none passes the point.)
+      if (lane == 0) found = at >= 0 ? at : some, found_before = at >= 0 ? start : some_before;
+    }
+    __syncthreads();
+    from = found * a.chunk, to = min(a.vocab, from + a.chunk), before = found_before;
+    __syncthreads();
+  }
+  // The token: a thread's consecutive share of the elements, the shares' sums scanned.
+  const int64_t share = (to - from + kThreads - 1) / kThreads;
+  const int64_t s0 = min(to, from + tid * share), s1 = min(to, s0 + share);
+  double s = 0.0;
+  for (int64_t v = s0; v < s1; ++v) s += weigh(p[v], DRAFT && q ? q[v] : p[v], v, whole);
+  const double upto = scan(s);
+  if (lane == 63) totals[wave] = upto;
+  if (tid == 0) found = INT32_MAX, ntried = -1;
+  __syncthreads();
+  double run = before + upto - s;
+  for (int i = 0; i < wave; ++i) run += totals[i];
+  int mine_first = INT32_MAX, mine_last = -1;
+  // (`gone` holds what ntried did.)
+  for (int64_t v = s0; v < s1; ++v) {
+    const double x = weigh(p[v], DRAFT && q ? q[v] : p[v], v, whole);
+    run += x;
+    if (x > 0.0) {
+      mine_last = static_cast<int>(v);
+      if (run > point && mine_first == INT32_MAX) mine_first = static_cast<int>(v);
+    }
+  }
+  if (mine_first != INT32_MAX) atomicMin(&found, mine_first);
+  if (mine_last >= 0) atomicMax(&ntried, mine_last);
+  __syncthreads();
+  if (tid == 0) a.next[b] = found != INT32_MAX ? found : ntried;
+}
+
+template <typename T>
+hxm_status launch_verify(const VerifyArgs& a, hipStream_t s) {
+  const int64_t groups = int64_t(a.batch) * a.chunks;
+  hxm_status st = check_grid("verify draft", groups, kThreads);
+  if (st != HXM_OK) return st;
+  const unsigned n = static_cast<unsigned>(groups);
+  if (a.draft) verify_draft_kernel<T, true><<<n, kThreads, 0, s>>>(a);
+  else verify_draft_kernel<T, false><<<n, kThreads, 0, s>>>(a);
+  return check_launch("verify draft");
+}
+
+}  // namespace
+}  // namespace hxm
+
+using namespace hxm;
+
+extern "C" hxm_status hxm_verify_draft(const int32_t* tokens, const int32_t* parents,
+                                       const void* target, int64_t ld_target, const void* draft,
+                                       int64_t ld_draft, const float* uniform, int32_t* path,
+                                       int32_t* counts, int32_t* next_tokens, int64_t batch,
+                                       int64_t nodes, int64_t vocab, int32_t dtype, void* stream) {
+  if (dtype != HXM_F16 && dtype != HXM_BF16 && dtype != HXM_F32)
+    return fail(HXM_UNSUPPORTED_DTYPE, "unsupported-dtype: verify_draft takes f16, bf16 or f32 "
+                "(got %d)", dtype);
+  if (batch < 0 || nodes < 1 || vocab < 1)
+    return fail(HXM_INVALID_ARG, "invalid-argument: verify_draft batch=%lld, nodes=%lld, vocab=%lld",
+                (long long)batch, (long long)nodes, (long long)vocab);
+  if (nodes > kMaxNodes || batch > (int64_t(1) << 20) || vocab > INT32_MAX / 2)
+    return fail(HXM_UNSUPPORTED_SHAPE,
+                "tile-alignment: verify_draft batch=%lld, nodes=%lld, vocab=%lld",
+                (long long)batch, (long long)nodes, (long long)vocab);
+  if (batch > 0 && (!tokens || !target || !uniform || !path || !counts || !next_tokens))
+    return fail(HXM_INVALID_ARG, "invalid-argument: verify_draft null operand");
+  for (const int64_t ld : {ld_target, draft ? ld_draft : vocab})
+    if (!stride_ok(ld) || (batch * nodes > 1 && ld < vocab))
+      return fail(HXM_INVALID_ARG, "invalid-argument: verify_draft ld=%lld of %lld",
+                  (long long)ld, (long long)vocab);
+  hxm_status st = require_device(nullptr);
+  if (st != HXM_OK) return st;
+  if (batch == 0) return ok();
+  VerifyArgs a{};
+  a.tokens = tokens, a.parents = parents, a.target = target, a.draft = draft;
+  a.uniform = uniform, a.ldt = ld_target, a.ldd = ld_draft, a.vocab = vocab;
+  a.path = path, a.counts = counts, a.next = next_tokens;
+  a.batch = static_cast<int>(batch), a.nodes = static_cast<int>(nodes);
+  const int64_t want = std::max(int64_t(1), kGroups / batch);
+  a.chunk = std::max(kLeastChunk, ceil_div(ceil_div(vocab, want), 64) * 64);
+  a.chunks = static_cast<int>(ceil_div(vocab, a.chunk));
+  hipStream_t s = as_stream(stream);
+  void* ws = nullptr;
+  if ((st = stream_workspace(s, static_cast<size_t>(batch) * 4, &ws, kWsCount)) != HXM_OK) return st;
+  a.arrived = static_cast<uint32_t*>(ws);
+  st = stream_workspace(s, static_cast<size_t>(batch) * a.chunks * 8, &ws, kWsLayer);
+  if (st != HXM_OK) return st;
+  a.sums = static_cast<double*>(ws);
+  if (dtype == HXM_F16) return launch_verify<_Float16>(a, s);
+  if (dtype == HXM_BF16) return launch_verify<__bf16>(a, s);
+  return launch_verify<float>(a, s);
+}

@@ -133,12 +133,12 @@ inline bool matrices_disjoint(uintptr_t a, int64_t lda, uintptr_t b, int64_t ldb
 inline bool stride_ok(int64_t s) { return s >= 0 && s <= (int64_t(1) << 40); }
 
 // Whether rows of `width` contiguous elements at strides s[0 .. dims) with
-// extents n[] (at most 4 dims) share no element: with the strides in order, each
+// extents n[] (at most 5 dims) share no element: with the strides in order, each
 // steps over everything the smaller ones span.
 inline bool strides_disjoint(const int64_t* n, const int64_t* s, int dims, int64_t width) {
   typedef __int128 wide;
-  bool used[4] = {false, false, false, false};
-  if (dims < 0 || dims > 4) return false;
+  bool used[5] = {false, false, false, false, false};
+  if (dims < 0 || dims > 5) return false;
   for (int i = 0; i < dims; ++i)
     if (n[i] <= 0) return true;
   wide span = width;
@@ -166,6 +166,16 @@ inline bool twins_disjoint(uintptr_t a, uintptr_t b, const int64_t* n, const int
   int64_t n2[4] = {2}, s2[4] = {static_cast<int64_t>(step / eb)};
   for (int i = 0; i < dims; ++i) n2[i + 1] = n[i], s2[i + 1] = s[i];
   return strides_disjoint(n2, s2, dims + 1, width);
+}
+
+// The same of arrays of 4 dims (a cache's layers, pages, heads and tokens).
+inline bool layer_twins_disjoint(uintptr_t a, uintptr_t b, const int64_t* n, const int64_t* s,
+                                 int64_t width, int64_t eb) {
+  const uintptr_t step = a < b ? b - a : a - b;
+  if (step % eb != 0) return false;
+  const int64_t n2[5] = {2, n[0], n[1], n[2], n[3]};
+  const int64_t s2[5] = {static_cast<int64_t>(step / eb), s[0], s[1], s[2], s[3]};
+  return strides_disjoint(n2, s2, 5, width);
 }
 
 // Division of n < 2^31 by a fixed d in [1, 2^31): with l = ceil(log2 d) and

@@ -60,7 +60,7 @@ constexpr int kWsMain = 0, kWsSplitK = 1, kWsStreamK = 2, kWsLayer = 3, kWsCount
 constexpr int64_t kSplitKPlaneBytesMax = int64_t(256) << 20;
 // Slot 2 holds the W8A16 stream-K partial tiles and arrival counters, slot 3 what
 // a decoder-layer operator keeps between its launches or workgroups, slot 4 the
-// arrival counters of paged attention (zero between launches).
+// arrival counters of paged attention and verify_draft (zero between launches).
 // *grown (when given) says whether the buffer was (re)allocated by this call.
 // True while `stream` captures a graph, or when that cannot be read (the null
 // stream during another stream's global-mode capture).
@@ -117,6 +117,9 @@ hxm_status pack_f32_operands(const float* A, int64_t lda, _Float16* ai, int64_t 
 hxm_status check_kv_cache(const char* op, const hxm_kv_cache* c, bool written);
 hxm_status check_heads(const char* op, const char* what, const hxm_heads* h, int64_t tokens,
                        int64_t heads, int64_t dim, bool written);
+// Whether `layers` (two and more) such caches, at these strides from c's keys and values,
+// share no element.
+bool layers_apart(const hxm_kv_cache* c, int64_t layers, int64_t kls, int64_t vls);
 // Whether the written view `out` is `in` itself, or shares nothing with it.
 bool heads_same(const hxm_heads* out, const hxm_heads* in, int64_t tokens, int64_t heads);
 bool heads_apart(const hxm_heads* out, int64_t out_heads, const hxm_heads* in, int64_t in_heads,

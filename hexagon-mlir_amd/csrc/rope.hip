@@ -143,6 +143,156 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
   }
 }
 
+// The norms of the heads in front of it: gamma and beta rows of a head, `hs` apart.
+struct HeadNorm {
+  const void *gamma, *beta;
+  int64_t hs;
+  float eps;
+  int kind;
+};
+struct NormRopeArgs : RopeArgs {
+  HeadNorm nq, nk;
+  int lanes;  // of a head: a power of two, its chunks and up
+};
+
+// The sum over the aligned group of `lanes` lanes (1 to 64) that this one is in.
+__device__ __forceinline__ float group_sum(float v, int lanes) {
+  if (lanes > 1) v += dpp<kDppQuadXor1>(v);
+  if (lanes > 2) v += dpp<kDppQuadXor2>(v);
+  if (lanes > 4) v += dpp<kDppRowHalfMirror>(v);
+  if (lanes > 8) v += dpp<kDppRowMirror>(v);
+  if (lanes > 16) v += __shfl_xor(v, 16, 64);
+  if (lanes > 32) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+
+// A head's norm, its rotation and its store in one pass over it: the lanes of a head, a
+// power of two, keep its chunks in registers as fp32 from the load to the one rounding
+// and share the statistics.  Threads of a token as above.
+template <typename T, bool PAIRS>
+__global__ __launch_bounds__(256) void norm_rope_append_kernel(NormRopeArgs a) {
+  const int t = blockIdx.x * (256 / a.tt) + static_cast<int>(threadIdx.x) / a.tt;
+  const int i = static_cast<int>(threadIdx.x) % a.tt;
+  if (t >= a.tokens) return;
+  const uint32_t slot = static_cast<uint32_t>(a.slots[t]);  // negative ones pass nslots too
+  const bool stored = slot < a.nslots;
+  const int64_t page = stored ? slot / a.page_size : 0;
+  const int64_t off = stored ? slot % a.page_size : 0;
+  T* kc = static_cast<T*>(a.kc) + page * a.kps + off * a.kts;
+  T* vc = static_cast<T*>(a.vc) + page * a.vps + off * a.vts;
+
+  const int per = a.tt / a.lanes;  // heads at a time
+  const int c = i % a.lanes;
+  const int half = a.rot / 2;
+  const bool turned = c < a.rchunks;
+  const bool two = !PAIRS && turned;  // of the half-split pairs, lo + half too
+  const int lo = turned ? c * kChunk : a.rot + (c - a.rchunks) * kChunk;
+  const int n = c < a.chunks ? min(kChunk, (turned ? (PAIRS ? a.rot : half) : a.dim) - lo) : 0;
+  constexpr int M = PAIRS ? kChunk / 2 : kChunk;  // pairs of a chunk
+  float cs[M], sn[M];
+  if (turned) {
+    const int32_t p = a.positions[t];
+    const bool good = p >= 0 && p < a.max_pos;
+    const float* row = a.cos_sin + (good ? p : 0) * a.ld_cs + (PAIRS ? lo / 2 : lo);
+    load_floats(row, PAIRS ? n / 2 : n, cs);
+    load_floats(row + half, PAIRS ? n / 2 : n, sn);
+    if (!good) {
+#pragma unroll
+      for (int e = 0; e < M; ++e) cs[e] = sn[e] = __builtin_nanf("");
+    }
+  }
+  const int heads = stored ? a.hq + a.hkv : a.hq;
+  const float count = 1.0f / static_cast<float>(a.dim);
+  // Every lane of a wave takes every turn: the sums need them all.
+  for (int h0 = 0; h0 < heads; h0 += per) {
+    const int h = h0 + i / a.lanes;
+    const bool on = h < heads && n > 0;
+    const bool isq = h < a.hq;
+    const int hh = isq ? h : h - a.hq;
+    const HeadNorm nm = isq ? a.nq : a.nk;
+    const T* src = isq ? static_cast<const T*>(a.q.p) + t * a.q.ts + hh * a.q.hs
+                       : static_cast<const T*>(a.k.p) + t * a.k.ts + hh * a.k.hs;
+    T* dst = isq ? static_cast<T*>(const_cast<void*>(a.qo.p)) + t * a.qo.ts + hh * a.qo.hs
+                 : kc + hh * a.khs;
+    float x[kChunk], y[kChunk];
+    RawVec<T> rx = RawVec<T>(T(0)), ry = rx, gx = rx, gy = rx, bx = rx, by = rx;
+    if (on) {
+      rx = load_n(src + lo, n);
+      if (two) ry = load_n(src + lo + half, n);
+      if (nm.gamma) {
+        const T* g = static_cast<const T*>(nm.gamma) + hh * nm.hs + lo;
+        gx = load_n(g, n);
+        if (two) gy = load_n(g + half, n);
+      }
+      if (nm.beta) {
+        const T* g = static_cast<const T*>(nm.beta) + hh * nm.hs + lo;
+        bx = load_n(g, n);
+        if (two) by = load_n(g + half, n);
+      }
+    }
+    // (load_n leaves zeros past n.)
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) x[e] = tof(rx[e]), y[e] = tof(ry[e]);
+    float mean = 0.0f, ss = 0.0f;
+    if (nm.kind == HXM_NORM_LAYER) {
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) mean += x[e] + y[e];
+    }
+    mean = group_sum(mean, a.lanes) * count;
+    if (nm.kind == HXM_NORM_LAYER) {
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) {
+        x[e] = e < n ? x[e] - mean : 0.0f;
+        y[e] = two && e < n ? y[e] - mean : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kChunk; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
+    ss = group_sum(ss, a.lanes) * count;
+    if (!on) continue;
+    if (nm.kind != HXM_NORM_NONE) {
+      const float r = 1.0f / sqrtf(ss + nm.eps);
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) {
+        x[e] *= r, y[e] *= r;
+        if (nm.gamma) x[e] *= tof(gx[e]), y[e] *= tof(gy[e]);
+        if (nm.beta) x[e] += tof(bx[e]), y[e] += tof(by[e]);
+      }
+    }
+    RawVec<T> ox, oy;
+    if (PAIRS && turned) {
+#pragma unroll
+      for (int e = 0; e < kChunk / 2; ++e) {
+        const int k = PAIRS ? e : 0;
+        const float u = x[2 * e], w = x[2 * e + 1];
+        ox[2 * e] = fromf<T>(fmaf(u, cs[k], -(w * sn[k])));
+        ox[2 * e + 1] = fromf<T>(fmaf(w, cs[k], u * sn[k]));
+      }
+    } else if (turned) {
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) {
+        const int k = PAIRS ? 0 : e;
+        ox[e] = fromf<T>(fmaf(x[e], cs[k], -(y[e] * sn[k])));
+        oy[e] = fromf<T>(fmaf(y[e], cs[k], x[e] * sn[k]));
+      }
+      if (isq) store_n<true>(dst + lo + half, oy, n);
+      else store_n<false>(dst + lo + half, oy, n);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) ox[e] = fromf<T>(x[e]);
+    }
+    if (isq) store_n<true>(dst + lo, ox, n);
+    else store_n<false>(dst + lo, ox, n);
+  }
+  if (!stored) return;
+  const int vch = a.dim / kChunk;
+  for (int j = i; j < a.hkv * vch; j += a.tt) {
+    const int hv = j / vch, d = (j - hv * vch) * kChunk;
+    const T* src = static_cast<const T*>(a.v.p) + t * a.v.ts + hv * a.v.hs + d;
+    store_n<false>(vc + hv * a.vhs + d, load_any(src), kChunk);
+  }
+}
+
 }  // namespace
 
 hxm_status check_heads(const char* op, const char* what, const hxm_heads* h, int64_t tokens,
@@ -201,6 +351,23 @@ static bool keys_values_apart(const hxm_kv_cache* c) {
   return twins_disjoint(k, v, n, ks, 3, c->dim, 2);
 }
 
+bool layers_apart(const hxm_kv_cache* c, int64_t layers, int64_t kls, int64_t vls) {
+  const int64_t n[4] = {layers, c->pages, c->heads, c->page_size};
+  const int64_t ks[4] = {kls, c->k_page_stride, c->k_head_stride, c->k_token_stride},
+                vs[4] = {vls, c->v_page_stride, c->v_head_stride, c->v_token_stride};
+  if (!strides_disjoint(n, ks, 4, c->dim) || !strides_disjoint(n, vs, 4, c->dim)) return false;
+  auto layer_span = [&](const int64_t* s) {
+    __int128 span = c->dim;
+    for (int i = 1; i < 4; ++i) span += static_cast<__int128>(n[i] - 1) * s[i];
+    return span < INT64_MAX ? static_cast<int64_t>(span) : INT64_MAX;
+  };
+  const uintptr_t k = reinterpret_cast<uintptr_t>(c->k), v = reinterpret_cast<uintptr_t>(c->v);
+  if (matrices_disjoint(k, kls, v, vls, layers, layer_span(ks), layer_span(vs), 2)) return true;
+  for (int i = 0; i < 4; ++i)
+    if (n[i] > 1 && ks[i] != vs[i]) return false;
+  return layer_twins_disjoint(k, v, n, ks, c->dim, 2);
+}
+
 hxm_status check_kv_cache(const char* op, const hxm_kv_cache* c, bool written) {
   if (!c || !c->k || !c->v)
     return fail(HXM_INVALID_ARG, "invalid-argument: %s null cache", op);
@@ -232,56 +399,49 @@ hxm_status check_kv_cache(const char* op, const hxm_kv_cache* c, bool written) {
   return HXM_OK;
 }
 
-}  // namespace hxm
-
-using namespace hxm;
-
-extern "C" hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q_heads,
-                                      const hxm_heads* k, const hxm_heads* v,
-                                      const int32_t* positions, const float* cos_sin,
-                                      int64_t ld_cos_sin, int64_t max_pos, int64_t rot_dim,
-                                      int32_t interleaved, const int32_t* slots,
-                                      const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
-                                      void* stream) {
+// The arguments of an append checked, and as the kernels take them.
+static hxm_status rope_args(const char* op, const hxm_heads* q, const hxm_heads* q_out,
+                            int64_t q_heads, const hxm_heads* k, const hxm_heads* v, const int32_t* positions,
+                            const float* cos_sin, int64_t ld_cos_sin, int64_t max_pos,
+                            int64_t rot_dim, int32_t interleaved, const int32_t* slots,
+                            const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
+                            RopeArgs& a) {
   if (dtype != HXM_F16 && dtype != HXM_BF16)
-    return fail(HXM_UNSUPPORTED_DTYPE, "unsupported-dtype: rope_append takes f16 or bf16 (got %d)",
-                dtype);
-  hxm_status st = check_kv_cache("rope_append", cache, true);
+    return fail(HXM_UNSUPPORTED_DTYPE, "unsupported-dtype: %s takes f16 or bf16 (got %d)",
+                op, dtype);
+  hxm_status st = check_kv_cache(op, cache, true);
   if (st != HXM_OK) return st;
   const int64_t dim = cache->dim, hkv = cache->heads;
   if (tokens < 0 || q_heads < 0)
-    return fail(HXM_INVALID_ARG, "invalid-argument: rope_append tokens=%lld q_heads=%lld",
+    return fail(HXM_INVALID_ARG, "invalid-argument: %s tokens=%lld q_heads=%lld", op,
                 (long long)tokens, (long long)q_heads);
   if (tokens > INT32_MAX / 2 || q_heads > 65535)
-    return fail(HXM_UNSUPPORTED_SHAPE, "tile-alignment: rope_append tokens=%lld q_heads=%lld",
+    return fail(HXM_UNSUPPORTED_SHAPE, "tile-alignment: %s tokens=%lld q_heads=%lld", op,
                 (long long)tokens, (long long)q_heads);
   if (rot_dim < 0 || rot_dim > dim || rot_dim % 2 != 0)
-    return fail(HXM_INVALID_ARG, "invalid-argument: rope_append rot_dim=%lld of %lld dims",
+    return fail(HXM_INVALID_ARG, "invalid-argument: %s rot_dim=%lld of %lld dims", op,
                 (long long)rot_dim, (long long)dim);
-  if ((st = check_heads("rope_append", "k", k, tokens, hkv, dim, false)) != HXM_OK) return st;
-  if ((st = check_heads("rope_append", "v", v, tokens, hkv, dim, false)) != HXM_OK) return st;
+  if ((st = check_heads(op, "k", k, tokens, hkv, dim, false)) != HXM_OK) return st;
+  if ((st = check_heads(op, "v", v, tokens, hkv, dim, false)) != HXM_OK) return st;
   if (q_heads > 0) {
-    if ((st = check_heads("rope_append", "q", q, tokens, q_heads, dim, false)) != HXM_OK) return st;
-    if ((st = check_heads("rope_append", "q_out", q_out, tokens, q_heads, dim, true)) != HXM_OK)
+    if ((st = check_heads(op, "q", q, tokens, q_heads, dim, false)) != HXM_OK) return st;
+    if ((st = check_heads(op, "q_out", q_out, tokens, q_heads, dim, true)) != HXM_OK)
       return st;
   }
   if (rot_dim > 0 && (max_pos < 1 || !stride_ok(ld_cos_sin) || ld_cos_sin < rot_dim))
-    return fail(HXM_INVALID_ARG, "invalid-argument: rope_append max_pos=%lld ld_cos_sin=%lld",
+    return fail(HXM_INVALID_ARG, "invalid-argument: %s max_pos=%lld ld_cos_sin=%lld", op,
                 (long long)max_pos, (long long)ld_cos_sin);
   if (tokens > 0 && (!slots || (rot_dim > 0 && (!positions || !cos_sin))))
     return fail(HXM_INVALID_ARG,
-                "invalid-argument: rope_append null slots, positions or cos_sin");
+                "invalid-argument: %s null slots, positions or cos_sin", op);
   if (q_heads > 0 && tokens > 0) {
     if ((!heads_same(q_out, q, tokens, q_heads) &&
          !heads_apart(q_out, q_heads, q, q_heads, tokens, dim)) ||
         !heads_apart(q_out, q_heads, k, hkv, tokens, dim) ||
         !heads_apart(q_out, q_heads, v, hkv, tokens, dim))
       return fail(HXM_INVALID_ARG,
-                  "invalid-argument: rope_append q_out overlaps q (without being it), k or v");
+                  "invalid-argument: %s q_out overlaps q (without being it), k or v", op);
   }
-  if ((st = require_device(nullptr)) != HXM_OK) return st;
-  if (tokens == 0) return ok();
-  RopeArgs a{};
   if (q_heads > 0) {
     a.q = {q->data, q->token_stride, q->head_stride};
     a.qo = {q_out->data, q_out->token_stride, q_out->head_stride};
@@ -299,6 +459,25 @@ extern "C" hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out
   a.hkv = static_cast<int>(hkv), a.dim = static_cast<int>(dim), a.rot = static_cast<int>(rot_dim);
   a.rchunks = static_cast<int>(ceil_div(interleaved ? rot_dim : rot_dim / 2, kChunk));
   a.chunks = a.rchunks + static_cast<int>(ceil_div(dim - rot_dim, kChunk));
+  return HXM_OK;
+}
+
+}  // namespace hxm
+
+using namespace hxm;
+
+extern "C" hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q_heads,
+                                      const hxm_heads* k, const hxm_heads* v,
+                                      const int32_t* positions, const float* cos_sin,
+                                      int64_t ld_cos_sin, int64_t max_pos, int64_t rot_dim,
+                                      int32_t interleaved, const int32_t* slots,
+                                      const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
+                                      void* stream) {
+  RopeArgs a{};
+  hxm_status st = rope_args("rope_append", q, q_out, q_heads, k, v, positions, cos_sin, ld_cos_sin,
+                            max_pos, rot_dim, interleaved, slots, cache, tokens, dtype, a);
+  if (st != HXM_OK || (st = require_device(nullptr)) != HXM_OK) return st;
+  if (tokens == 0) return ok();
   // Threads of a token: one for each chunk it has, a power of two from 64 to
   // a workgroup's 256, or 128 once the tokens fill the chip that way (a head has at
   // most 33 chunks).  32 + 8 heads of 128: 8192 tokens 42.7 us with 256, 41.2 with 128, 46
@@ -317,4 +496,47 @@ extern "C" hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out
     interleaved ? rope_append_kernel<__bf16, true><<<g, 256, 0, s>>>(a)
                 : rope_append_kernel<__bf16, false><<<g, 256, 0, s>>>(a);
   return check_launch("rope append");
+}
+
+extern "C" hxm_status hxm_norm_rope_append(const hxm_heads* q, const hxm_heads* q_out,
+                                           int64_t q_heads, const hxm_heads* k, const hxm_heads* v,
+                                           const hxm_head_norm* q_norm, const hxm_head_norm* k_norm,
+                                           const int32_t* positions, const float* cos_sin,
+                                           int64_t ld_cos_sin, int64_t max_pos, int64_t rot_dim,
+                                           int32_t interleaved, const int32_t* slots,
+                                           const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
+                                           void* stream) {
+  NormRopeArgs a{};
+  hxm_status st = rope_args("norm_rope_append", q, q_out, q_heads, k, v, positions, cos_sin,
+                            ld_cos_sin, max_pos, rot_dim, interleaved, slots, cache, tokens, dtype,
+                            a);
+  if (st != HXM_OK) return st;
+  for (const bool isq : {true, false}) {
+    if (isq && q_heads == 0) continue;
+    const hxm_head_norm* m = isq ? q_norm : k_norm;
+    if (!m || m->kind < HXM_NORM_NONE || m->kind > HXM_NORM_LAYER || !(m->eps >= 0.0f) ||
+        !stride_ok(m->head_stride) || (m->head_stride > 0 && m->head_stride < cache->dim) ||
+        (m->kind == HXM_NORM_NONE && (m->gamma || m->beta)))
+      return fail(HXM_INVALID_ARG, "invalid-argument: norm_rope_append norm of %s",
+                  isq ? "q" : "k");
+    (isq ? a.nq : a.nk) = HeadNorm{m->gamma, m->beta, m->head_stride, m->eps, m->kind};
+  }
+  if ((st = require_device(nullptr)) != HXM_OK) return st;
+  if (tokens == 0) return ok();
+  a.lanes = 1;
+  while (a.lanes < a.chunks) a.lanes *= 2;
+  a.tt = 64;
+  const int most = tokens >= 2048 ? 128 : 256;
+  while (a.tt < most && a.tt < a.lanes * (a.hq + a.hkv)) a.tt *= 2;
+  const int64_t groups = ceil_div(tokens, 256 / a.tt);
+  if ((st = check_grid("norm rope append", groups, 256)) != HXM_OK) return st;
+  const unsigned g = static_cast<unsigned>(groups);
+  hipStream_t s = as_stream(stream);
+  if (dtype == HXM_F16)
+    interleaved ? norm_rope_append_kernel<_Float16, true><<<g, 256, 0, s>>>(a)
+                : norm_rope_append_kernel<_Float16, false><<<g, 256, 0, s>>>(a);
+  else
+    interleaved ? norm_rope_append_kernel<__bf16, true><<<g, 256, 0, s>>>(a)
+                : norm_rope_append_kernel<__bf16, false><<<g, 256, 0, s>>>(a);
+  return check_launch("norm rope append");
 }

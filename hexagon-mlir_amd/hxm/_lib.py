@@ -84,6 +84,7 @@ class Plan(ctypes.Structure):
 # (a call packs them anew each time: a tenth of what building a ctypes.Structure
 # of their fields takes).
 ROW_NORM = struct.Struct("@ifPP")   # hxm_row_norm: kind, eps, gamma, beta
+HEAD_NORM = struct.Struct("@ifPPq")  # hxm_head_norm: kind, eps, gamma, beta, head stride
 HEADS = struct.Struct("@Pqq")       # hxm_heads: data, token stride, head stride
 KV_CACHE = struct.Struct("@PP10q")  # hxm_kv_cache: k, v, pages, page_size, heads, dim, strides
 
@@ -153,8 +154,17 @@ SIGNATURES = {
                                      _p, _i64, _p, _i64, _i64, _i64, _i32, _p]),
     "hxm_rope_append": (_st, [_p, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _p, _p, _i64,
                               _i32, _p]),
+    "hxm_norm_rope_append": (_st, [_p, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32,
+                                   _p, _p, _i64, _i32, _p]),
     "hxm_paged_attention": (_st, [_p, _p, _i64, _p, _p, _i64, _i64, _p, _i64, _f32, _i64, _p,
                                   _i32, _p]),
+    "hxm_tree_attention": (_st, [_p, _p, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _f32, _i64,
+                                 _p, _i32, _p]),
+    "hxm_verify_draft": (_st, [_p, _p, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i32,
+                               _p]),
+    "hxm_compact_cache": (_st, [_p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _i64, _i64,
+                                _i32, _p]),
+    "hxm_copy_pages": (_st, [_p, _i64, _i64, _i64, _p, _p, _p, _i64, _i32, _p]),
     "hxm_lora_add": (_st, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64,
                            _i64, _i32, _p]),
     "hxm_probe_copy": (_st, [_p, _p, _i64, _p]),

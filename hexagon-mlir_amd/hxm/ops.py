@@ -16,7 +16,7 @@ from typing import Optional, Sequence
 import torch
 
 from ._lib import (B_KN, B_NK, BF16, F16, F32, I8, I32, IMAGE_GEMM, IMAGE_W8A16, NORM_LAYER,
-                   HEADS, KV_CACHE, NORM_NONE, NORM_RMS, OP_W8A16, OP_W8A16_SWIGLU, ROW_NORM,
+                   HEAD_NORM, HEADS, KV_CACHE, NORM_NONE, NORM_RMS, OP_W8A16, OP_W8A16_SWIGLU, ROW_NORM,
                    W_NK, W_PACKED, GemmConfig, HxmError, check, lib)
 
 _DT = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32,
@@ -791,6 +791,12 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     then sines) rotate the first rot_dim dims, in halves or (``interleaved``)
     in neighbouring pairs; without cos_sin nothing is rotated.  ``q_out`` may be
     q."""
+    return _append("hxm_rope_append", q, k, v, k_cache, v_cache, slots, positions, cos_sin,
+                   interleaved, q_out, None)
+
+
+def _append(entry, q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved, q_out, norms):
+    """The call of either append; norms: (kind, eps, q_weight, q_bias, k_weight, k_bias)."""
     cache, heads, dim, dtype, dev = _kv_cache(k_cache, v_cache)
     if k.dim() != 3:
         raise ValueError(f"k must be [tokens, heads, dim] (got {tuple(k.shape)})")
@@ -822,12 +828,75 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         oh = _heads(q_out, dtype, (T, hq, dim), dev, "q_out")
     elif q_out is not None:
         raise ValueError("q_out needs q")
-    st = lib.hxm_rope_append(qh, oh, hq, kh, vh, pos_p, tab_p, ld, max_pos, rot,
-                             int(interleaved), slot_p, cache, T, _DT[dtype],
-                             _current_stream(dev))
+    if norms is None:
+        st = lib.hxm_rope_append(qh, oh, hq, kh, vh, pos_p, tab_p, ld, max_pos, rot,
+                                 int(interleaved), slot_p, cache, T, _DT[dtype],
+                                 _current_stream(dev))
+    else:
+        kind, eps, qw, qb, kw, kb = norms
+        qn, *keep_q = _head_norm(kind, eps, qw, qb, hq, dim, dtype, dev, "q")
+        kn, *keep_k = _head_norm(kind, eps, kw, kb, heads, dim, dtype, dev, "k")
+        st = lib.hxm_norm_rope_append(qh, oh, hq, kh, vh, qn, kn, pos_p, tab_p, ld, max_pos, rot,
+                                      int(interleaved), slot_p, cache, T, _DT[dtype],
+                                      _current_stream(dev))
     if st:
-        check(st, "hxm_rope_append")
+        check(st, entry)
     return q_out
+
+
+def _head_norm(kind: str, eps: float, weight, bias, heads: int, dim: int, dtype, dev: int,
+               name: str):
+    """The hxm_head_norm, and the tensors it points to (to be kept until the call)."""
+    if kind not in _NORMS:
+        raise ValueError(f"norm must be one of {sorted(_NORMS)} (got {kind!r})")
+    each = any(t is not None and t.dim() == 2 for t in (weight, bias))
+    ptrs, keep = [], []
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            ptrs.append(0)
+            continue
+        if t.shape != ((heads, dim) if each else (dim,)) or t.dtype != dtype or \
+                t.get_device() != dev:
+            raise ValueError(f"{name}_{what} must be {dtype} [{dim}] or [{heads}, {dim}], like its "
+                             f"{'bias' if what == 'weight' else 'weight'}, on cuda:{dev} "
+                             f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
+        t = t.contiguous()
+        keep.append(t)
+        ptrs.append(t.data_ptr())
+    return (HEAD_NORM.pack(_NORMS[kind], eps, *ptrs, dim if each else 0), *keep)
+
+
+@_on_stream
+def norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                     k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                     positions: Optional[torch.Tensor] = None,
+                     cos_sin: Optional[torch.Tensor] = None, *, norm: str = "rms",
+                     q_weight: Optional[torch.Tensor] = None,
+                     k_weight: Optional[torch.Tensor] = None,
+                     q_bias: Optional[torch.Tensor] = None,
+                     k_bias: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                     interleaved: bool = False,
+                     q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """:func:`rope_append` with the norm of each query and key head ("rms" or
+    "layer" over its D elements) in front of the rotation, in the same pass
+    (hxm_norm_rope_append).  Weights and biases of the inputs' dtype: [D] for all
+    heads, or [heads, D]; without one it is 1 / 0."""
+    return _append("hxm_norm_rope_append", q, k, v, k_cache, v_cache, slots, positions, cos_sin,
+                   interleaved, q_out, (norm, eps, q_weight, q_bias, k_weight, k_bias))
+
+
+
+
+def _block_table(t: torch.Tensor, batch: int, dev: int):
+    """(address, row stride, columns) of an int32 [batch, table_pages] table."""
+    _mat(t, "block_table")
+    if t.dtype != torch.int32:
+        raise TypeError(f"block_table must be torch.int32 (got {t.dtype})")
+    rows, table_pages = t.shape
+    if rows != batch or t.get_device() != dev:
+        raise ValueError(f"block_table must have {batch} rows on cuda:{dev} "
+                         f"(got {tuple(t.shape)} on {t.device})")
+    return t.data_ptr(), _ld(t), table_pages
 
 
 @_on_stream
@@ -851,24 +920,161 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     oh = _heads(out, dtype, (B, hq, dim), dev, "out")
-    _mat(block_table, "block_table")
-    if block_table.dtype != torch.int32:
-        raise TypeError(f"block_table must be torch.int32 (got {block_table.dtype})")
-    rows, table_pages = block_table.shape
-    if rows != B or block_table.get_device() != dev:
-        raise ValueError(f"block_table must have {B} rows on cuda:{dev} "
-                         f"(got {tuple(block_table.shape)} on {block_table.device})")
+    table_p, ld_table, table_pages = _block_table(block_table, B, dev)
     lens_p = _ints(seq_lens, (B,), dev, "seq_lens")
     lse = lse_p = None
     if return_lse:
         lse = torch.empty(B, hq, dtype=torch.float32, device=q.device)
         lse_p = lse.data_ptr()
-    st = lib.hxm_paged_attention(qh, oh, hq, cache, block_table.data_ptr(), _ld(block_table),
-                                 table_pages, lens_p, B, dim ** -0.5 if scale is None else scale,
+    st = lib.hxm_paged_attention(qh, oh, hq, cache, table_p, ld_table, table_pages, lens_p, B, dim ** -0.5 if scale is None else scale,
                                  window, lse_p, _DT[dtype], _current_stream(dev))
     if st:
         check(st, "hxm_paged_attention")
     return (out, lse) if return_lse else out
+
+
+@_on_stream
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   block_table: torch.Tensor, seq_lens: torch.Tensor,
+                   parents: Optional[torch.Tensor] = None, *, scale: Optional[float] = None,
+                   window: int = 0, out: Optional[torch.Tensor] = None,
+                   return_lse: bool = False):
+    """Attention of a tree of drafted tokens per sequence over a paged cache
+    (hxm_tree_attention): q [B, T, Hq, D] f16 / bf16, T (up to 64) tokens of each
+    sequence, which are the last of its ``seq_lens`` tokens in the caches
+    (:func:`paged_attention` describes those).  ``parents`` int32 [B, T]: the
+    token before each in its branch, an earlier one of the T or -1 for the
+    context; -2 marks padding (zeros, -inf in lse); None is a chain.  A token
+    sees the context, itself and the tokens above it, ``window`` (0: all) the
+    nearest of them.  Returns out, or (out, lse) with lse fp32 [B, T, Hq]."""
+    cache, _, dim, dtype, dev = _kv_cache(k_cache, v_cache)
+    if q.dim() != 4:
+        raise ValueError(f"q must be [batch, tokens, heads, dim] (got {tuple(q.shape)})")
+    B, T, hq, _ = q.shape
+    qh = _heads(_tokens(q, "q"), dtype, (B * T, hq, dim), dev, "q")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape:
+        _tensor(out, dtype, q.shape, dev, "out")
+    oh = _heads(_tokens(out, "out"), dtype, (B * T, hq, dim), dev, "out")
+    table_p, ld_table, table_pages = _block_table(block_table, B, dev)
+    lens_p = _ints(seq_lens, (B,), dev, "seq_lens")
+    parents_p = None if parents is None else _ints(parents, (B, T), dev, "parents")
+    lse = lse_p = None
+    if return_lse:
+        lse = torch.empty(B, T, hq, dtype=torch.float32, device=q.device)
+        lse_p = lse.data_ptr()
+    st = lib.hxm_tree_attention(qh, oh, hq, cache, table_p, ld_table, table_pages, lens_p,
+                                parents_p, B, T, dim ** -0.5 if scale is None else scale, window,
+                                lse_p, _DT[dtype], _current_stream(dev))
+    if st:
+        check(st, "hxm_tree_attention")
+    return (out, lse) if return_lse else out
+
+
+def _tokens(t: torch.Tensor, name: str) -> torch.Tensor:
+    """[batch, tokens, heads, dim] as [batch * tokens, heads, dim], without a copy."""
+    try:
+        return t.view(-1, *t.shape[2:]) if t.shape[0] and t.shape[1] else t.flatten(0, 1)
+    except RuntimeError:
+        raise ValueError(f"{name}'s tokens must be evenly strided over the batch") from None
+
+
+@_on_stream
+def verify_draft(tokens: torch.Tensor, target: torch.Tensor, uniform: torch.Tensor,
+                 parents: Optional[torch.Tensor] = None, draft: Optional[torch.Tensor] = None):
+    """Which drafted tokens the target's probabilities keep, and the token that
+    follows them (hxm_verify_draft, which has the rule): returns (path [B, T],
+    counts [B], next_tokens [B]), int32.
+
+    ``tokens`` int32 [B, T] (up to 64), the first the last token sampled before;
+    ``parents`` as :func:`tree_attention` takes them (None: chains).  ``target``
+    [B, T, V] holds the target's probabilities after each token, ``draft`` those
+    that its child was drawn from (of one child each; None: children chosen
+    without chance), f16, bf16 or f32; ``uniform`` fp32 [B, T] random numbers, the
+    first of a sequence for the token that follows."""
+    dev = _on_current(target, "target")
+    if target.dim() != 3:
+        raise ValueError(f"target must be [batch, tokens, vocab] (got {tuple(target.shape)})")
+    B, T, V = target.shape
+    dtype = target.dtype
+    _dtype(target, _FLOATS, "target")
+    tokens_p = _ints(tokens, (B, T), dev, "tokens")
+    parents_p = None if parents is None else _ints(parents, (B, T), dev, "parents")
+    if not _tensor(uniform, torch.float32, (B, T), dev, "uniform").is_contiguous():
+        raise ValueError("uniform must be contiguous")
+    t2 = _mat(_tokens(target, "target"), "target")
+    draft_p, ldd = None, 0
+    if draft is not None:
+        d2 = _mat(_tokens(_tensor(draft, dtype, (B, T, V), dev, "draft"), "draft"), "draft")
+        draft_p, ldd = d2.data_ptr(), _row_ld(d2, B * T, V)
+    out = torch.empty(B * T + 2 * B, dtype=torch.int32, device=target.device)
+    path, counts, following = out[:B * T].view(B, T), out[B * T:B * T + B], out[B * T + B:]
+    at = out.data_ptr()
+    st = lib.hxm_verify_draft(tokens_p, parents_p, t2.data_ptr(), _row_ld(t2, B * T, V), draft_p,
+                              ldd, uniform.data_ptr(), at, at + 4 * B * T, at + 4 * B * (T + 1), B,
+                              T, V, _DT[dtype], _current_stream(dev))
+    if st:
+        check(st, "hxm_verify_draft")
+    return path, counts, following
+
+
+def _kv_layers(k: torch.Tensor, v: torch.Tensor):
+    """(hxm_kv_cache of the first layer, layers, their strides, dtype, device) of
+    [layers, pages, heads, page_size, dim] caches, or of one layer's."""
+    if k.dim() == 4:
+        cache, _, _, dtype, dev = _kv_cache(k, v)
+        return cache, 1, 0, 0, dtype, dev
+    if k.dim() != 5 or v.shape != k.shape or not k.shape[0]:
+        raise ValueError("k_cache and v_cache must be [pages, heads, page_size, dim], or with a "
+                         f"dimension of layers before (got {tuple(k.shape)}, {tuple(v.shape)})")
+    cache, _, _, dtype, dev = _kv_cache(k[0], v[0])
+    return cache, k.shape[0], k.stride(0), v.stride(0), dtype, dev
+
+
+@_on_stream
+def compact_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                  seq_lens: torch.Tensor, path: torch.Tensor,
+                  counts: torch.Tensor) -> torch.Tensor:
+    """The rows of the kept tokens moved behind the context in all layers' caches
+    (hxm_compact_cache): returns the sequences' new lengths, int32 [B].
+
+    The caches are [layers, pages, Hkv, page_size, D] (or one layer's, without the
+    first dimension), f16 / bf16, any strides; ``block_table`` and ``seq_lens`` as
+    :func:`tree_attention` takes them, ``path`` int32 [B, T] and ``counts`` int32
+    [B] as :func:`verify_draft` gives them."""
+    cache, layers, kls, vls, dtype, dev = _kv_layers(k_cache, v_cache)
+    if path.dim() != 2:
+        raise ValueError(f"path must be [batch, tokens] (got {tuple(path.shape)})")
+    B, T = path.shape
+    path_p = _ints(path, (B, T), dev, "path")
+    counts_p = _ints(counts, (B,), dev, "counts")
+    lens_p = _ints(seq_lens, (B,), dev, "seq_lens")
+    table_p, ld_table, table_pages = _block_table(block_table, B, dev)
+    lens = torch.empty(B, dtype=torch.int32, device=path.device)
+    st = lib.hxm_compact_cache(cache, layers, kls, vls, table_p, ld_table, table_pages, lens_p,
+                               path_p, counts_p, lens.data_ptr(), B, T, _DT[dtype],
+                               _current_stream(dev))
+    if st:
+        check(st, "hxm_compact_cache")
+    return lens
+
+
+@_on_stream
+def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+               rows: Optional[torch.Tensor] = None) -> None:
+    """Pages copied in all layers' caches (hxm_copy_pages; the caches as
+    :func:`compact_cache` takes them), for sequences that fork: page ``dst``[i]
+    receives page ``src``[i], or its first ``rows``[i] tokens.  int32 [N] each; -1
+    marks padding.  No page may be one pair's dst and another's src or dst."""
+    cache, layers, kls, vls, dtype, dev = _kv_layers(k_cache, v_cache)
+    N = src.numel()
+    src_p, dst_p = _ints(src, (N,), dev, "src"), _ints(dst, (N,), dev, "dst")
+    rows_p = None if rows is None else _ints(rows, (N,), dev, "rows")
+    st = lib.hxm_copy_pages(cache, layers, kls, vls, src_p, dst_p, rows_p, N, _DT[dtype],
+                            _current_stream(dev))
+    if st:
+        check(st, "hxm_copy_pages")
 
 
 @_on_stream

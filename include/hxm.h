@@ -575,6 +575,30 @@ hxm_status hxm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q
                            const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
                            void* stream);
 
+/* Norm of each head of q or k: kind and eps as in hxm_row_norm, over the head's
+ * dim elements; gamma and beta of the heads' dtype, or NULL for 1 / 0: [dim] for
+ * all heads (head_stride 0), or a row for each head, head_stride >= dim apart. */
+typedef struct hxm_head_norm {
+  int32_t kind;
+  float eps; /* >= 0 */
+  const void* gamma;
+  const void* beta;
+  int64_t head_stride;
+} hxm_head_norm;
+
+/* hxm_rope_append with the norms of the query and key heads in the same pass:
+ * q[t] and k[t] are normed head by head, then rotated; v is stored as it is.
+ * fp32 from the load to the one rounding.  Everything else as there (q_norm is
+ * not read with q_heads 0). */
+hxm_status hxm_norm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q_heads,
+                                const hxm_heads* k, const hxm_heads* v,
+                                const hxm_head_norm* q_norm, const hxm_head_norm* k_norm,
+                                const int32_t* positions, const float* cos_sin,
+                                int64_t ld_cos_sin, int64_t max_pos, int64_t rot_dim,
+                                int32_t interleaved, const int32_t* slots,
+                                const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
+                                void* stream);
+
 /* Attention of one new token per sequence over a paged cache:
  *   out[b,h,:] = sum_t softmax_t(scale * q[b,h,:] . K[t,h',:]) V[t,h',:],
  *   h' = h / (q_heads / cache->heads),
@@ -602,6 +626,90 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
                                int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
                                int64_t batch, float scale, int64_t window, float* lse,
                                int32_t dtype, void* stream);
+
+/* Attention of a tree of drafted tokens per sequence over a paged cache.  The
+ * nodes (1 to 64) of a sequence are the last of its seq_lens[b] = n tokens in
+ * the cache, node i at offset ctx + i, ctx = n - nodes.  Node i's parent is
+ * parents[b, i] (int32 [batch, nodes]): -1, the context, or a node before it;
+ * below -1 marks padding.  NULL: a chain, each node the one before's child.
+ * With d(i) the number of nodes above i,
+ *   out[b * nodes + i, h, :] = sum_t softmax_t(scale * q . K[t,h',:]) V[t,h',:],
+ *   h' = h / (q_heads / cache->heads),
+ * over the context's tokens t < ctx, node i and those above it; with a window
+ * (0: none) only those at positions (ctx + d for a node) above ctx + d(i) -
+ * window.  q, out: row b * nodes + i.  lse (fp32 [batch, nodes, q_heads], or
+ * NULL) as in hxm_paged_attention, which one node per sequence equals.  A
+ * padded node, and a sequence without tokens (n <= 0), give zeros, and -inf in
+ * lse.  What the cache holds where a node does not look (NaN included) never
+ * reaches it, nor do table entries past a sequence's last page.  NaN are: the
+ * outputs of a node whose parent (or one above) is padding or no node before
+ * it; of nodes that see a token of a page outside [0, pages); of a sequence of 0 <
+ * n < nodes tokens, or of more than table_pages * page_size or 2^30.  dtype F16
+ * or BF16, one for q, cache and out; precision as in hxm_paged_attention.  out
+ * must not overlap q; out and lse nothing else.  Sequences are split over
+ * workgroups (in batches of up to 256) and joined in a fixed order.  Uses the
+ * per-stream workspace where table_pages * page_size is 481 or more. */
+hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
+                              const hxm_kv_cache* cache, const int32_t* block_table,
+                              int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
+                              const int32_t* parents, int64_t batch, int64_t nodes, float scale,
+                              int64_t window, float* lse, int32_t dtype, void* stream);
+
+/* Which drafted tokens the target's probabilities keep, and the token that
+ * follows them.  The nodes (1 to 64) of a sequence and their parents are those of
+ * hxm_tree_attention: node 0 (parent -1) is the last token sampled before and
+ * always kept, parents[b, i] in [0, i) the node before i in its branch, anything
+ * else no branch; a sequence whose parents[b, 0] is not -1 has no tokens (counts
+ * 0, next_tokens -1).  NULL: chains.  tokens int32 [batch, nodes]; target
+ * [batch * nodes, vocab] (ld_target) holds in row b * nodes + i the target's
+ * probabilities p of the token after node i, draft (or NULL) likewise the
+ * probabilities q that node i's child was drawn from; uniform fp32 [batch,
+ * nodes] random numbers in [0, 1).  From node 0 on, the children x of a node are
+ * tried in their order, the first with
+ *   uniform[b, x] * q(token x) * left < p(token x)
+ * is kept and the walk goes on from it.  With draft, only a node's first child
+ * is tried (left 1), and what is left where it is not kept is max(p - q, 0).
+ * Without, q is 1 (tokens chosen without chance), left is 1 less p of the
+ * children tried before, and what is left is p without them; a token that an
+ * earlier child had is not tried again.  At the node where no child is kept,
+ * next_tokens[b] is the first token where the running sum w of what is left (of p
+ * without children) passes uniform[b, 0] * sum w; where nothing is left, of p;
+ * -1 where p has no finite sum above 0.  path int32 [batch, nodes] receives the
+ * kept nodes in order, then -1; counts int32 [batch] how many.  A token outside
+ * [0, vocab) is never kept nor tried.  Probabilities below 0 and NaN count as 0.
+ * Products and sums are fp64.  dtype F16, BF16 or F32, of target and draft.
+ * Outputs must overlap nothing else.  Uses the per-stream workspace. */
+hxm_status hxm_verify_draft(const int32_t* tokens, const int32_t* parents, const void* target,
+                            int64_t ld_target, const void* draft, int64_t ld_draft,
+                            const float* uniform, int32_t* path, int32_t* counts,
+                            int32_t* next_tokens, int64_t batch, int64_t nodes, int64_t vocab,
+                            int32_t dtype, void* stream);
+
+/* The rows of the kept nodes moved behind the context, in the caches of all layers:
+ * with ctx = seq_lens[b] - nodes, the row at offset ctx + path[b, k] of sequence b
+ * goes to ctx + k, k < counts[b] (path and counts as hxm_verify_draft gives
+ * them, as if all were read before any is written), and lens_out[b] (int32, or
+ * NULL) receives ctx + counts[b].  cache is the first layer's, the others lie
+ * k_layer_stride and v_layer_stride elements on.  A sequence of fewer than nodes
+ * tokens or more than table_pages * page_size, whose counts are not in [0,
+ * nodes] or whose path does not ascend in [0, nodes), is left as it is, and
+ * lens_out[b] is its length; a row from or to a page outside [0, pages) does not
+ * move.  The drafted tokens' pages must be each sequence's own.  dtype F16 or
+ * BF16.  lens_out overlaps nothing else. */
+hxm_status hxm_compact_cache(const hxm_kv_cache* cache, int64_t layers, int64_t k_layer_stride,
+                             int64_t v_layer_stride, const int32_t* block_table,
+                             int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
+                             const int32_t* path, const int32_t* counts, int32_t* lens_out,
+                             int64_t batch, int64_t nodes, int32_t dtype, void* stream);
+
+/* Pages of the caches of all layers copied, for sequences that fork: page dst[i]
+ * receives the first rows[i] tokens (rows int32 [count] or NULL: all of them) of
+ * page src[i], i < count.  A pair with a page outside [0, pages), -1 by custom,
+ * is padding.  A page that is one pair's dst must not be another's src or dst (either content
+ * may end there, element by element).  Layers as in hxm_compact_cache. */
+hxm_status hxm_copy_pages(const hxm_kv_cache* cache, int64_t layers, int64_t k_layer_stride,
+                          int64_t v_layer_stride, const int32_t* src, const int32_t* dst,
+                          const int32_t* rows, int64_t count, int32_t dtype, void* stream);
 
 /* Low-rank adapters of many requests beside a projection they share:
  *   out[m,:] = y[m,:] + scale[a] * (x[m,:] A[a]^T) B[a]^T,  a = index[m]
