@@ -975,7 +975,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 def _tokens(t: torch.Tensor, name: str) -> torch.Tensor:
     """[batch, tokens, heads, dim] as [batch * tokens, heads, dim], without a copy."""
     try:
-        return t.view(-1, *t.shape[2:]) if t.shape[0] and t.shape[1] else t.flatten(0, 1)
+        return t.view(t.shape[0] * t.shape[1], *t.shape[2:])
     except RuntimeError:
         raise ValueError(f"{name}'s tokens must be evenly strided over the batch") from None
 
