@@ -78,39 +78,32 @@ __device__ __forceinline__ End walk(const VerifyArgs& a, int b, int lane) {
     if (DRAFT) q = prob(static_cast<const T*>(a.draft)[row * a.ldd + token]);
   }
   if (!child) parent = -1;
-  // Brothers in order: what the older ones of other tokens leave (they were not kept), and
-  // whether one of them had this token.
+  // From node to node; a node's children in their order.
+  const double bound = u * q;
+  r.node = 0, r.kept = 1, r.count = 1;
   double left = 1.0;
-  bool again = false, older = false;
-  for (int j = 1; j < a.nodes; ++j) {
-    const int pj = __builtin_amdgcn_readlane(parent, j);
-    if (pj < 0) continue;
-    const bool brother = child && lane > j && parent == pj;
-    older |= brother;
+  for (uint64_t children = __ballot(parent == 0); children;) {
+    const int c = __builtin_ctzll(children);
+    const uint64_t bit = children & (0 - children);
+    children ^= bit;
     if (!DRAFT) {
-      const int tj = __builtin_amdgcn_readlane(token, j);
-      const bool fresh_j = __builtin_amdgcn_readlane(static_cast<int>(again), j) == 0;
-      const double p_j = lane_f64(p, j);
-      again |= brother && token == tj;
-      if (brother && fresh_j) left -= p_j;
+      const int tc = __builtin_amdgcn_readlane(token, c);
+      const uint64_t same = __ballot(token == tc) & r.tried;
+      r.tried |= bit;
+      if (same) continue;
     }
-  }
-  const bool ok = child && (DRAFT ? !older : !again) && u * q * left < p;
-  const uint64_t oks = __ballot(ok), firsts = __ballot(child && !older);
-  int node = 0;
-  r.kept = 1, r.count = 1;
-  while (true) {
-    const uint64_t children = __ballot(child && parent == node);
-    const uint64_t good = children & oks;
-    if (!good) {
-      r.tried = DRAFT ? children & firsts : children;
+    const double pc = lane_f64(p, c);
+    if (lane_f64(bound, c) * left < pc) {
+      r.node = c, r.kept |= bit, ++r.count;
+      r.tried = 0, left = 1.0;
+      children = __ballot(parent == c);
+    } else if (DRAFT) {
+      r.tried = bit;
       break;
+    } else {
+      left -= pc;
     }
-    node = __builtin_ctzll(good);
-    r.kept |= uint64_t(1) << node;
-    ++r.count;
   }
-  r.node = node;
   return r;
 }
 
@@ -126,8 +119,8 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
   const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = threadIdx.x;
   __shared__ double totals[kThreads / 64];
-  __shared__ int32_t tried[kMaxNodes];
-  __shared__ int ntried, last;
+  __shared__ int32_t gone[kMaxNodes];
+  __shared__ int furthest, last;
   __shared__ double found_before;
   __shared__ int found;
 
@@ -145,37 +138,47 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
     if (lane == 0 && end.node < 0) a.next[b] = -1;
   }
   if (end.node < 0) return;
-  // Tokens that are gone from the row (a one-hot draft's), by their order.
-  if (wave == 0) {
-    if ((end.tried >> lane) & 1)
-      tried[__builtin_popcountll(end.tried & ((uint64_t(1) << lane) - 1))] = end.token;
-    if (lane == 0) ntried = __builtin_popcountll(end.tried);
-  }
-  __syncthreads();
+  // The tokens in [from, to) that are gone from the row (a one-hot draft's).
+  auto list_gone = [&](int64_t from, int64_t to) {
+    if (DRAFT) return 0;
+    __syncthreads();
+    const uint64_t in =
+        __ballot(((end.tried >> lane) & 1) != 0 && end.token >= from && end.token < to);
+    if (wave == 0 && ((in >> lane) & 1))
+      gone[__builtin_popcountll(in & ((uint64_t(1) << lane) - 1))] = end.token;
+    __syncthreads();
+    return static_cast<int>(__builtin_popcountll(in));
+  };
   const int64_t row = static_cast<int64_t>(b) * a.nodes + end.node;
   const T* p = static_cast<const T*>(a.target) + row * a.ldt;
   const T* q = DRAFT && end.tried ? static_cast<const T*>(a.draft) + row * a.ldd : nullptr;
-  const int gone = DRAFT ? 0 : ntried;
-  // What the row leaves of element v (whole: of all of them).
-  auto weigh = [&](T pv, T qv, int64_t v, bool whole) {
+  // What the row leaves of element v, `ngone` of the tokens listed (whole: of all of them).
+  auto weigh = [&](T pv, T qv, int64_t v, int ngone, bool whole) {
     double w = prob(pv);
     if (DRAFT && q && !whole) w = fmax(w - prob(qv), 0.0);
-    if (!DRAFT && !whole)
-      for (int i = 0; i < gone; ++i) w = tried[i] == v ? 0.0 : w;
+    if (!DRAFT)
+      for (int i = 0; i < ngone; ++i) w = gone[i] == v ? 0.0 : w;
     return w;
   };
-  const int64_t lo = chunk * a.chunk, hi = min(a.vocab, lo + a.chunk);
-  auto sum_of = [&](int64_t from, int64_t to, bool whole) {
-    double s = 0.0;
-    for (int64_t v = from + tid * E; v < to; v += kThreads * E) {
-      const int m = static_cast<int>(min(static_cast<int64_t>(E), to - v));
-      const RawVec<T> pv = m == E ? load_any(p + v) : load_tail(p, v, to, T(0));
-      RawVec<T> qv = pv;
-      if (DRAFT && q) qv = m == E ? load_any(q + v) : load_tail(q, v, to, T(0));
+  // N vectors of a thread, at a distance of `step` elements, from v on, as far as `to`.
+  auto weights = [&](auto& w, int64_t v, int64_t step, int64_t to, int ngone, bool whole) {
+    constexpr int N = sizeof(w) / sizeof(w[0]) / E;
+    RawVec<T> pv[N], qv[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t x = v + i * step;
+      pv[i] = x + E <= to ? load_any(p + x) : x < to ? load_tail(p, x, to, T(0)) : RawVec<T>(T(0));
+      qv[i] = pv[i];
+      if (DRAFT && q && x < to) qv[i] = x + E <= to ? load_any(q + x) : load_tail(q, x, to, T(0));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (e < m) s += weigh(pv[e], qv[e], v + e, whole);
-    }
+        w[i * E + e] = weigh(pv[i][e], qv[i][e], v + i * step + e, ngone, whole);
+  };
+  const int64_t lo = chunk * a.chunk, hi = min(a.vocab, lo + a.chunk);
+  auto block_sum = [&](double s) {
     s = wave_sum(s);
     __syncthreads();
     if (lane == 0) totals[wave] = s;
@@ -184,6 +187,18 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
 #pragma unroll
     for (int i = 0; i < kThreads / 64; ++i) t += totals[i];
     return t;
+  };
+  auto sum_of = [&](int64_t from, int64_t to, bool whole) {
+    constexpr int N = 4;
+    const int ngone = whole ? 0 : list_gone(from, to);
+    double s = 0.0;
+    for (int64_t v = from; v < to; v += kThreads * N * E) {
+      double w[N * E];
+      weights(w, v + tid * E, kThreads * E, to, ngone, whole);
+#pragma unroll
+      for (int e = 0; e < N * E; ++e) s += w[e];
+    }
+    return block_sum(s);
   };
   const double mine = sum_of(lo, hi, false);
   double* sums = a.sums + static_cast<int64_t>(b) * a.chunks;
@@ -254,31 +269,41 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
     from = found * a.chunk, to = min(a.vocab, from + a.chunk), before = found_before;
     __syncthreads();
   }
-  // The token: a thread's consecutive share of the elements, the shares' sums scanned.
-  const int64_t share = (to - from + kThreads - 1) / kThreads;
-  const int64_t s0 = min(to, from + tid * share), s1 = min(to, s0 + share);
-  double s = 0.0;
-  for (int64_t v = s0; v < s1; ++v) s += weigh(p[v], DRAFT && q ? q[v] : p[v], v, whole);
-  const double upto = scan(s);
-  if (lane == 63) totals[wave] = upto;
-  if (tid == 0) found = INT32_MAX, ntried = -1;
-  __syncthreads();
-  double run = before + upto - s;
-  for (int i = 0; i < wave; ++i) run += totals[i];
-  int mine_first = INT32_MAX, mine_last = -1;
-  // (`gone` holds what ntried did.)
-  for (int64_t v = s0; v < s1; ++v) {
-    const double x = weigh(p[v], DRAFT && q ? q[v] : p[v], v, whole);
-    run += x;
-    if (x > 0.0) {
-      mine_last = static_cast<int>(v);
-      if (run > point && mine_first == INT32_MAX) mine_first = static_cast<int>(v);
+  // The token: blocks of consecutive elements, a thread 16 of them.
+  constexpr int P = 16;
+  const int ngone = whole ? 0 : list_gone(from, to);
+  if (tid == 0) found = INT32_MAX, furthest = -1;
+  for (int64_t v0 = from; v0 < to; v0 += kThreads * P) {
+    const int64_t v = v0 + tid * P;
+    double w[P];
+    weights(w, v, E, to, ngone, whole);
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < P; ++e) s += w[e];
+    const double upto = scan(s);
+    __syncthreads();
+    if (lane == 63) totals[wave] = upto;
+    __syncthreads();
+    double run = before + (upto - s);
+    for (int i = 0; i < wave; ++i) run += totals[i];
+    int first = INT32_MAX, end_of = -1;
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      run += w[e];
+      if (w[e] > 0.0) {
+        end_of = static_cast<int>(v + e);
+        if (run > point && first == INT32_MAX) first = end_of;
+      }
     }
+    if (first != INT32_MAX) atomicMin(&found, first);
+    if (end_of >= 0) atomicMax(&furthest, end_of);
+    __syncthreads();
+    if (found != INT32_MAX) break;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) before += totals[i];
   }
-  if (mine_first != INT32_MAX) atomicMin(&found, mine_first);
-  if (mine_last >= 0) atomicMax(&ntried, mine_last);
-  __syncthreads();
-  if (tid == 0) a.next[b] = found != INT32_MAX ? found : ntried;
+  // (The sums round: the last that has any where none passes the point.)
+  if (tid == 0) a.next[b] = found != INT32_MAX ? found : furthest;
 }
 
 template <typename T>

@@ -116,9 +116,12 @@ __device__ __forceinline__ Node node_of(const TreeArgs& a, int b, int ctx, int l
   return r;
 }
 
+constexpr int tree_waves(int dt) { return dt <= 128 ? 2 : 1; }
+
 // WR of the four waves side by side over the rows, 32 each, the others over tokens.
 template <typename T, int DT, int WR>
-__global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kWaves * 64)
+    __attribute__((amdgpu_waves_per_eu(tree_waves(DT)))) void tree_attention_kernel(TreeArgs a) {
   using F = Frag<T>;
   using V8 = typename F::V;
   constexpr int WT = kWaves / WR;
@@ -135,6 +138,8 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
   constexpr int kLoopBytes = WT * NB * 2 * kTileBytes, kOutBytes = kWaves * 32 * PITCH * 4;
   __shared__ __align__(16) uint8_t lds[kLoopBytes > kOutBytes ? kLoopBytes : kOutBytes];
   __shared__ float sm[kWaves][32], sl[kWaves][32];
+  __shared__ uint64_t row_sees[32 * WR];
+  __shared__ int row_first[32 * WR], odd;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -214,15 +219,38 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
   auto vswz = [](int t) { return DT == 64 ? (t >> 1) & 1 : t & 3; };
   auto kswz = [](int t) { return DT == 64 ? (t >> 1) & 7 : t & 15; };
   auto buffer = [&](int i) { return lds + (tg * NB + i % NB) * (2 * kTileBytes); };
+  // A tile that some row does not see the whole of.
+  auto at_edge = [&](int base) {
+    return base + TK > ctx || base < lo || (a.reach > 0 && base < n - a.reach);
+  };
   // Into LDS: keys of a page that is none as NaN, values of tokens outside [lo, n) as zeros
-  // (0 * V must be 0 for what lies in the cache there).
-  auto store = [&](int base, const Ids& ids, uint8_t* to) {
+  // (0 * V must be 0 for what lies in the cache there), and so at an edge those that are no
+  // numbers, which join at the end (`odd`).
+  auto store = [&](int base, const Ids& ids, int i) {
+    uint8_t* to = buffer(i);
+    if (at_edge(base)) {
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const int t = base + j * RP + trow;
+        const bool in = t >= lo && t < n && ids.page[j] < a.pages;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const uint32_t x = in ? vr[j][y] : 0u;
+          const uint32_t bad = ((x & F::kExp) == F::kExp ? 0xffffu : 0u) |
+                               ((x & (F::kExp << 16)) == (F::kExp << 16) ? 0xffff0000u : 0u);
+          any |= bad != 0;
+          vr[j][y] = x & ~bad;
+        }
+      }
+      if (any && in_dim) odd = 1;
+    }
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const int r = j * RP + trow, t = base + r;
-      const bool good = ids.page[j] < a.pages, in = t >= lo && t < n;
+      const int r = j * RP + trow;
+      const bool good = ids.page[j] < a.pages;
       const v4u32_t k = !in_dim ? v4u32_t(0u) : good ? kr[j] : v4u32_t(F::kNan);
-      const v4u32_t v = in_dim && good && in ? vr[j] : v4u32_t(0u);
+      const v4u32_t v = in_dim && good ? vr[j] : v4u32_t(0u);
       *reinterpret_cast<v4u32_t*>(to + r * (DT * 2) + ((chunk ^ kswz(r)) << 4)) = k;
       *reinterpret_cast<v4u32_t*>(to + kTileBytes + r * (DT * 2) +
                                   ((((chunk >> 2) ^ vswz(r)) << 6) | ((chunk & 3) << 4))) = v;
@@ -236,6 +264,7 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
   const float scale2 = fabsf(a.scale) * kLog2e;
 
   auto compute = [&](int base, const uint8_t* from) {
+    const bool edge = at_edge(base);
     const uint8_t* keys = from;
     const uint8_t* values = from + kTileBytes;
     // S^T: register i of lane (h, c) is row c's score of token 8 (i / 4) + 4 h + i % 4.
@@ -250,18 +279,24 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
             keys + (32 * t + c) * (DT * 2) + (((2 * k + h) ^ kswz(c)) << 4));
         s[t] = F::mfma(__builtin_bit_cast(V8, x), qf[k], s[t]);
       }
-    const bool edge = base + TK > ctx || base < lo || (a.reach > 0 && base < n - a.reach);
     float by = scale2;
     if (edge) {
 #pragma unroll
-      for (int t = 0; t < TB; ++t)
+      for (int t = 0; t < TB; ++t) {
+        const int at = base + 32 * t, from_ctx = at - ctx;
+        auto ones = [](int k) {  // the first k bits
+          return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1;
+        };
+        const uint32_t drafted =
+            from_ctx >= 0 ? (from_ctx < 64 ? static_cast<uint32_t>(sees >> from_ctx) : 0u)
+                          : (from_ctx > -32 ? static_cast<uint32_t>(sees) << -from_ctx : 0u);
+        // (first is INT32_MAX for padding; at - first then stays in range.)
+        const uint32_t seen = (ones(-from_ctx) & ~ones(first - at)) | drafted;  // a bit a token
+        const uint32_t mine = seen >> (4 * h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int tok = base + 32 * t + 8 * (i / 4) + 4 * h + i % 4;
-          const bool seen = tok < ctx ? tok >= first
-                                      : tok < n && ((sees >> ((tok - ctx) & 63)) & 1) != 0;
-          s[t][i] = seen ? s[t][i] * scale2 : -__builtin_huge_valf();
-        }
+        for (int i = 0; i < 16; ++i)
+          s[t][i] = (mine >> (8 * (i / 4) + i % 4)) & 1 ? s[t][i] * scale2 : -__builtin_huge_valf();
+      }
       by = 1.0f;
     }
     float top = s[0][0];
@@ -280,24 +315,20 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
       for (int e = 0; e < DB; ++e) acc[e] *= alpha;
     }
     const float ref = finite(m) - F::kShift;
-    V8 p[2 * TB], rest[2 * TB];
-#pragma unroll
-    for (int t = 0; t < TB; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i], by, -ref));
-        s[t][i] = e;
-        l += e;
-        p[2 * t + i / 8][i % 8] = fromf<T>(e);
-        rest[2 * t + i / 8][i % 8] = fromf<T>(e - tof(p[2 * t + i / 8][i % 8]));
-      }
     // O^T: dims 32 e of the 16 tokens of step t, transposed on the way out of LDS: four
     // tokens of 16 dims for each 16 lanes.
     const int vlane = lane & 15, vdim = 16 * ((lane >> 4) & 1) + 4 * (vlane & 3);
     const int vtok = 4 * h + (vlane >> 2);
-    bool odd = false;
 #pragma unroll
-    for (int t = 0; t < 2 * TB; ++t)
+    for (int t = 0; t < 2 * TB; ++t) {
+      V8 p, rest;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[t / 2][8 * (t % 2) + i], by, -ref));
+        l += x;
+        p[i] = fromf<T>(x);
+        rest[i] = fromf<T>(x - tof(p[i]));
+      }
 #pragma unroll
       for (int e = 0; e < DB; ++e) {
         v4u32_t x;
@@ -310,54 +341,21 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
                          (__attribute__((address_space(3))) v4i16*)(at)));
           x[2 * y] = z[0], x[2 * y + 1] = z[1];
         }
-        if (edge) {
-          // What some rows must not meet: values that are no numbers join below.
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const uint32_t lo16 = (x[y] & F::kExp) == F::kExp ? 0xffffu : 0u;
-            const uint32_t hi16 = (x[y] & (F::kExp << 16)) == (F::kExp << 16) ? 0xffff0000u : 0u;
-            odd |= (lo16 | hi16) != 0;
-            x[y] &= ~(lo16 | hi16);
-          }
-        }
-        acc[e] = F::mfma(__builtin_bit_cast(V8, x), p[t], acc[e]);
-        acc[e] = F::mfma(__builtin_bit_cast(V8, x), rest[t], acc[e]);
-      }
-    if (edge && __any(odd)) {
-#pragma unroll 1
-      for (int r = 0; r < TK; ++r) {
-        float own = 0.0f;  // the weight of token r, or of r ^ 4 where that is this lane's
-#pragma unroll
-        for (int t = 0; t < TB; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            own = 32 * t + 8 * (i / 4) + i % 4 == (r & ~4) ? s[t][i] : own;
-        const float other = shfl_xor(own, 32);
-        const float weight = ((r >> 2) & 1) == h ? own : other;
-        const int tok = base + r;
-        const bool seen = tok < ctx ? tok >= first
-                                    : tok < n && ((sees >> ((tok - ctx) & 63)) & 1) != 0;
-#pragma unroll
-        for (int e = 0; e < DB; ++e)
-#pragma unroll
-          for (int y = 0; y < 16; ++y) {
-            const int d = 8 * (y / 4) + 4 * h + y % 4;
-            const T v = *reinterpret_cast<const T*>(values + r * (DT * 2) +
-                                                    ((e ^ vswz(r)) << 6) + d * 2);
-            const bool join = seen && (__builtin_bit_cast(uint16_t, v) & F::kExp) == F::kExp;
-            acc[e][y] = join ? fmaf(weight, tof(v), acc[e][y]) : acc[e][y];
-          }
+        acc[e] = F::mfma(__builtin_bit_cast(V8, x), p, acc[e]);
+        acc[e] = F::mfma(__builtin_bit_cast(V8, x), rest, acc[e]);
       }
     }
   };
 
+  if (threadIdx.x == 0) odd = 0;
+  __syncthreads();
   if (!broken && w.begin < w.end) {
     constexpr int STEP = WT * TK;
     const int count = (w.end - w.begin + STEP - 1) / STEP;
     int base = w.begin + tg * TK;
     Ids ids = locate(base), next = locate(base + STEP);
     load(base, ids);
-    store(base, ids, buffer(0));
+    store(base, ids, 0);
     if (NB > 1) __syncthreads();
     for (int i = 0; i < count; ++i, base += STEP) {
       if (NB == 1) asm volatile("" ::: "memory");
@@ -369,7 +367,7 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
       }
       if (base < w.end) compute(base, buffer(i));
       if (NB == 1) asm volatile("" ::: "memory");
-      if (more) store(base + STEP, ids, buffer(i + 1));
+      if (more) store(base + STEP, ids, i + 1);
       if (NB > 1) __syncthreads();
     }
   }
@@ -380,6 +378,7 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
   if (first == INT32_MAX) m = -__builtin_huge_valf(), l = 0.0f;  // padding
   if (broken || bad) l = __builtin_nanf("");
   if (h == 0) sm[wave][c] = m, sl[wave][c] = l;
+  if (h == 0 && tg == 0) row_sees[32 * wr + c] = sees, row_first[32 * wr + c] = first;
   auto out_at = [&](int v, int r, int d) {
     return reinterpret_cast<float*>(lds) + (v * 32 + r) * PITCH + d;
   };
@@ -400,6 +399,26 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
   float* part = a.parts + ((static_cast<int64_t>(w.slot) * a.heads +
                             (hk * a.tiles + tile) * static_cast<int64_t>(w.pieces)) + w.index) *
                               slot_floats;
+  // The values that are no numbers in the tiles at an edge, of the tokens that row r sees:
+  // their weights are above zero, whatever they are.
+  auto stray = [&](int r, int d) {
+    v4f32 x = v4f32(0.0f);
+    for (int base = w.begin; base < w.end; base += TK) {
+      if (!at_edge(base)) continue;
+      for (int t = max(base, lo); t < min(base + TK, w.end); ++t) {
+        const bool seen =
+            t < ctx ? t >= row_first[r] : ((row_sees[r] >> (t - ctx)) & 1) != 0;
+        const uint32_t id = static_cast<uint32_t>(table[page_of(t)]);
+        if (!seen || id >= a.pages) continue;
+        const T* v = vbase + id * a.vps +
+                     static_cast<int64_t>(t - static_cast<int>(page_of(t) * a.page_size)) * a.vts;
+        for (int e = 0; e < 4; ++e)
+          if ((__builtin_bit_cast(uint16_t, v[4 * d + e]) & F::kExp) == F::kExp)
+            x[e] += tof(v[4 * d + e]);
+      }
+    }
+    return x;
+  };
   for (int x = threadIdx.x; x < items; x += kWaves * 64) {
     const int r = x / d4, d = x - r * d4, wv = r >> 5, rr = r & 31;
     float M = sm[wv][rr];
@@ -415,6 +434,7 @@ __global__ __launch_bounds__(kWaves * 64) void tree_attention_kernel(TreeArgs a)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
     }
+    if (odd) o += stray(r, d);
     if (w.pieces == 1) {
       const int nd = (tile0 + r) / a.group, hd = hk * a.group + (tile0 + r - nd * a.group);
       const int64_t tok = static_cast<int64_t>(b) * a.nodes + nd;
