@@ -192,7 +192,8 @@ inline FastDiv fast_div(uint32_t d) {
   return FastDiv{static_cast<uint32_t>((p + d - 1) / d), 31 + l};
 }
 
-// How paged attention cuts a batch into pieces, one for a workgroup.  Lengths count in
+// How paged attention cuts a batch into pieces, one for a workgroup (kAttnGroups of them where
+// the sequences allow it; an attention that runs several workgroups a CU says how many).  Lengths count in
 // units of kAttnUnit tokens (of the window, from its first tile on; no sequence is 0).  A
 // sequence of up to kAttnWhole units is one piece.  Longer ones are cut into equal pieces
 // of at most `size` units: with share = all units / kAttnGroups, the least of
@@ -211,8 +212,8 @@ constexpr uint32_t attn_units(int32_t n, int32_t lo) {  // of tokens [lo, n)
   return w > 1 ? w : 1;
 }
 // (No sequence has more than 2^23 units: a larger share cuts nothing either.)
-constexpr uint32_t attn_share(uint64_t units, uint64_t heads) {
-  const uint64_t s = (units * heads + kAttnGroups - 1) / kAttnGroups;
+constexpr uint32_t attn_share(uint64_t units, uint64_t heads, uint32_t groups = kAttnGroups) {
+  const uint64_t s = (units * heads + groups - 1) / groups;
   return s < (uint64_t(1) << 25) ? static_cast<uint32_t>(s) : uint32_t(1) << 25;
 }
 constexpr uint32_t attn_size(uint32_t share, uint32_t k) {  // share, 5/4, 3/2, 2 of it
@@ -231,12 +232,13 @@ constexpr uint32_t attn_cut(uint32_t w, uint32_t size) {
 // 16384 tokens and the others of 200, 2 heads: 157 us whole, 23 cut).
 constexpr int64_t kAttnCutBatch = 256;
 // Workgroups that hold the pieces of any lengths, of at most `capacity` tokens.
-inline int64_t attn_grid(int64_t batch, int64_t heads, int64_t capacity) {
+inline int64_t attn_grid(int64_t batch, int64_t heads, int64_t capacity,
+                         uint32_t groups = kAttnGroups) {
   const int64_t bh = batch * heads;
   if (batch > kAttnCutBatch) return bh;
   const int64_t units = ceil_div(capacity + kAttnTile, kAttnUnit);
   const int64_t even = bh * (units / 2 + 1), fine = bh * (units / kAttnFineLeast + 1);
-  const int64_t g = kAttnGroups, f = kAttnFine * g + bh;
+  const int64_t g = groups, f = kAttnFine * g + bh;
   const int64_t a = even < g ? even : g, b = fine < f ? fine : f;
   return a > b ? a : b;
 }

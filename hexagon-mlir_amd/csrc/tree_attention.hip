@@ -118,6 +118,9 @@ __device__ __forceinline__ Node node_of(const TreeArgs& a, int b, int ctx, int l
 
 constexpr int tree_waves(int dt) { return dt <= 128 ? 2 : 1; }
 
+// Pieces of a batch: as many as run at once.
+constexpr uint32_t tree_groups(int dt) { return (dt <= 128 ? 2 : 1) * kAttnGroups; }
+
 // WR of the four waves side by side over the rows, 32 each, the others over tokens.
 template <typename T, int DT, int WR>
 __global__ __launch_bounds__(kWaves * 64)
@@ -151,7 +154,7 @@ __global__ __launch_bounds__(kWaves * 64)
   const uint32_t pair = blockIdx.x / (8u * a.tiles) * 8u + blockIdx.x % 8u;
   const int tile = static_cast<int>(blockIdx.x / 8u % static_cast<uint32_t>(a.tiles));
   const int hk = static_cast<int>(pair % static_cast<uint32_t>(a.hkv));
-  const Piece w = find_piece<false>(a, pair / static_cast<uint32_t>(a.hkv), lane);
+  const Piece w = find_piece<false, tree_groups(DT)>(a, pair / static_cast<uint32_t>(a.hkv), lane);
   if (w.b < 0) return;
   const int D = a.dim;
   const int b = w.b, n = w.n, lo = w.lo;
@@ -455,14 +458,14 @@ __global__ __launch_bounds__(kWaves * 64)
 
 // Joins the pieces of the sequences that were cut, in their order: a thread a row's four
 // dims.
-template <typename T>
+template <typename T, uint32_t GROUPS>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int tile_rows, int slices) {
   const int lane = threadIdx.x & 63;
   const uint32_t x = blockIdx.x / static_cast<uint32_t>(slices);
   const int slice = static_cast<int>(blockIdx.x % static_cast<uint32_t>(slices));
   const int b = static_cast<int>(x / static_cast<uint32_t>(a.heads));
   const int ht = static_cast<int>(x % static_cast<uint32_t>(a.heads));
-  const Piece w = find_piece<true>(a, static_cast<uint32_t>(b), lane);
+  const Piece w = find_piece<true, GROUPS>(a, static_cast<uint32_t>(b), lane);
   if (w.b < 0 || w.pieces < 2) return;
   const int D = a.dim, d4 = D / 4, per = 256 / d4;
   const int hk = ht / a.tiles, tile = ht % a.tiles;
@@ -517,7 +520,7 @@ int tile_rows(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 template <typename T, int DT>
 hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
   const int rows = tile_rows(int64_t(a.nodes) * a.group);
-  const int64_t pairs = ceil_div(attn_grid(a.batch, a.heads, a.capacity), a.tiles);
+  const int64_t pairs = ceil_div(attn_grid(a.batch, a.heads, a.capacity, tree_groups(DT)), a.tiles);
   const int64_t groups = ceil_div(pairs, 8) * 8 * a.tiles;
   const int per = 256 / (a.dim / 4), slices = static_cast<int>(ceil_div(rows, per));
   const int64_t joins = int64_t(a.batch) * a.heads * slices;
@@ -530,7 +533,8 @@ hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
   if ((st = check_launch("tree attention")) != HXM_OK) return st;
   // Sequences of up to kAttnWhole units are one piece each.
   if (a.batch > kAttnCutBatch || a.capacity <= kAttnWhole * kAttnUnit - kAttnTile) return ok();
-  tree_join_kernel<T><<<static_cast<unsigned>(joins), 256, 0, stream>>>(a, rows, slices);
+  tree_join_kernel<T, tree_groups(DT)>
+      <<<static_cast<unsigned>(joins), 256, 0, stream>>>(a, rows, slices);
   return check_launch("tree attention join");
 }
 
@@ -612,8 +616,9 @@ extern "C" hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* ou
   // Partial results of the sequences cut in pieces.
   hipStream_t s = as_stream(stream);
   if (batch <= kAttnCutBatch && a.capacity > kAttnWhole * kAttnUnit - kAttnTile) {
-    const int64_t slots =
-        std::min(attn_grid(batch, a.heads, a.capacity), int64_t(2 * kAttnFine * kAttnGroups));
+    const uint32_t pieces = tree_groups(a.dim);
+    const int64_t slots = std::min(attn_grid(batch, a.heads, a.capacity, pieces),
+                                   int64_t(2 * kAttnFine * pieces));
     void* ws = nullptr;
     st = stream_workspace(s, static_cast<size_t>(slots * rows * (a.dim + 2) * 4), &ws, kWsLayer);
     if (st != HXM_OK) return st;
