@@ -3,6 +3,7 @@
 // The rows that share a key head, nodes x group of them, are the 32-wide side of the
 // MFMAs, so that one read of the keys and values serves up to 128 rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_cut.h"
 #include "device_util.h"
@@ -62,6 +63,7 @@ struct Frag<__bf16> {
 
 typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float v8f32 __attribute__((ext_vector_type(8)));
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float shfl_xor(float v, int m) { return __shfl_xor(v, m, 64); }
@@ -121,8 +123,12 @@ constexpr int tree_waves(int dt) { return dt <= 128 ? 2 : 1; }
 // Pieces of a batch: as many as run at once.
 constexpr uint32_t tree_groups(int dt) { return (dt <= 128 ? 2 : 1) * kAttnGroups; }
 
+// Kinds of instructions to the scheduler.
+constexpr int kValu = 0x2, kMfma = 0x8, kDsRead = 0x100;
+constexpr int kStepValu = 56;  // of the weights of 16 tokens
+
 // WR of the four waves side by side over the rows, 32 each, the others over tokens.
-template <typename T, int DT, int WR>
+template <typename T, int DT, int WR, bool P>
 __global__ __launch_bounds__(kWaves * 64)
     __attribute__((amdgpu_waves_per_eu(tree_waves(DT)))) void tree_attention_kernel(TreeArgs a) {
   using F = Frag<T>;
@@ -198,25 +204,38 @@ __global__ __launch_bounds__(kWaves * 64)
   const int trow = gt / CK, chunk = gt % CK;
   const bool in_dim = chunk * 8 < D;
   const int dim0 = in_dim ? chunk * 8 : 0;
+  // Where the rows lie.  P: a wave's rows of a load are of one page, whose number and
+  // address the scalar unit works out; otherwise every thread its own.
+  constexpr int RW = 64 / CK;  // rows of a wave's load
   struct Ids {
     uint32_t page[NP];
+    int off[NP];  // of the first row in its page
   };
-  auto token = [&](int base, int j) { return min(max(base + j * RP + trow, lo), n - 1); };
+  typedef const int32_t __attribute__((address_space(4))) * ConstInts;
+  const ConstInts ctable = (ConstInts)(reinterpret_cast<uintptr_t>(table));
   auto locate = [&](int base) {
     Ids r;
 #pragma unroll
-    for (int j = 0; j < NP; ++j) r.page[j] = static_cast<uint32_t>(table[page_of(token(base, j))]);
+    for (int j = 0; j < NP; ++j) {
+      const int t = P ? min(max(base + j * RP + wr * RW, lo & -RW), (n - 1) & -RW)
+                      : min(max(base + j * RP + trow, lo), n - 1);
+      const uint32_t k = page_of(t);
+      r.page[j] = static_cast<uint32_t>(P ? ctable[k] : table[k]);
+      r.off[j] = t - static_cast<int>(k * a.page_size);
+    }
     return r;
   };
+  const uint32_t klane = (P ? lane / CK * static_cast<uint32_t>(a.kts) : 0u) + dim0;
+  const uint32_t vlane = (P ? lane / CK * static_cast<uint32_t>(a.vts) : 0u) + dim0;
   v4u32_t kr[NP], vr[NP];
-  auto load = [&](int base, const Ids& ids) {
+  auto load = [&](const Ids& ids) {
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const int t = token(base, j);
-      const uint32_t id = ids.page[j] < a.pages ? ids.page[j] : 0u;
-      const int64_t off = t - static_cast<int>(page_of(t) * a.page_size);
-      kr[j] = *reinterpret_cast<const any4*>(kbase + id * a.kps + off * a.kts + dim0);
-      vr[j] = *reinterpret_cast<const any4*>(vbase + id * a.vps + off * a.vts + dim0);
+      const int64_t id = ids.page[j] < a.pages ? ids.page[j] : 0u, off = ids.off[j];
+      const T* k = kbase + id * a.kps + off * a.kts;
+      const T* v = vbase + id * a.vps + off * a.vts;
+      kr[j] = *reinterpret_cast<const any4*>(k + klane);
+      vr[j] = *reinterpret_cast<const any4*>(v + vlane);
     }
   };
   auto vswz = [](int t) { return DT == 64 ? (t >> 1) & 1 : t & 3; };
@@ -231,12 +250,16 @@ __global__ __launch_bounds__(kWaves * 64)
   // numbers, which join at the end (`odd`).
   auto store = [&](int base, const Ids& ids, int i) {
     uint8_t* to = buffer(i);
-    if (at_edge(base)) {
+    bool bad_page = false;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) bad_page |= ids.page[j] >= a.pages;
+    if (at_edge(base) || (P ? bad_page : __any(bad_page))) {
       bool any = false;
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         const int t = base + j * RP + trow;
-        const bool in = t >= lo && t < n && ids.page[j] < a.pages;
+        const bool good = ids.page[j] < a.pages, in = t >= lo && t < n && good;
+        if (!good) kr[j] = v4u32_t(F::kNan);
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           const uint32_t x = in ? vr[j][y] : 0u;
@@ -248,15 +271,19 @@ __global__ __launch_bounds__(kWaves * 64)
       }
       if (any && in_dim) odd = 1;
     }
+    if (D < DT) {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        kr[j] = in_dim ? kr[j] : v4u32_t(0u);
+        vr[j] = in_dim ? vr[j] : v4u32_t(0u);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       const int r = j * RP + trow;
-      const bool good = ids.page[j] < a.pages;
-      const v4u32_t k = !in_dim ? v4u32_t(0u) : good ? kr[j] : v4u32_t(F::kNan);
-      const v4u32_t v = in_dim && good ? vr[j] : v4u32_t(0u);
-      *reinterpret_cast<v4u32_t*>(to + r * (DT * 2) + ((chunk ^ kswz(r)) << 4)) = k;
+      *reinterpret_cast<v4u32_t*>(to + r * (DT * 2) + ((chunk ^ kswz(r)) << 4)) = kr[j];
       *reinterpret_cast<v4u32_t*>(to + kTileBytes + r * (DT * 2) +
-                                  ((((chunk >> 2) ^ vswz(r)) << 6) | ((chunk & 3) << 4))) = v;
+                                  ((((chunk >> 2) ^ vswz(r)) << 6) | ((chunk & 3) << 4))) = vr[j];
     }
   };
 
@@ -282,6 +309,14 @@ __global__ __launch_bounds__(kWaves * 64)
             keys + (32 * t + c) * (DT * 2) + (((2 * k + h) ^ kswz(c)) << 4));
         s[t] = F::mfma(__builtin_bit_cast(V8, x), qf[k], s[t]);
       }
+    // Four keys ahead of the products.
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+    for (int i = 0; i < KS * TB - 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
     float by = scale2;
     if (edge) {
 #pragma unroll
@@ -320,18 +355,22 @@ __global__ __launch_bounds__(kWaves * 64)
     const float ref = finite(m) - F::kShift;
     // O^T: dims 32 e of the 16 tokens of step t, transposed on the way out of LDS: four
     // tokens of 16 dims for each 16 lanes.
-    const int vlane = lane & 15, vdim = 16 * ((lane >> 4) & 1) + 4 * (vlane & 3);
-    const int vtok = 4 * h + (vlane >> 2);
-#pragma unroll
-    for (int t = 0; t < 2 * TB; ++t) {
-      V8 p, rest;
+    const int v16 = lane & 15, vdim = 16 * ((lane >> 4) & 1) + 4 * (v16 & 3);
+    const int vtok = 4 * h + (v16 >> 2);
+    V8 p[2], rest[2], vt[2][DB];
+    auto weights = [&](int t) {  // of step t's tokens
+      v8f32 x;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[t / 2][8 * (t % 2) + i], by, -ref));
-        l += x;
-        p[i] = fromf<T>(x);
-        rest[i] = fromf<T>(x - tof(p[i]));
+        x[i] = __builtin_amdgcn_exp2f(fmaf(s[t / 2][8 * (t % 2) + i], by, -ref));
+        l += x[i];
       }
+      p[t % 2] = __builtin_convertvector(x, V8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] -= tof(p[t % 2][i]);
+      rest[t % 2] = __builtin_convertvector(x, V8);
+    };
+    auto read_values = [&](int t) {
 #pragma unroll
       for (int e = 0; e < DB; ++e) {
         v4u32_t x;
@@ -344,10 +383,30 @@ __global__ __launch_bounds__(kWaves * 64)
                          (__attribute__((address_space(3))) v4i16*)(at)));
           x[2 * y] = z[0], x[2 * y + 1] = z[1];
         }
-        acc[e] = F::mfma(__builtin_bit_cast(V8, x), p, acc[e]);
-        acc[e] = F::mfma(__builtin_bit_cast(V8, x), rest, acc[e]);
+        vt[t % 2][e] = __builtin_bit_cast(V8, x);
       }
+    };
+    // The next step's weights are made and its values read under this one's products (both
+    // halves of one dim apart: the second waits for the first).
+    read_values(0);
+    weights(0);
+#pragma unroll
+    for (int t = 0; t < 2 * TB; ++t) {
+      if (t + 1 < 2 * TB) read_values(t + 1), weights(t + 1);
+#pragma unroll
+      for (int e = 0; e < DB; ++e) acc[e] = F::mfma(vt[t % 2][e], p[t % 2], acc[e]);
+#pragma unroll
+      for (int e = 0; e < DB; ++e) acc[e] = F::mfma(vt[t % 2][e], rest[t % 2], acc[e]);
     }
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * DB, 1);
+    __builtin_amdgcn_sched_group_barrier(kValu, kStepValu, 1);
+#pragma unroll
+    for (int i = 0; i < (2 * TB - 1) * 2 * DB; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(kValu, (kStepValu + 2 * DB - 1) / (2 * DB), 1);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 1);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMfma, 2 * DB, 1);
   };
 
   if (threadIdx.x == 0) odd = 0;
@@ -357,7 +416,7 @@ __global__ __launch_bounds__(kWaves * 64)
     const int count = (w.end - w.begin + STEP - 1) / STEP;
     int base = w.begin + tg * TK;
     Ids ids = locate(base), next = locate(base + STEP);
-    load(base, ids);
+    load(ids);
     store(base, ids, 0);
     if (NB > 1) __syncthreads();
     for (int i = 0; i < count; ++i, base += STEP) {
@@ -365,7 +424,7 @@ __global__ __launch_bounds__(kWaves * 64)
       const bool more = i + 1 < count;
       if (more) {
         ids = next;
-        load(base + STEP, ids);
+        load(ids);
         next = locate(base + 2 * STEP);
       }
       if (base < w.end) compute(base, buffer(i));
@@ -527,9 +586,16 @@ hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
   hxm_status st = check_grid("tree attention", std::max(groups, joins), 256);
   if (st != HXM_OK) return st;
   const unsigned n = static_cast<unsigned>(groups);
-  if (rows == 32) tree_attention_kernel<T, DT, 1><<<n, 256, 0, stream>>>(a);
-  else if (rows == 64) tree_attention_kernel<T, DT, 2><<<n, 256, 0, stream>>>(a);
-  else tree_attention_kernel<T, DT, 4><<<n, 256, 0, stream>>>(a);
+  // A wave loads 512 / DT rows at a time.
+  const bool paged = a.page_size % (512 / DT) == 0 && std::max(a.kts, a.vts) <= (int64_t(1) << 24);
+  auto launch = [&](auto wr) {
+    constexpr int WR = decltype(wr)::value;
+    if (paged) tree_attention_kernel<T, DT, WR, true><<<n, 256, 0, stream>>>(a);
+    else tree_attention_kernel<T, DT, WR, false><<<n, 256, 0, stream>>>(a);
+  };
+  if (rows == 32) launch(std::integral_constant<int, 1>{});
+  else if (rows == 64) launch(std::integral_constant<int, 2>{});
+  else launch(std::integral_constant<int, 4>{});
   if ((st = check_launch("tree attention")) != HXM_OK) return st;
   // Sequences of up to kAttnWhole units are one piece each.
   if (a.batch > kAttnCutBatch || a.capacity <= kAttnWhole * kAttnUnit - kAttnTile) return ok();
