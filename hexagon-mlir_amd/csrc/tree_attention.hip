@@ -40,6 +40,8 @@ struct TreeArgs {
   float scale;
 };
 
+typedef float v8f32 __attribute__((ext_vector_type(8)));
+
 template <typename T>
 struct Frag;
 template <>
@@ -50,6 +52,17 @@ struct Frag<_Float16> {
   static __device__ __forceinline__ v16f32 mfma(V a, V b, v16f32 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  // x towards zero; x keeps what that leaves.
+  static __device__ __forceinline__ V split(v8f32& x) {
+    V r;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const auto h = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
+      r[i] = static_cast<_Float16>(h[0]), r[i + 1] = static_cast<_Float16>(h[1]);
+      x[i] -= static_cast<float>(h[0]), x[i + 1] -= static_cast<float>(h[1]);
+    }
+    return r;
+  }
 };
 template <>
 struct Frag<__bf16> {
@@ -59,11 +72,22 @@ struct Frag<__bf16> {
   static __device__ __forceinline__ v16f32 mfma(V a, V b, v16f32 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ V split(v8f32& x) {
+    v4u32_t r;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const uint32_t a = __builtin_bit_cast(uint32_t, static_cast<float>(x[i])),
+                     b = __builtin_bit_cast(uint32_t, static_cast<float>(x[i + 1]));
+      r[i / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      x[i] -= __builtin_bit_cast(float, a & 0xffff0000u);
+      x[i + 1] -= __builtin_bit_cast(float, b & 0xffff0000u);
+    }
+    return __builtin_bit_cast(V, r);
+  }
 };
 
 typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef float v8f32 __attribute__((ext_vector_type(8)));
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float shfl_xor(float v, int m) { return __shfl_xor(v, m, 64); }
@@ -219,7 +243,10 @@ __global__ __launch_bounds__(kWaves * 64)
     for (int j = 0; j < NP; ++j) {
       const int t = P ? min(max(base + j * RP + wr * RW, lo & -RW), (n - 1) & -RW)
                       : min(max(base + j * RP + trow, lo), n - 1);
-      const uint32_t k = page_of(t);
+      // (P: page_size is 2 or more, and the shift 32 or more.)
+      const uint32_t k = P ? __umulhi(static_cast<uint32_t>(t), a.page_div.mul) >>
+                                 (a.page_div.shift - 32)
+                           : page_of(t);
       r.page[j] = static_cast<uint32_t>(P ? ctable[k] : table[k]);
       r.off[j] = t - static_cast<int>(k * a.page_size);
     }
@@ -231,9 +258,18 @@ __global__ __launch_bounds__(kWaves * 64)
   auto load = [&](const Ids& ids) {
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const int64_t id = ids.page[j] < a.pages ? ids.page[j] : 0u, off = ids.off[j];
-      const T* k = kbase + id * a.kps + off * a.kts;
-      const T* v = vbase + id * a.vps + off * a.vts;
+      const uint32_t id = ids.page[j] < a.pages ? ids.page[j] : 0u;
+      const T *k = kbase, *v = vbase;
+      if constexpr (P) {
+        const uint32_t off = static_cast<uint32_t>(ids.off[j]);
+        k += static_cast<uint64_t>(id) * static_cast<uint32_t>(a.kps) +
+             off * static_cast<uint32_t>(a.kts);
+        v += static_cast<uint64_t>(id) * static_cast<uint32_t>(a.vps) +
+             off * static_cast<uint32_t>(a.vts);
+      } else {
+        k += id * a.kps + ids.off[j] * a.kts;
+        v += id * a.vps + ids.off[j] * a.vts;
+      }
       kr[j] = *reinterpret_cast<const any4*>(k + klane);
       vr[j] = *reinterpret_cast<const any4*>(v + vlane);
     }
@@ -365,9 +401,7 @@ __global__ __launch_bounds__(kWaves * 64)
         x[i] = __builtin_amdgcn_exp2f(fmaf(s[t / 2][8 * (t % 2) + i], by, -ref));
         l += x[i];
       }
-      p[t % 2] = __builtin_convertvector(x, V8);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] -= tof(p[t % 2][i]);
+      p[t % 2] = F::split(x);
       rest[t % 2] = __builtin_convertvector(x, V8);
     };
     auto read_values = [&](int t) {
@@ -586,8 +620,10 @@ hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
   hxm_status st = check_grid("tree attention", std::max(groups, joins), 256);
   if (st != HXM_OK) return st;
   const unsigned n = static_cast<unsigned>(groups);
-  // A wave loads 512 / DT rows at a time.
-  const bool paged = a.page_size % (512 / DT) == 0 && std::max(a.kts, a.vts) <= (int64_t(1) << 24);
+  // A wave loads 512 / DT rows at a time; a page and its stride within 32 bits.
+  const bool paged = a.page_size % (512 / DT) == 0 &&
+                     std::max(a.kts, a.vts) <= (int64_t(1) << 30) / a.page_size &&
+                     std::max(a.kps, a.vps) <= UINT32_MAX;
   auto launch = [&](auto wr) {
     constexpr int WR = decltype(wr)::value;
     if (paged) tree_attention_kernel<T, DT, WR, true><<<n, 256, 0, stream>>>(a);
