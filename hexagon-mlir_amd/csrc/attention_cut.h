@@ -51,7 +51,7 @@ struct Piece {
 // trying the others, which took 13 us instead of 15.4 for 256 x 600 tokens, one head, 12.3 for
 // 13.7 (128 x 600, two) and 149 for 152 (256 x 2048, eight), and 15 for 11.6 where few tokens
 // are many sequences' (65 x 1024, one head) and 30 for 25 (200 x 2048, one).
-template <bool BY_SEQUENCE, uint32_t GROUPS = kAttnGroups, typename Args>
+template <bool BY_SEQUENCE, uint32_t GROUPS = kAttnGroups, bool STEPS = false, typename Args>
 __device__ __forceinline__ Piece find_piece(const Args& a, uint32_t u, int lane) {
   auto tokens = [&](int32_t len, int* lo) {
     const int n = len > a.capacity ? 0 : max(len, 0);
@@ -88,8 +88,8 @@ __device__ __forceinline__ Piece find_piece(const Args& a, uint32_t u, int lane)
   uint32_t size = 0;
   bool fits = false;
   if (a.batch <= 64)
-    for (uint32_t k = 0; k < 4 && !fits; ++k) {
-      size = attn_size(share, k);
+    for (uint32_t k = 0; k < (STEPS ? kAttnSteps : 4) && !fits; ++k) {
+      size = STEPS ? attn_step_size(share, k) : attn_size(share, k);
       fits = wave_sum(attn_cut(w[0], size)) * a.heads <= GROUPS;
     }
   if (!fits) size = attn_fine_size(share);

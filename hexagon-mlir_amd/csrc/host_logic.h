@@ -220,6 +220,14 @@ constexpr uint32_t attn_size(uint32_t share, uint32_t k) {  // share, 5/4, 3/2, 
   const uint32_t s = share + (k < 3 ? k : 4) * share / 4;
   return s > 2 ? s : 2;
 }
+// The same in smaller steps, for pieces of many rows (a piece that is a quarter longer than
+// the others' share is a quarter more time where the products bound it).
+constexpr int kAttnSteps = 7;
+constexpr uint32_t attn_step_size(uint32_t share, uint32_t k) {
+  const uint32_t part = k == 0 ? 0 : 1u << (k - 1);  // of 32: 0, 1, 2, 4, 8, 16, 32
+  const uint32_t s = share + (share * part + 31) / 32;
+  return s > 2 ? s : 2;
+}
 constexpr uint32_t attn_fine_size(uint32_t share) {
   const uint32_t s = (share + kAttnFine - 1) / kAttnFine;
   return s > kAttnFineLeast ? s : kAttnFineLeast;

@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kWaves * 64)
   const uint32_t pair = blockIdx.x / (8u * a.tiles) * 8u + blockIdx.x % 8u;
   const int tile = static_cast<int>(blockIdx.x / 8u % static_cast<uint32_t>(a.tiles));
   const int hk = static_cast<int>(pair % static_cast<uint32_t>(a.hkv));
-  const Piece w = find_piece<false, tree_groups(DT)>(a, pair / static_cast<uint32_t>(a.hkv), lane);
+  const Piece w = find_piece<false, tree_groups(DT), true>(a, pair / static_cast<uint32_t>(a.hkv), lane);
   if (w.b < 0) return;
   const int D = a.dim;
   const int b = w.b, n = w.n, lo = w.lo;
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int tile_row
   const int slice = static_cast<int>(blockIdx.x % static_cast<uint32_t>(slices));
   const int b = static_cast<int>(x / static_cast<uint32_t>(a.heads));
   const int ht = static_cast<int>(x % static_cast<uint32_t>(a.heads));
-  const Piece w = find_piece<true, GROUPS>(a, static_cast<uint32_t>(b), lane);
+  const Piece w = find_piece<true, GROUPS, true>(a, static_cast<uint32_t>(b), lane);
   if (w.b < 0 || w.pieces < 2) return;
   const int D = a.dim, d4 = D / 4, per = 256 / d4;
   const int hk = ht / a.tiles, tile = ht % a.tiles;
