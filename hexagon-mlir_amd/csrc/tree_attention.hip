@@ -111,11 +111,10 @@ __device__ __forceinline__ Node node_of(const TreeArgs& a, int b, int ctx, int l
   const bool pad = p < -1;
   const uint64_t pads = __ballot(pad), wrong = __ballot(p >= lane);
   if (p >= lane) p = -1;
-  // Ancestors by doubling: after k steps those up to 2^k - 1 above.
+  // Ancestors by doubling: those up to 2 k - 1 above.
   uint64_t up = uint64_t(1) << lane;
   int to = p;
-#pragma unroll
-  for (int k = 0; k < 6; ++k) {
+  for (int k = 1; k < a.nodes; k *= 2) {
     const int at = max(to, 0);
     const uint64_t more = shfl64(up, at);
     const int next = __shfl(to, at, 64);
@@ -146,10 +145,6 @@ constexpr int tree_waves(int dt) { return dt <= 128 ? 2 : 1; }
 
 // Pieces of a batch: as many as run at once.
 constexpr uint32_t tree_groups(int dt) { return (dt <= 128 ? 2 : 1) * kAttnGroups; }
-
-// Kinds of instructions to the scheduler.
-constexpr int kValu = 0x2, kMfma = 0x8, kDsRead = 0x100;
-constexpr int kStepValu = 56;  // of the weights of 16 tokens
 
 // WR of the four waves side by side over the rows, 32 each, the others over tokens.
 template <typename T, int DT, int WR, bool P>
@@ -197,25 +192,6 @@ __global__ __launch_bounds__(kWaves * 64)
   const int node = live ? row / a.group : 0;
   const int head = hk * a.group + (live ? row - node * a.group : 0);
 
-  const Node mine = node_of(a, b, ctx, lane);
-  const uint64_t sees = shfl64(mine.sees, node);
-  const int first = __shfl(mine.first, node, 64);
-  const bool bad = __shfl(static_cast<int>(mine.bad), node, 64) != 0;
-
-  // Q^T: dims 16k + 8h .. of row c, zeros past the last row and past D.  A negative scale
-  // is Q's sign.
-  V8 qf[KS];
-  {
-    const T* q = static_cast<const T*>(a.q) +
-                 (static_cast<int64_t>(b) * a.nodes + node) * a.q_ts + head * a.q_hs;
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int d = k * 16 + h * 8;
-      const v4u32_t x = *reinterpret_cast<const any4*>(q + (d < D ? d : 0));
-      qf[k] = __builtin_bit_cast(V8, live && d < D ? x ^ flip : v4u32_t(0u));
-    }
-  }
   const T* kbase = static_cast<const T*>(a.kc) + hk * a.khs;
   const T* vbase = static_cast<const T*>(a.vc) + hk * a.vhs;
   const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
@@ -274,6 +250,37 @@ __global__ __launch_bounds__(kWaves * 64)
       vr[j] = *reinterpret_cast<const any4*>(v + vlane);
     }
   };
+  // The first tile on its way before anything else.
+  constexpr int STEP = WT * TK;
+  const bool any_tokens = !broken && w.begin < w.end;
+  int base = w.begin + tg * TK;
+  Ids ids{}, next{};
+  if (any_tokens) {
+    ids = locate(base);
+    load(ids);
+    next = locate(base + STEP);
+  }
+
+  // Q^T: dims 16k + 8h .. of row c, zeros past the last row and past D.  A negative scale
+  // is Q's sign.
+  V8 qf[KS];
+  {
+    const T* q = static_cast<const T*>(a.q) +
+                 (static_cast<int64_t>(b) * a.nodes + node) * a.q_ts + head * a.q_hs;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int d = k * 16 + h * 8;
+      const v4u32_t x = *reinterpret_cast<const any4*>(q + (d < D ? d : 0));
+      qf[k] = __builtin_bit_cast(V8, live && d < D ? x ^ flip : v4u32_t(0u));
+    }
+  }
+
+  const Node mine = node_of(a, b, ctx, lane);
+  const uint64_t sees = shfl64(mine.sees, node);
+  const int first = __shfl(mine.first, node, 64);
+  const bool bad = __shfl(static_cast<int>(mine.bad), node, 64) != 0;
+
   auto vswz = [](int t) { return DT == 64 ? (t >> 1) & 1 : t & 3; };
   auto kswz = [](int t) { return DT == 64 ? (t >> 1) & 7 : t & 15; };
   auto buffer = [&](int i) { return lds + (tg * NB + i % NB) * (2 * kTileBytes); };
@@ -345,14 +352,6 @@ __global__ __launch_bounds__(kWaves * 64)
             keys + (32 * t + c) * (DT * 2) + (((2 * k + h) ^ kswz(c)) << 4));
         s[t] = F::mfma(__builtin_bit_cast(V8, x), qf[k], s[t]);
       }
-    // Four keys ahead of the products.
-    __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
-#pragma unroll
-    for (int i = 0; i < KS * TB - 4; ++i) {
-      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
     float by = scale2;
     if (edge) {
 #pragma unroll
@@ -432,25 +431,12 @@ __global__ __launch_bounds__(kWaves * 64)
 #pragma unroll
       for (int e = 0; e < DB; ++e) acc[e] = F::mfma(vt[t % 2][e], rest[t % 2], acc[e]);
     }
-    __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * DB, 1);
-    __builtin_amdgcn_sched_group_barrier(kValu, kStepValu, 1);
-#pragma unroll
-    for (int i = 0; i < (2 * TB - 1) * 2 * DB; ++i) {
-      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
-      __builtin_amdgcn_sched_group_barrier(kValu, (kStepValu + 2 * DB - 1) / (2 * DB), 1);
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 1);
-    }
-    __builtin_amdgcn_sched_group_barrier(kMfma, 2 * DB, 1);
   };
 
   if (threadIdx.x == 0) odd = 0;
   __syncthreads();
-  if (!broken && w.begin < w.end) {
-    constexpr int STEP = WT * TK;
+  if (any_tokens) {
     const int count = (w.end - w.begin + STEP - 1) / STEP;
-    int base = w.begin + tg * TK;
-    Ids ids = locate(base), next = locate(base + STEP);
-    load(ids);
     store(base, ids, 0);
     if (NB > 1) __syncthreads();
     for (int i = 0; i < count; ++i, base += STEP) {
