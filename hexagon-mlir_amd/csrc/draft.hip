@@ -23,8 +23,8 @@ namespace {
 
 constexpr int kMaxNodes = 64;
 constexpr int kThreads = 256;
-// Elements of a chunk at the least, and workgroups of a launch that the rows are cut for.
-constexpr int64_t kLeastChunk = 4096, kGroups = 1024;
+// A chunk is whole blocks of elements, 16 a thread; as many chunks as give this many workgroups.
+constexpr int64_t kBlock = 16 * kThreads, kGroups = 1024;
 
 struct VerifyArgs {
   const int32_t* tokens;
@@ -160,16 +160,32 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
       for (int i = 0; i < ngone; ++i) w = gone[i] == v ? 0.0 : w;
     return w;
   };
-  // N vectors of a thread, at a distance of `step` elements, from v on, as far as `to`.
-  auto weights = [&](auto& w, int64_t v, int64_t step, int64_t to, int ngone, bool whole) {
+  // Vectors of a thread, at a distance of `step` elements, from v on, as far as `to` (inside:
+  // all of them of every thread, which are loaded at once).
+  auto weights = [&](auto& w, int64_t v, int64_t step, int64_t to, bool inside, int ngone,
+                     bool whole) {
     constexpr int N = sizeof(w) / sizeof(w[0]) / E;
     RawVec<T> pv[N], qv[N];
+    if (inside) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t x = v + i * step;
-      pv[i] = x + E <= to ? load_any(p + x) : x < to ? load_tail(p, x, to, T(0)) : RawVec<T>(T(0));
-      qv[i] = pv[i];
-      if (DRAFT && q && x < to) qv[i] = x + E <= to ? load_any(q + x) : load_tail(q, x, to, T(0));
+      for (int i = 0; i < N; ++i) pv[i] = load_any(p + v + i * step);
+      if (DRAFT && q) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) qv[i] = load_any(q + v + i * step);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t x = v + i * step;
+        pv[i] = qv[i] = RawVec<T>(T(0));
+        if (x + E <= to) {
+          pv[i] = load_any(p + x);
+          if (DRAFT && q) qv[i] = load_any(q + x);
+        } else if (x < to) {
+          pv[i] = load_tail(p, x, to, T(0));
+          if (DRAFT && q) qv[i] = load_tail(q, x, to, T(0));
+        }
+      }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -189,12 +205,12 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
     return t;
   };
   auto sum_of = [&](int64_t from, int64_t to, bool whole) {
-    constexpr int N = 4;
+    constexpr int N = 16 / E;
     const int ngone = whole ? 0 : list_gone(from, to);
     double s = 0.0;
     for (int64_t v = from; v < to; v += kThreads * N * E) {
       double w[N * E];
-      weights(w, v + tid * E, kThreads * E, to, ngone, whole);
+      weights(w, v + tid * E, kThreads * E, to, v + kThreads * N * E <= to, ngone, whole);
 #pragma unroll
       for (int e = 0; e < N * E; ++e) s += w[e];
     }
@@ -203,9 +219,11 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
   const double mine = sum_of(lo, hi, false);
   double* sums = a.sums + static_cast<int64_t>(b) * a.chunks;
   if (tid == 0) {
+    // Written through to the coherence point, and there before the arrival is.
     __hip_atomic_store(sums + chunk, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const uint32_t before =
-        __hip_atomic_fetch_add(a.arrived + b, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_fetch_add(a.arrived + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last = before == static_cast<uint32_t>(a.chunks - 1);
     if (last) __hip_atomic_store(a.arrived + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
@@ -276,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
   for (int64_t v0 = from; v0 < to; v0 += kThreads * P) {
     const int64_t v = v0 + tid * P;
     double w[P];
-    weights(w, v, E, to, ngone, whole);
+    weights(w, v, E, to, v0 + kThreads * P <= to, ngone, whole);
     double s = 0.0;
 #pragma unroll
     for (int e = 0; e < P; ++e) s += w[e];
@@ -352,7 +370,7 @@ extern "C" hxm_status hxm_verify_draft(const int32_t* tokens, const int32_t* par
   a.path = path, a.counts = counts, a.next = next_tokens;
   a.batch = static_cast<int>(batch), a.nodes = static_cast<int>(nodes);
   const int64_t want = std::max(int64_t(1), kGroups / batch);
-  a.chunk = std::max(kLeastChunk, ceil_div(ceil_div(vocab, want), 64) * 64);
+  a.chunk = ceil_div(ceil_div(vocab, want), kBlock) * kBlock;
   a.chunks = static_cast<int>(ceil_div(vocab, a.chunk));
   hipStream_t s = as_stream(stream);
   void* ws = nullptr;
