@@ -1,7 +1,7 @@
 // How the attention kernels over a paged cache cut a batch into pieces, one for a
 // workgroup, on the device (the arithmetic is host_logic.h's).  Args has batch, heads
 // (workgroups that read a piece), lens, capacity (tokens a table row holds) and window
-// (of the last tokens, 0: all).
+// (of the last tokens, 0: all); with STEPS whole, which says that no sequence is cut.
 #pragma once
 
 #include "device_util.h"
@@ -66,7 +66,9 @@ __device__ __forceinline__ Piece find_piece(const Args& a, uint32_t u, int lane)
   auto length = [&](int b) { return b < a.batch ? a.lens[b] : 0; };
   Piece r{};
   r.b = -1;
-  if (a.batch > kAttnCutBatch) {  // a whole sequence each
+  bool whole = a.batch > kAttnCutBatch;
+  if constexpr (STEPS) whole = a.whole;
+  if (whole) {  // a sequence each
     if (u >= static_cast<uint32_t>(a.batch)) return r;
     const int32_t len = a.lens[u];
     r.b = static_cast<int>(u), r.n = tokens(len, &r.lo), r.over = len > a.capacity;

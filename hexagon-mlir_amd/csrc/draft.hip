@@ -59,6 +59,7 @@ struct End {
   uint64_t kept;   // a bit each
   uint64_t tried;  // its children that were tried, none kept
   int token;       // lane i: node i's token
+  double first;    // node 0's random number
 };
 template <typename T, bool DRAFT>
 __device__ __forceinline__ End walk(const VerifyArgs& a, int b, int lane) {
@@ -69,7 +70,7 @@ __device__ __forceinline__ End walk(const VerifyArgs& a, int b, int lane) {
   const double u = a.uniform[at];
   // No child: past the nodes, of no earlier node, or of a token that is none.
   const bool child = in && parent >= 0 && parent < lane && token >= 0 && token < a.vocab;
-  End r{-1, 0, 0, 0, token};
+  End r{-1, 0, 0, 0, token, lane_f64(u, 0)};
   if (__builtin_amdgcn_readfirstlane(parent) != -1) return r;
   double p = 0.0, q = 1.0;
   if (child) {
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void verify_draft_kernel(VerifyArgs a) {
     if (tid == 0) a.next[b] = -1;
     return;
   }
-  const double point = static_cast<double>(a.uniform[static_cast<int64_t>(b) * a.nodes]) * total;
+  const double point = end.first * total;
   int64_t from = 0, to = a.vocab;
   double before = 0.0;
   if (!whole) {

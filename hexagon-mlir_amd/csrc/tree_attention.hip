@@ -38,6 +38,7 @@ struct TreeArgs {
   int window;  // tokens that some node of a sequence sees (the last ones, 0: all)
   int reach;   // and that one node sees
   float scale;
+  bool whole;  // no sequence is cut
 };
 
 typedef float v8f32 __attribute__((ext_vector_type(8)));
@@ -599,7 +600,9 @@ int tile_rows(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 template <typename T, int DT>
 hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
   const int rows = tile_rows(int64_t(a.nodes) * a.group);
-  const int64_t pairs = ceil_div(attn_grid(a.batch, a.heads, a.capacity, tree_groups(DT)), a.tiles);
+  const int64_t pairs =
+      a.whole ? int64_t(a.batch) * a.hkv
+              : ceil_div(attn_grid(a.batch, a.heads, a.capacity, tree_groups(DT)), a.tiles);
   const int64_t groups = ceil_div(pairs, 8) * 8 * a.tiles;
   const int per = 256 / (a.dim / 4), slices = static_cast<int>(ceil_div(rows, per));
   const int64_t joins = int64_t(a.batch) * a.heads * slices;
@@ -619,8 +622,7 @@ hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
   else if (rows == 64) launch(std::integral_constant<int, 2>{});
   else launch(std::integral_constant<int, 4>{});
   if ((st = check_launch("tree attention")) != HXM_OK) return st;
-  // Sequences of up to kAttnWhole units are one piece each.
-  if (a.batch > kAttnCutBatch || a.capacity <= kAttnWhole * kAttnUnit - kAttnTile) return ok();
+  if (a.whole) return ok();
   tree_join_kernel<T, tree_groups(DT)>
       <<<static_cast<unsigned>(joins), 256, 0, stream>>>(a, rows, slices);
   return check_launch("tree attention join");
@@ -703,7 +705,9 @@ extern "C" hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* ou
   a.scale = scale;
   // Partial results of the sequences cut in pieces.
   hipStream_t s = as_stream(stream);
-  if (batch <= kAttnCutBatch && a.capacity > kAttnWhole * kAttnUnit - kAttnTile) {
+  // Sequences of up to kAttnWhole units are one piece each.
+  a.whole = batch > kAttnCutBatch || a.capacity <= kAttnWhole * kAttnUnit;
+  if (!a.whole) {
     const uint32_t pieces = tree_groups(a.dim);
     const int64_t slots = std::min(attn_grid(batch, a.heads, a.capacity, pieces),
                                    int64_t(2 * kAttnFine * pieces));

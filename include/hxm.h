@@ -648,7 +648,8 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * or BF16, one for q, cache and out; precision as in hxm_paged_attention.  out
  * must not overlap q; out and lse nothing else.  Sequences are split over
  * workgroups (in batches of up to 256) and joined in a fixed order.  Uses the
- * per-stream workspace where table_pages * page_size is 481 or more. */
+ * per-stream workspace where table_pages * page_size is over 512 and batch up to
+ * 256. */
 hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
                               const hxm_kv_cache* cache, const int32_t* block_table,
                               int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
