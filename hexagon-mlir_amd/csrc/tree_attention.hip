@@ -605,7 +605,7 @@ hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
               : ceil_div(attn_grid(a.batch, a.heads, a.capacity, tree_groups(DT)), a.tiles);
   const int64_t groups = ceil_div(pairs, 8) * 8 * a.tiles;
   const int per = 256 / (a.dim / 4), slices = static_cast<int>(ceil_div(rows, per));
-  const int64_t joins = int64_t(a.batch) * a.heads * slices;
+  const int64_t joins = a.whole ? 0 : int64_t(a.batch) * a.heads * slices;
   hxm_status st = check_grid("tree attention", std::max(groups, joins), 256);
   if (st != HXM_OK) return st;
   const unsigned n = static_cast<unsigned>(groups);
@@ -657,10 +657,12 @@ extern "C" hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* ou
                 "%lld, window=%lld",
                 (long long)batch, (long long)nodes, (long long)q_heads, (long long)cache->heads,
                 (long long)window);
-  // 2^22 sequences times heads times tiles of rows keep every count of workgroups in 32 bits.
-  constexpr int64_t kMaxRows = int64_t(1) << 22;
-  if (nodes > kMaxNodes || q_heads > 65535 || batch > kMaxRows ||
-      batch * cache->heads * ceil_div(nodes * (q_heads / cache->heads), 32) > kMaxRows)
+  // 2^18 sequences times heads times tiles of rows: neither launch then holds more than 2^23
+  // workgroups of 256.
+  constexpr int64_t kMaxHeads = int64_t(1) << 18;
+  const int64_t of_head = std::min(nodes, int64_t(kMaxNodes)) * (q_heads / cache->heads);
+  if (nodes > kMaxNodes || q_heads > 65535 || batch > kMaxHeads ||
+      batch * cache->heads * ceil_div(of_head, tile_rows(of_head)) > kMaxHeads)
     return fail(HXM_UNSUPPORTED_SHAPE,
                 "tile-alignment: tree_attention batch=%lld, nodes=%lld, %lld heads",
                 (long long)batch, (long long)nodes, (long long)q_heads);

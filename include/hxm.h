@@ -23,7 +23,8 @@
  *     decoder-layer operators) may be captured; the tuners, the
  *     resident-weight cache and hxm_release_cache allocate or synchronise and
  *     may not.  A compute entry that uses the per-stream workspace (f32
- *     operands, a [K,N] B, a K split, paged attention, adapters) needs it
+ *     operands, a [K,N] B, a K split, paged and tree attention, drafted
+ *     tokens' verification, adapters) needs it
  *     already large enough: one call of the shape on the stream before the
  *     capture grows it (it is kept until hxm_release_cache, also past a later
  *     growth once a graph has captured it).  Such a graph holds the workspace
@@ -490,7 +491,10 @@ hxm_status hxm_layernorm_rows(const void* x, int64_t ldx, const void* gamma,
  * What a decoder layer needs around its projections and its FFN block: the
  * norms on both sides of a block with the residual add between them, rotary
  * positions with the paged key-value cache, attention of one new token per
- * sequence over that cache, and low-rank adapters beside a projection.  They
+ * sequence over that cache, low-rank adapters beside a projection, and a step
+ * with drafted tokens: the heads' norms before the rotation, attention of a
+ * chain or tree of tokens, their verification, and the moves in the cache that
+ * follow (the kept rows, pages of sequences that fork).  They
  * have no counterpart in the reference, which stops at the single linalg ops;
  * they continue its row reductions and its int8 matmuls.  All are for
  * inference (no backward pass). */
@@ -588,8 +592,8 @@ typedef struct hxm_head_norm {
 
 /* hxm_rope_append with the norms of the query and key heads in the same pass:
  * q[t] and k[t] are normed head by head, then rotated; v is stored as it is.
- * fp32 from the load to the one rounding.  Everything else as there (q_norm is
- * not read with q_heads 0). */
+ * fp32 from the load to the one rounding.  gamma and beta must not overlap q_out
+ * or the cache.  Everything else as there (q_norm is not read with q_heads 0). */
 hxm_status hxm_norm_rope_append(const hxm_heads* q, const hxm_heads* q_out, int64_t q_heads,
                                 const hxm_heads* k, const hxm_heads* v,
                                 const hxm_head_norm* q_norm, const hxm_head_norm* k_norm,
@@ -646,8 +650,9 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * it; of nodes that see a token of a page outside [0, pages); of a sequence of 0 <
  * n < nodes tokens, or of more than table_pages * page_size or 2^30.  dtype F16
  * or BF16, one for q, cache and out; precision as in hxm_paged_attention.  out
- * must not overlap q; out and lse nothing else.  Sequences are split over
- * workgroups (in batches of up to 256) and joined in a fixed order.  Uses the
+ * must not overlap q; out and lse nothing else.  batch * cache->heads, times the tiles of
+ * 32, 64 or 128 that nodes * q_heads / cache->heads rows make, up to 2^18.  Sequences are
+ * split over workgroups (in batches of up to 256) and joined in a fixed order.  Uses the
  * per-stream workspace where table_pages * page_size is over 512 and batch up to
  * 256. */
 hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,

@@ -1,11 +1,18 @@
-"""The refusals of the C entries of a step with drafted tokens, every one before the device
-is touched.  Every call starts from one that is right (it gets as far as the missing device)
+"""The operators of a step with drafted tokens on the host: their arithmetic under
+AddressSanitizer and UndefinedBehaviorSanitizer (tests/sanitize/draft_logic_check.cpp), and
+the refusals of their C entries, every one before the device is touched.  Every call starts from one that is right (it gets as far as the missing device)
 and changes one thing; the addresses are stand-ins, 1 MiB apart."""
+import os
+import shutil
+import subprocess
+
 import pytest
 import torch
 
 import hxm
 from hxm import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 INVALID, SHAPE, DTYPE = (_lib.HXM_INVALID_ARG, _lib.HXM_UNSUPPORTED_SHAPE,
                          _lib.HXM_UNSUPPORTED_DTYPE)
@@ -15,6 +22,20 @@ MB = 1 << 20
 
 pytestmark = pytest.mark.skipif(torch.cuda.device_count() > 0,
                                 reason="stand-in addresses: only where nothing can launch")
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_draft_logic_under_asan_and_ubsan(tmp_path):
+    exe = tmp_path / "draft_logic_check"
+    src = os.path.join(ROOT, "tests", "sanitize", "draft_logic_check.cpp")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fno-omit-frame-pointer",
+                    "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-Wall", "-Werror", src, "-o", str(exe)], check=True, timeout=300)
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=1:abort_on_error=0",
+               UBSAN_OPTIONS="print_stacktrace=1:halt_on_error=1")
+    env.pop("LD_PRELOAD", None)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and "draft logic ok" in r.stdout, r.stdout + r.stderr
 
 
 def _refused(status, want):
