@@ -143,6 +143,8 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeArgs a) {
   }
 }
 
+typedef float v8f32 __attribute__((ext_vector_type(8)));
+
 // The norms of the heads in front of it: gamma and beta rows of a head, `hs` apart.
 struct HeadNorm {
   const void *gamma, *beta;
@@ -214,7 +216,6 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(NormRopeArgs a) {
                        : static_cast<const T*>(a.k.p) + t * a.k.ts + hh * a.k.hs;
     T* dst = isq ? static_cast<T*>(const_cast<void*>(a.qo.p)) + t * a.qo.ts + hh * a.qo.hs
                  : kc + hh * a.khs;
-    float x[kChunk], y[kChunk];
     RawVec<T> rx = RawVec<T>(T(0)), ry = rx, gx = rx, gy = rx, bx = rx, by = rx;
     if (on) {
       rx = load_n(src + lo, n);
@@ -231,56 +232,56 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(NormRopeArgs a) {
       }
     }
     // (load_n leaves zeros past n.)
-#pragma unroll
-    for (int e = 0; e < kChunk; ++e) x[e] = tof(rx[e]), y[e] = tof(ry[e]);
-    float mean = 0.0f, ss = 0.0f;
+    v8f32 x = __builtin_convertvector(rx, v8f32), y = __builtin_convertvector(ry, v8f32);
     if (nm.kind == HXM_NORM_LAYER) {
+      float mean = 0.0f;
 #pragma unroll
       for (int e = 0; e < kChunk; ++e) mean += x[e] + y[e];
-    }
-    mean = group_sum(mean, a.lanes) * count;
-    if (nm.kind == HXM_NORM_LAYER) {
+      mean = group_sum(mean, a.lanes) * count;
 #pragma unroll
       for (int e = 0; e < kChunk; ++e) {
         x[e] = e < n ? x[e] - mean : 0.0f;
         y[e] = two && e < n ? y[e] - mean : 0.0f;
       }
     }
+    float ss = 0.0f;
 #pragma unroll
     for (int e = 0; e < kChunk; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
     ss = group_sum(ss, a.lanes) * count;
     if (!on) continue;
     if (nm.kind != HXM_NORM_NONE) {
       const float r = 1.0f / sqrtf(ss + nm.eps);
-#pragma unroll
-      for (int e = 0; e < kChunk; ++e) {
-        x[e] *= r, y[e] *= r;
-        if (nm.gamma) x[e] *= tof(gx[e]), y[e] *= tof(gy[e]);
-        if (nm.beta) x[e] += tof(bx[e]), y[e] += tof(by[e]);
+      x *= r, y *= r;
+      if (nm.gamma) {
+        x *= __builtin_convertvector(gx, v8f32);
+        if (!PAIRS) y *= __builtin_convertvector(gy, v8f32);
+      }
+      if (nm.beta) {
+        x += __builtin_convertvector(bx, v8f32);
+        if (!PAIRS) y += __builtin_convertvector(by, v8f32);
       }
     }
-    RawVec<T> ox, oy;
-    if (PAIRS && turned) {
+    if (turned) {
+      v8f32 u;
+      if constexpr (PAIRS) {
 #pragma unroll
-      for (int e = 0; e < kChunk / 2; ++e) {
-        const int k = PAIRS ? e : 0;
-        const float u = x[2 * e], w = x[2 * e + 1];
-        ox[2 * e] = fromf<T>(fmaf(u, cs[k], -(w * sn[k])));
-        ox[2 * e + 1] = fromf<T>(fmaf(w, cs[k], u * sn[k]));
+        for (int e = 0; e < M; ++e) {
+          u[2 * e] = fmaf(x[2 * e], cs[e], -(x[2 * e + 1] * sn[e]));
+          u[2 * e + 1] = fmaf(x[2 * e + 1], cs[e], x[2 * e] * sn[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < M; ++e) {
+          u[e] = fmaf(x[e], cs[e], -(y[e] * sn[e]));
+          y[e] = fmaf(y[e], cs[e], x[e] * sn[e]);
+        }
+        const RawVec<T> oy = __builtin_convertvector(y, RawVec<T>);
+        if (isq) store_n<true>(dst + lo + half, oy, n);
+        else store_n<false>(dst + lo + half, oy, n);
       }
-    } else if (turned) {
-#pragma unroll
-      for (int e = 0; e < kChunk; ++e) {
-        const int k = PAIRS ? 0 : e;
-        ox[e] = fromf<T>(fmaf(x[e], cs[k], -(y[e] * sn[k])));
-        oy[e] = fromf<T>(fmaf(y[e], cs[k], x[e] * sn[k]));
-      }
-      if (isq) store_n<true>(dst + lo + half, oy, n);
-      else store_n<false>(dst + lo + half, oy, n);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kChunk; ++e) ox[e] = fromf<T>(x[e]);
+      x = u;
     }
+    const RawVec<T> ox = __builtin_convertvector(x, RawVec<T>);
     if (isq) store_n<true>(dst + lo, ox, n);
     else store_n<false>(dst + lo, ox, n);
   }
