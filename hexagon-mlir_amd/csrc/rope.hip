@@ -1,5 +1,6 @@
 // Rotary positions and the append to the paged key-value cache, in one launch:
-// q -> rotated q, k -> rotated k in its cache row, v -> its cache row.
+// q -> rotated q, k -> rotated k in its cache row, v -> its cache row; and the same with a
+// norm of each query and key head before the rotation.
 //
 // Bound by memory: every element of q, k and v is read once and written once (8192 tokens,
 // 32 + 8 heads of 128, bf16: 206 MB in 40 us, 5.1 TB/s; a copy of 1 GiB runs at 5.3); a
@@ -170,7 +171,10 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
 
 // A head's norm, its rotation and its store in one pass over it: the lanes of a head, a
 // power of two, keep its chunks in registers as fp32 from the load to the one rounding
-// and share the statistics.  Threads of a token as above.
+// and share the statistics by DPP sums (LayerNorm: the mean, then the squares around it).
+// Bound by memory as above: 8192 tokens, 32 + 8 heads of 128, bf16, 206 MB in 39.9 us,
+// 5.2 TB/s, what the rotation without norms takes.  (The next head's loads issued before this
+// one's sums: 68 us with 128 threads a token, for 45.7.)
 template <typename T, bool PAIRS>
 __global__ __launch_bounds__(256) void norm_rope_append_kernel(NormRopeArgs a) {
   const int t = blockIdx.x * (256 / a.tt) + static_cast<int>(threadIdx.x) / a.tt;
@@ -526,8 +530,11 @@ extern "C" hxm_status hxm_norm_rope_append(const hxm_heads* q, const hxm_heads* 
   if (tokens == 0) return ok();
   a.lanes = 1;
   while (a.lanes < a.chunks) a.lanes *= 2;
+  // Threads of a token: as rope_append, and one wave where the tokens fill the chip that way
+  // (32 + 8 heads of 128: 8192 tokens 39.9 us with 64, 45.7 with 128, 60 with 256; 4096 19.4,
+  // 20.4, 24.9; 2048 12.9, 11.7, 14.6; 1024 12.1, 9.5, 9.0; 64 8.7, 6.4, 5.3).
   a.tt = 64;
-  const int most = tokens >= 2048 ? 128 : 256;
+  const int most = tokens >= 4096 ? 64 : tokens >= 2048 ? 128 : 256;
   while (a.tt < most && a.tt < a.lanes * (a.hq + a.hkv)) a.tt *= 2;
   const int64_t groups = ceil_div(tokens, 256 / a.tt);
   if ((st = check_grid("norm rope append", groups, 256)) != HXM_OK) return st;

@@ -1,7 +1,40 @@
 // Attention of a tree of drafted tokens per sequence over the paged key-value cache.
 //
 // The rows that share a key head, nodes x group of them, are the 32-wide side of the
-// MFMAs, so that one read of the keys and values serves up to 128 rows.
+// MFMAs, so that one read of the keys and values serves up to 128 rows: 4 * dim bytes a
+// token against 4 * dim * rows operations.  Few rows are bound by memory, many by the matrix
+// cores and the exponentials beside them: 4 sequences to 32768 tokens, 64 nodes, 8 x 4 heads of
+// 128, 109 GFLOP in 201 us (545 TFLOP/s; with the second half of the probabilities, below,
+// 815 on the matrix cores, 43% of their cycles); 16 sequences to 4096, 16 nodes, 46 us, 2.9
+// TB/s, of which the join takes 7 and a workgroup's start and end 9.
+//
+// A workgroup has four waves of 32 rows.  Up to 32 rows, its waves take tokens in turn, each
+// with tiles of its own; up to 64 rows two by two; more, all four share a tile of 64 tokens,
+// and rows past 128 take further workgroups, eight blocks on, so that they run on the same XCD
+// and read the tile from its L2 (210 MB of 424 come from beyond it at 4 x 64 x 32768).
+//
+// S^T = K Q^T leaves lane (h, c) = (lane / 32, lane % 32) 16 scores of row c of 32 tokens,
+// of tokens 8 j + 4 h + 0 .. 3.  O^T = V^T P^T wants 8 tokens of P^T in each lane's right
+// operand; taking exactly those 16 scores as two of them fixes which tokens of V^T the left
+// operand has, and the transposing LDS read delivers those.  So the probabilities stay in the
+// lane they are in, and a row's maximum, sum and output in one column of lanes.
+//
+// Keys and values come in whole rows through registers into LDS, the next tile's on their way
+// while this one is multiplied.  Row t of keys has its 16-byte chunk q at q ^ t % 16 (of 8
+// chunks q ^ t / 2 % 8), row t of values its 64-byte chunk e at e ^ t % 4 (of 2: e ^ t / 2 %
+// 2): no read or write meets a bank twice.
+//
+// A tile that some row does not see the whole of (drafted tokens, the window's edge, the ends)
+// takes a mask of 32 bits a row.  Values there that are no numbers would pass into every row
+// (0 * NaN), so they go into LDS as zeros and join those rows that see them at the very end;
+// inside the loop that branch cost every tile its registers (4 x 64 over 32768: 677 us spilled,
+// 361 without).
+//
+// The running maximum moves only when a score passes it by more than 2^8, as in the
+// attention of one token, and the probabilities enter the second product as two 16-bit
+// halves, the first cut off and not rounded (the rest is exact then, and its rounding leaves
+// 21 bits in f16, 15 in bf16).  One half alone took 170 us for 201 at 4 x 64 over 32768 and added as
+// much to the error as the output's own rounding; elsewhere its time does not show.
 #include <algorithm>
 #include <type_traits>
 
@@ -144,7 +177,8 @@ __device__ __forceinline__ Node node_of(const TreeArgs& a, int b, int ctx, int l
 
 constexpr int tree_waves(int dt) { return dt <= 128 ? 2 : 1; }
 
-// Pieces of a batch: as many as run at once.
+// Pieces of a batch: as many as run at once, two workgroups a CU where registers and LDS hold
+// them (one a CU: 4 x 64 over 32768 361 us for 242, 16 x 16 over 4096 72 for 51).
 constexpr uint32_t tree_groups(int dt) { return (dt <= 128 ? 2 : 1) * kAttnGroups; }
 
 // WR of the four waves side by side over the rows, 32 each, the others over tokens.

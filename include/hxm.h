@@ -649,12 +649,15 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * outputs of a node whose parent (or one above) is padding or no node before
  * it; of nodes that see a token of a page outside [0, pages); of a sequence of 0 <
  * n < nodes tokens, or of more than table_pages * page_size or 2^30.  dtype F16
- * or BF16, one for q, cache and out; precision as in hxm_paged_attention.  out
- * must not overlap q; out and lse nothing else.  batch * cache->heads, times the tiles of
- * 32, 64 or 128 that nodes * q_heads / cache->heads rows make, up to 2^18.  Sequences are
- * split over workgroups (in batches of up to 256) and joined in a fixed order.  Uses the
- * per-stream workspace where table_pages * page_size is over 512 and batch up to
- * 256. */
+ * or BF16, one for q, cache and out; scores, maxima and sums are fp32, the
+ * probabilities enter the product with V with 21 bits (f16; one below 2^-10 of
+ * the largest to 2^-32 of that) or 15 (bf16), as two 16-bit halves (which make a
+ * dim whose V is infinite infinite or NaN).  out must not overlap q; out and lse
+ * nothing else.  batch * cache->heads, times the tiles of 32, 64 or 128 that nodes
+ * * q_heads / cache->heads rows make, up to 2^18.  Sequences are split over
+ * workgroups (in batches of up to 256) and joined in a fixed order.  Uses the
+ * per-stream workspace where table_pages * page_size is over 512 and batch up
+ * to 256. */
 hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
                               const hxm_kv_cache* cache, const int32_t* block_table,
                               int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
