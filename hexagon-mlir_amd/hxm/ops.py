@@ -758,16 +758,21 @@ def _kv_cache(k: torch.Tensor, v: torch.Tensor):
     """The hxm_kv_cache of [pages, heads, page_size, dim] tensors of any strides
     (a cache that keeps tokens before heads is passed transposed), its heads
     and dim, dtype and device."""
+    if k.dim() != 4:
+        raise ValueError(f"k_cache must be [pages, heads, page_size, dim] (got {tuple(k.shape)})")
+    return _kv_pack(k, v, k.shape, k.stride(), v.stride())
+
+
+def _kv_pack(k: torch.Tensor, v: torch.Tensor, shape, k_strides, v_strides):
+    """_kv_cache() of a layer of this shape and these strides at the start of k and v."""
     dev = _on_current(k, "k_cache")
-    dtype, shape = k.dtype, k.shape
-    if len(shape) != 4:
-        raise ValueError(f"k_cache must be [pages, heads, page_size, dim] (got {tuple(shape)})")
+    dtype = k.dtype
     if dtype not in _HALVES:
         raise TypeError(f"k_cache must be {' or '.join(str(d) for d in _HALVES)} (got {dtype})")
-    _tensor(v, dtype, shape, dev, "v_cache")
+    _tensor(v, dtype, k.shape, dev, "v_cache")
     pages, heads, page, dim = shape
-    kp, kh, kt, ki = k.stride()
-    vp, vh, vt, vi = v.stride()
+    kp, kh, kt, ki = k_strides
+    vp, vh, vt, vi = v_strides
     if ki != 1 or vi != 1:
         raise ValueError("k_cache and v_cache must have a contiguous last dimension")
     return (KV_CACHE.pack(k.data_ptr(), v.data_ptr(), pages, page, heads, dim, kp, kh, kt, vp, vh,
@@ -849,21 +854,24 @@ def _head_norm(kind: str, eps: float, weight, bias, heads: int, dim: int, dtype,
     """The hxm_head_norm, and the tensors it points to (to be kept until the call)."""
     if kind not in _NORMS:
         raise ValueError(f"norm must be one of {sorted(_NORMS)} (got {kind!r})")
-    each = any(t is not None and t.dim() == 2 for t in (weight, bias))
-    ptrs, keep = [], []
-    for t, what in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            ptrs.append(0)
-            continue
-        if t.shape != ((heads, dim) if each else (dim,)) or t.dtype != dtype or \
-                t.get_device() != dev:
-            raise ValueError(f"{name}_{what} must be {dtype} [{dim}] or [{heads}, {dim}], like its "
-                             f"{'bias' if what == 'weight' else 'weight'}, on cuda:{dev} "
-                             f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
-        t = t.contiguous()
-        keep.append(t)
-        ptrs.append(t.data_ptr())
-    return (HEAD_NORM.pack(_NORMS[kind], eps, *ptrs, dim if each else 0), *keep)
+    each = (weight is not None and weight.dim() == 2) or (bias is not None and bias.dim() == 2)
+    shape = (heads, dim) if each else (dim,)
+    w, w_ptr = _head_param(weight, dtype, shape, dev, name, "weight")
+    b, b_ptr = _head_param(bias, dtype, shape, dev, name, "bias")
+    return HEAD_NORM.pack(_NORMS[kind], eps, w_ptr, b_ptr, dim if each else 0), w, b
+
+
+def _head_param(t: Optional[torch.Tensor], dtype: torch.dtype, shape, dev: int, name: str,
+                what: str):
+    """(contiguous t, its address): of this shape and dtype on this device, or None."""
+    if t is None:
+        return None, 0
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+        raise ValueError(f"{name}_{what} must be {dtype} {shape} on cuda:{dev}, [{shape[-1]}] for "
+                         f"all heads or [heads, {shape[-1]}], like its other parameter "
+                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
+    t = t.contiguous()
+    return t, t.data_ptr()
 
 
 @_on_stream
@@ -951,12 +959,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if q.dim() != 4:
         raise ValueError(f"q must be [batch, tokens, heads, dim] (got {tuple(q.shape)})")
     B, T, hq, _ = q.shape
-    qh = _heads(_tokens(q, "q"), dtype, (B * T, hq, dim), dev, "q")
+    qh = _token_heads(q, dtype, (B, T, hq, dim), dev, "q")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape:
-        _tensor(out, dtype, q.shape, dev, "out")
-    oh = _heads(_tokens(out, "out"), dtype, (B * T, hq, dim), dev, "out")
+    oh = _token_heads(out, dtype, (B, T, hq, dim), dev, "out")
     table_p, ld_table, table_pages = _block_table(block_table, B, dev)
     lens_p = _ints(seq_lens, (B,), dev, "seq_lens")
     parents_p = None if parents is None else _ints(parents, (B, T), dev, "parents")
@@ -970,6 +976,20 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if st:
         check(st, "hxm_tree_attention")
     return (out, lse) if return_lse else out
+
+
+def _token_heads(t: torch.Tensor, dtype: torch.dtype, shape, dev: int, name: str) -> bytes:
+    """The hxm_heads of a [batch, tokens, heads, dim] tensor, its tokens one after the
+    other over the batch."""
+    if t.dtype != dtype or t.shape != shape or t.get_device() != dev:
+        _tensor(t, dtype, shape, dev, name)
+    bs, ts, hs, inner = t.stride()
+    if inner != 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
+    B, T = shape[0], shape[1]
+    if B > 1 and T > 1 and bs != T * ts:
+        raise ValueError(f"{name}'s tokens must be evenly strided over the batch")
+    return HEADS.pack(t.data_ptr(), ts if T > 1 else bs, hs)
 
 
 def _tokens(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -1028,8 +1048,9 @@ def _kv_layers(k: torch.Tensor, v: torch.Tensor):
     if k.dim() != 5 or v.shape != k.shape or not k.shape[0]:
         raise ValueError("k_cache and v_cache must be [pages, heads, page_size, dim], or with a "
                          f"dimension of layers before (got {tuple(k.shape)}, {tuple(v.shape)})")
-    cache, _, _, dtype, dev = _kv_cache(k[0], v[0])
-    return cache, k.shape[0], k.stride(0), v.stride(0), dtype, dev
+    ks, vs = k.stride(), v.stride()
+    cache, _, _, dtype, dev = _kv_pack(k, v, k.shape[1:], ks[1:], vs[1:])
+    return cache, k.shape[0], ks[0], vs[0], dtype, dev
 
 
 @_on_stream
