@@ -377,3 +377,68 @@ def test_wrong_arguments_are_refused(dev):
     refused(hxm.HxmError, *ok, scale=NAN)
     refused(hxm.HxmError, *ok, out=q)
     refused(ValueError, *ok, out=z(3, 5, 4, 32))
+
+
+def test_offsets_past_32_bits(dev):
+    """A cache of more than 2^31 elements, its last pages in use; and rows too far apart for
+    32-bit offsets within a page."""
+    pages, page, heads, dim, T = 70000, 16, 8, 256, 3
+    kc = torch.zeros(pages, heads, page, dim, dtype=torch.bfloat16, device=dev)
+    vc = torch.zeros_like(kc)
+    assert kc.numel() > 2 ** 31
+    g = torch.Generator().manual_seed(5)
+    ids = [pages - 1, 3, pages - 2]
+    small = [torch.randn(4, heads, page, dim, generator=g).bfloat16().to(dev) for _ in range(2)]
+    for i, p in enumerate(ids):
+        kc[p], vc[p] = small[0][i], small[1][i]
+    q = torch.randn(1, T, 16, dim, generator=g).bfloat16().to(dev)
+    lens = torch.tensor([45], dtype=torch.int32, device=dev)
+    near = ops.tree_attention(q, *small, torch.tensor([[0, 1, 2]], dtype=torch.int32, device=dev),
+                              lens)
+    far = ops.tree_attention(q, kc, vc, torch.tensor([ids], dtype=torch.int32, device=dev), lens)
+    assert torch.equal(near, far)
+    del kc, vc
+    apart = 2 ** 26 + 8
+    wide = [torch.zeros(16 * apart, dtype=torch.bfloat16, device=dev).as_strided(
+        (1, 1, 16, 64), (16 * apart, 16 * apart, apart, 1)) for _ in range(2)]
+    packed = [torch.randn(1, 1, 16, 64, generator=g).bfloat16().to(dev) for _ in range(2)]
+    for w, p in zip(wide, packed):
+        w.copy_(p)
+    q = torch.randn(1, T, 2, 64, generator=g).bfloat16().to(dev)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    lens = torch.tensor([14], dtype=torch.int32, device=dev)
+    assert torch.equal(ops.tree_attention(q, *packed, table, lens),
+                       ops.tree_attention(q, *wide, table, lens))
+
+
+def test_same_results_every_time_and_on_streams_at_once(dev):
+    """Results repeat bit for bit, also beside another stream's calls, whose workspace is its own."""
+    g = torch.Generator().manual_seed(6)
+    jobs = []
+    for lens, T, group in (([3000, 40, 700], 6, 4), ([900, 2000], 20, 5)):
+        rows = trees(g, lens, T, "ragged")
+        q, kc, vc, table, ld, _ = build(g, "f16", lens, T, rows, 2, group, 128, 16, "nhd", dev)
+        jobs.append((q.to(dev), kc, vc, table, ld, torch.tensor(rows, dtype=torch.int32, device=dev)))
+    want = [ops.tree_attention(*j, return_lse=True) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = [ops.tree_attention(*j, return_lse=True, stream=s) for j, s in zip(jobs, streams)]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_a_call_of_its_own_beside_other_sequences(dev):
+    """A sequence that is not cut gives the same alone and in a batch."""
+    g = torch.Generator().manual_seed(7)
+    lens, T = [100, 333, 500, 64], 5
+    rows = trees(g, lens, T, "full")
+    q, kc, vc, table, ld, _ = build(g, "bf16", lens, T, rows, 2, 4, 64, 16, "hnd", dev)
+    parents = torch.tensor(rows, dtype=torch.int32, device=dev)
+    q = q.to(dev)
+    all_of_them = ops.tree_attention(q, kc, vc, table, ld, parents)
+    for b in range(len(lens)):
+        one = ops.tree_attention(q[b:b + 1], kc, vc, table[b:b + 1].contiguous(), ld[b:b + 1],
+                                 parents[b:b + 1])
+        assert torch.equal(one[0], all_of_them[b]), b

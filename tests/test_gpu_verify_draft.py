@@ -253,3 +253,40 @@ def test_wrong_arguments_are_refused(dev):
         ops.verify_draft(z(1, 4, dt=i), z(1, 4, 0), z(1, 4))
     none = ops.verify_draft(z(0, 4, dt=i), z(0, 4, 8), z(0, 4))
     assert [tuple(t.shape) for t in none] == [(0, 4), (0,), (0,)]
+
+
+def test_offsets_past_32_bits(dev):
+    """Rows of the tables beyond 2^31 elements."""
+    B, T, V = 3, 4, 200_000_000
+    p = torch.zeros(B, T, V, dtype=torch.float16, device=dev)
+    assert p.numel() > 2 ** 31
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)                 # noqa: E731
+    far = [V - 3, 150_000_001, 7]
+    for b in range(B):
+        p[b, :, far[b]], p[b, :, 5] = 0.75, 0.25
+    tokens = i([[1] + [f] * 3 for f in far])
+    u = torch.full((B, T), 0.5, device=dev)
+    u[:, 3] = 0.9                                  # 0.9 of 1 is not below 0.75
+    path, counts, following = ops.verify_draft(tokens, p, u)
+    assert counts.tolist() == [3] * B and path.tolist() == [[0, 1, 2, -1]] * B
+    assert following.tolist() == [5] * B           # what is left of the third row
+    u[:, 3] = 0.1
+    path, counts, following = ops.verify_draft(tokens, p, u)
+    assert counts.tolist() == [4] * B
+    assert following.tolist() == far
+
+
+def test_streams_at_once(dev):
+    """Calls on two streams beside each other: each has its own sums and counters."""
+    g = torch.Generator().manual_seed(8)
+    jobs = [tuple(t.to(dev) for t in case(g, B, 5, V, "chain", torch.float32, True))
+            for B, V in ((20, 30000), (7, 120000))]
+    call = lambda j, s=None: ops.verify_draft(j[1], j[2], j[4], j[0], j[3], stream=s)  # noqa: E731
+    want = [call(j) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = [call(j, s) for j, s in zip(jobs, streams)]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
