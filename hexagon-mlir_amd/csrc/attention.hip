@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kWaves * 64)
   __shared__ int last;
 
   const int head = blockIdx.x % a.heads;
-  const Piece w = find_piece<false>(a, blockIdx.x / a.heads, lane);
+  const Piece w = find_piece(a, blockIdx.x / a.heads, lane);
   if (w.b < 0) return;
   const int tile = head % a.tiles, hk = head / a.tiles;
   const int rows = min(kHeads, a.group - tile * kHeads);  // query heads here

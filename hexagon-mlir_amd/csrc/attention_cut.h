@@ -45,13 +45,13 @@ struct Piece {
   bool over;          // longer than its table row
 };
 
-// Piece u of the batch (BY_SEQUENCE: the first piece of sequence u), its sequences in order, cut as host_logic.h says.  Every wave
+// Piece u of the batch, its sequences in order, cut as host_logic.h says.  Every wave
 // works it out from the lengths, 64 sequences at a time, all loaded at once: they are on
 // the device, so the host cannot.  Batches of more than 64 take the fine pieces without
 // trying the others, which took 13 us instead of 15.4 for 256 x 600 tokens, one head, 12.3 for
 // 13.7 (128 x 600, two) and 149 for 152 (256 x 2048, eight), and 15 for 11.6 where few tokens
 // are many sequences' (65 x 1024, one head) and 30 for 25 (200 x 2048, one).
-template <bool BY_SEQUENCE, uint32_t GROUPS = kAttnGroups, bool STEPS = false, typename Args>
+template <uint32_t GROUPS = kAttnGroups, bool STEPS = false, typename Args>
 __device__ __forceinline__ Piece find_piece(const Args& a, uint32_t u, int lane) {
   auto tokens = [&](int32_t len, int* lo) {
     const int n = len > a.capacity ? 0 : max(len, 0);
@@ -101,8 +101,7 @@ __device__ __forceinline__ Piece find_piece(const Args& a, uint32_t u, int lane)
     if (64 * i >= a.batch) break;
     const uint32_t c = attn_cut(w[i], size), cs = c > 1 ? c : 0u;
     const uint32_t upto = wave_scan(c, lane), upto_s = wave_scan(cs, lane);
-    const uint64_t hit = __ballot(BY_SEQUENCE ? u == static_cast<uint32_t>(64 * i + lane)
-                                              : u < first + upto);
+    const uint64_t hit = __ballot(u < first + upto);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       const int32_t len_l = static_cast<int32_t>(lane_u32(static_cast<uint32_t>(len[i]), l));
@@ -112,7 +111,7 @@ __device__ __forceinline__ Piece find_piece(const Args& a, uint32_t u, int lane)
       r.n = tokens(len_l, &r.lo);
       r.over = len_l > a.capacity;
       r.pieces = static_cast<int>(pieces);
-      r.index = BY_SEQUENCE ? 0 : static_cast<int>(u - (first + lane_u32(upto, l) - pieces));
+      r.index = static_cast<int>(u - (first + lane_u32(upto, l) - pieces));
       r.slot = slots + lane_u32(upto_s, l) - lane_u32(cs, l);
       r.begin = (r.lo & ~static_cast<int>(kAttnTile - 1)) + r.index * step;
       r.end = r.index + 1 < r.pieces ? min(r.n, r.begin + step) : r.n;

@@ -5,8 +5,8 @@
 // token against 4 * dim * rows operations.  Few rows are bound by memory, many by the matrix
 // cores and the exponentials beside them: 4 sequences to 32768 tokens, 64 nodes, 8 x 4 heads of
 // 128, 109 GFLOP in 201 us (545 TFLOP/s; with the second half of the probabilities, below,
-// 815 on the matrix cores, 43% of their cycles); 16 sequences to 4096, 16 nodes, 46 us, 2.9
-// TB/s, of which the join takes 7 and a workgroup's start and end 9.
+// 815 on the matrix cores, 43% of their cycles); 16 sequences to 4096, 16 nodes, 45 us, 3.0
+// TB/s, of which the join takes 6 and a workgroup's start and end 9.
 //
 // A workgroup has four waves of 32 rows.  Up to 32 rows, its waves take tokens in turn, each
 // with tiles of its own; up to 64 rows two by two; more, all four share a tile of 64 tokens,
@@ -64,6 +64,7 @@ struct TreeArgs {
   int64_t q_ts, q_hs, o_ts, o_hs;
   int64_t kps, khs, kts, vps, vhs, vts;
   int64_t ld_table, capacity;  // tokens a table row holds
+  int2* cuts;  // [batch]: pieces of a sequence and the partial slots before them
   float* parts;
   uint32_t pages, page_size;
   FastDiv page_div;
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(kWaves * 64)
   const uint32_t pair = blockIdx.x / (8u * a.tiles) * 8u + blockIdx.x % 8u;
   const int tile = static_cast<int>(blockIdx.x / 8u % static_cast<uint32_t>(a.tiles));
   const int hk = static_cast<int>(pair % static_cast<uint32_t>(a.hkv));
-  const Piece w = find_piece<false, tree_groups(DT), true>(a, pair / static_cast<uint32_t>(a.hkv), lane);
+  const Piece w = find_piece<tree_groups(DT), true>(a, pair / static_cast<uint32_t>(a.hkv), lane);
   if (w.b < 0) return;
   const int D = a.dim;
   const int b = w.b, n = w.n, lo = w.lo;
@@ -510,6 +511,8 @@ __global__ __launch_bounds__(kWaves * 64)
     }
   __syncthreads();
 
+  if (!a.whole && w.index == 0 && hk == 0 && tile == 0 && threadIdx.x == 0)
+    a.cuts[b] = make_int2(w.pieces, static_cast<int>(w.slot));
   const int tile0 = tile * 32 * WR, rows = min(32 * WR, total - tile0);
   const int d4 = D / 4, items = rows * d4;
   const int64_t slot_floats = static_cast<int64_t>(32 * WR) * (D + 2);
@@ -571,16 +574,16 @@ __global__ __launch_bounds__(kWaves * 64)
 }
 
 // Joins the pieces of the sequences that were cut, in their order: a thread a row's four
-// dims.
-template <typename T, uint32_t GROUPS>
+// dims.  How a sequence was cut its first workgroup has written down (worked out again from the
+// lengths, 16 x 16 over 4096 took 45.9 us for 44.7).
+template <typename T>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int tile_rows, int slices) {
-  const int lane = threadIdx.x & 63;
   const uint32_t x = blockIdx.x / static_cast<uint32_t>(slices);
   const int slice = static_cast<int>(blockIdx.x % static_cast<uint32_t>(slices));
   const int b = static_cast<int>(x / static_cast<uint32_t>(a.heads));
   const int ht = static_cast<int>(x % static_cast<uint32_t>(a.heads));
-  const Piece w = find_piece<true, GROUPS, true>(a, static_cast<uint32_t>(b), lane);
-  if (w.b < 0 || w.pieces < 2) return;
+  const int pieces = a.cuts[b].x, slot = a.cuts[b].y;
+  if (pieces < 2) return;
   const int D = a.dim, d4 = D / 4, per = 256 / d4;
   const int hk = ht / a.tiles, tile = ht % a.tiles;
   const int r = slice * per + static_cast<int>(threadIdx.x) / d4;
@@ -590,22 +593,22 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int tile_row
     return;
   const int64_t slot_floats = static_cast<int64_t>(tile_rows) * (D + 2);
   const float* part =
-      a.parts + (static_cast<int64_t>(w.slot) * a.heads + ht * static_cast<int64_t>(w.pieces)) *
+      a.parts + (static_cast<int64_t>(slot) * a.heads + ht * static_cast<int64_t>(pieces)) *
                     slot_floats;
   float M = -__builtin_huge_valf(), L = 0.0f;
   v4f32 o = v4f32(0.0f);
-  for (int s = 0; s < w.pieces; s += 8) {
+  for (int s = 0; s < pieces; s += 8) {
     v4f32 y[8];
     float mm[8], ll[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float* at = part + min(s + i, w.pieces - 1) * slot_floats;
+      const float* at = part + min(s + i, pieces - 1) * slot_floats;
       mm[i] = at[2 * r], ll[i] = at[2 * r + 1];
       y[i] = *reinterpret_cast<const v4f32*>(at + 2 * tile_rows + r * D + 4 * d);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (s + i >= w.pieces) break;
+      if (s + i >= pieces) break;
       const float mn = fmaxf(M, mm[i]);
       const float fa = __builtin_amdgcn_exp2f(M - finite(mn));
       const float fb = __builtin_amdgcn_exp2f(mm[i] - finite(mn));
@@ -657,8 +660,7 @@ hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
   else launch(std::integral_constant<int, 4>{});
   if ((st = check_launch("tree attention")) != HXM_OK) return st;
   if (a.whole) return ok();
-  tree_join_kernel<T, tree_groups(DT)>
-      <<<static_cast<unsigned>(joins), 256, 0, stream>>>(a, rows, slices);
+  tree_join_kernel<T><<<static_cast<unsigned>(joins), 256, 0, stream>>>(a, rows, slices);
   return check_launch("tree attention join");
 }
 
@@ -739,7 +741,7 @@ extern "C" hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* ou
   a.reach = window >= kAttnMaxTokens ? 0 : static_cast<int>(window);
   a.window = a.reach > 0 ? a.reach + a.nodes - 1 : 0;
   a.scale = scale;
-  // Partial results of the sequences cut in pieces.
+  // How the sequences were cut, and the partial results of those in pieces.
   hipStream_t s = as_stream(stream);
   // Sequences of up to kAttnWhole units are one piece each.
   a.whole = batch > kAttnCutBatch || a.capacity <= kAttnWhole * kAttnUnit;
@@ -748,9 +750,12 @@ extern "C" hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* ou
     const int64_t slots = std::min(attn_grid(batch, a.heads, a.capacity, pieces),
                                    int64_t(2 * kAttnFine * pieces));
     void* ws = nullptr;
-    st = stream_workspace(s, static_cast<size_t>(slots * rows * (a.dim + 2) * 4), &ws, kWsLayer);
+    const int64_t cuts = ceil_div(batch * static_cast<int64_t>(sizeof(int2)), 256) * 256;
+    st = stream_workspace(s, static_cast<size_t>(cuts + slots * rows * (a.dim + 2) * 4), &ws,
+                          kWsLayer);
     if (st != HXM_OK) return st;
-    a.parts = static_cast<float*>(ws);
+    a.cuts = static_cast<int2*>(ws);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + cuts);
   }
   return dtype == HXM_F16 ? launch_tree_dim<_Float16>(a, s) : launch_tree_dim<__bf16>(a, s);
 }
