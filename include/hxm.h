@@ -644,9 +644,10 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * window.  q, out: row b * nodes + i.  lse (fp32 [batch, nodes, q_heads], or
  * NULL) as in hxm_paged_attention, which one node per sequence equals.  A
  * padded node, and a sequence without tokens (n <= 0), give zeros, and -inf in
- * lse.  What the cache holds where a node does not look (NaN included) never
- * reaches it, nor do table entries past a sequence's last page.  NaN are: the
- * outputs of a node whose parent (or one above) is padding or no node before
+ * lse, whatever else holds of them.  What the cache holds where a node does not
+ * look (NaN included) never reaches it, nor do table entries past a sequence's
+ * last page.  NaN are, else: the outputs of a node whose parent (or one above) is
+ * padding or no node before
  * it; of nodes that see a token of a page outside [0, pages); of a sequence of 0 <
  * n < nodes tokens, or of more than table_pages * page_size or 2^30.  dtype F16
  * or BF16, one for q, cache and out; scores, maxima and sums are fp32, the
