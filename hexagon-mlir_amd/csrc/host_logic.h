@@ -250,6 +250,26 @@ inline int64_t attn_grid(int64_t batch, int64_t heads, int64_t capacity,
   const int64_t a = even < g ? even : g, b = fine < f ? fine : f;
   return a > b ? a : b;
 }
+// Tokens that a sequence of up to `capacity`, of which the last `window` are read (0: all),
+// has from its first tile on.
+inline int64_t attn_span(int64_t capacity, int64_t window) {
+  const int64_t most = window + kAttnTile - 1;
+  return window > 0 && most < capacity ? most : capacity;
+}
+// attn_grid() of a cut in small steps.  The longest, two shares, always serves up to 64
+// sequences of half as many pairs as workgroups: units * heads / (2 * share), which is up to
+// groups / 2, and one more of each pair.
+inline int64_t attn_step_grid(int64_t batch, int64_t heads, int64_t span, uint32_t groups) {
+  const int64_t bh = batch * heads;
+  if (batch > 64 || bh > groups / 2) return attn_grid(batch, heads, span, groups);
+  const int64_t even = bh * (ceil_div(span, kAttnUnit) / 2 + 1);
+  return even < groups ? even : groups;
+}
+// Partial results of the sequences in pieces, of all heads.
+inline int64_t attn_step_slots(int64_t batch, int64_t heads, int64_t span, uint32_t groups) {
+  const int64_t grid = attn_step_grid(batch, heads, span, groups), most = 2 * kAttnFine * groups;
+  return grid < most ? grid : most;
+}
 
 // One entry of the tuning-cache file: "op M N K bm bn bk waves_m waves_n
 // stages split_k reps".  Every field is read as 64-bit and range-checked

@@ -64,6 +64,7 @@ struct TreeArgs {
   int64_t q_ts, q_hs, o_ts, o_hs;
   int64_t kps, khs, kts, vps, vhs, vts;
   int64_t ld_table, capacity;  // tokens a table row holds
+  int64_t span;                // and those of them that a sequence can have read
   int2* cuts;  // [batch]: pieces of a sequence and the partial slots before them
   float* parts;
   uint32_t pages, page_size;
@@ -640,7 +641,7 @@ hxm_status launch_tree(const TreeArgs& a, hipStream_t stream) {
   const int rows = tile_rows(int64_t(a.nodes) * a.group);
   const int64_t pairs =
       a.whole ? int64_t(a.batch) * a.hkv
-              : ceil_div(attn_grid(a.batch, a.heads, a.capacity, tree_groups(DT)), a.tiles);
+              : ceil_div(attn_step_grid(a.batch, a.heads, a.span, tree_groups(DT)), a.tiles);
   const int64_t groups = ceil_div(pairs, 8) * 8 * a.tiles;
   const int per = 256 / (a.dim / 4), slices = static_cast<int>(ceil_div(rows, per));
   const int64_t joins = a.whole ? 0 : int64_t(a.batch) * a.heads * slices;
@@ -745,11 +746,10 @@ extern "C" hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* ou
   // How the sequences were cut, and the partial results of those in pieces.
   hipStream_t s = as_stream(stream);
   // Sequences of up to kAttnWhole units are one piece each.
-  a.whole = batch > kAttnCutBatch || a.capacity <= kAttnWhole * kAttnUnit;
+  a.span = attn_span(a.capacity, a.window);
+  a.whole = batch > kAttnCutBatch || a.span <= kAttnWhole * kAttnUnit;
   if (!a.whole) {
-    const uint32_t pieces = tree_groups(a.dim);
-    const int64_t slots = std::min(attn_grid(batch, a.heads, a.capacity, pieces),
-                                   int64_t(2 * kAttnFine * pieces));
+    const int64_t slots = attn_step_slots(batch, a.heads, a.span, tree_groups(a.dim));
     void* ws = nullptr;
     const int64_t cuts = ceil_div(batch * static_cast<int64_t>(sizeof(int2)), 256) * 256;
     st = stream_workspace(s, static_cast<size_t>(cuts + slots * rows * (a.dim + 2) * 4), &ws,
