@@ -30,10 +30,10 @@
 // inside the loop that branch cost every tile its registers (4 x 64 over 32768: 677 us spilled,
 // 361 without).
 //
-// The running maximum moves only when a score passes it by more than 2^8, as in the
-// attention of one token, and the probabilities enter the second product as two 16-bit
-// halves, the first cut off and not rounded (the rest is exact then, and its rounding leaves
-// 21 bits in f16, 15 in bf16).  One half alone took 170 us for 201 at 4 x 64 over 32768 and added as
+// The running maximum moves only when a score passes it by more than 2^8, and the
+// probabilities enter the second product as two 16-bit halves, each rounded (22 bits in f16, 16
+// in bf16; the first cut off instead leaves one fewer in the same time, 203 us at 4 x 64 over
+// 32768), both as in the attention of one token.  One half alone took 170 us there and added as
 // much to the error as the output's own rounding; elsewhere its time does not show.
 #include <algorithm>
 #include <type_traits>
@@ -88,15 +88,10 @@ struct Frag<_Float16> {
   static __device__ __forceinline__ v16f32 mfma(V a, V b, v16f32 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  // x towards zero; x keeps what that leaves.
+  // x rounded; x keeps what that leaves.
   static __device__ __forceinline__ V split(v8f32& x) {
-    V r;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const auto h = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
-      r[i] = static_cast<_Float16>(h[0]), r[i + 1] = static_cast<_Float16>(h[1]);
-      x[i] -= static_cast<float>(h[0]), x[i + 1] -= static_cast<float>(h[1]);
-    }
+    const V r = __builtin_convertvector(x, V);
+    x -= __builtin_convertvector(r, v8f32);
     return r;
   }
 };
@@ -109,16 +104,14 @@ struct Frag<__bf16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ V split(v8f32& x) {
-    v4u32_t r;
+    const V r = __builtin_convertvector(x, V);
+    const v4u32_t b = __builtin_bit_cast(v4u32_t, r);
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      const uint32_t a = __builtin_bit_cast(uint32_t, static_cast<float>(x[i])),
-                     b = __builtin_bit_cast(uint32_t, static_cast<float>(x[i + 1]));
-      r[i / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-      x[i] -= __builtin_bit_cast(float, a & 0xffff0000u);
-      x[i + 1] -= __builtin_bit_cast(float, b & 0xffff0000u);
+      x[i] -= __builtin_bit_cast(float, b[i / 2] << 16);
+      x[i + 1] -= __builtin_bit_cast(float, b[i / 2] & 0xffff0000u);
     }
-    return __builtin_bit_cast(V, r);
+    return r;
   }
 };
 

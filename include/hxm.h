@@ -651,9 +651,9 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * it; of nodes that see a token of a page outside [0, pages); of a sequence of 0 <
  * n < nodes tokens, or of more than table_pages * page_size or 2^30.  dtype F16
  * or BF16, one for q, cache and out; scores, maxima and sums are fp32, the
- * probabilities enter the product with V with 21 bits (f16; one below 2^-10 of
- * the largest to 2^-32 of that) or 15 (bf16), as two 16-bit halves (which make a
- * dim whose V is infinite infinite or NaN).  out must not overlap q; out and lse
+ * probabilities enter the product with V as two 16-bit halves: 22 bits (f16; one
+ * below 2^-10 of the largest to 2^-32 of that) or 16 (bf16), which make a dim
+ * whose V is infinite infinite or NaN.  out must not overlap q; out and lse
  * nothing else.  batch * cache->heads, times the tiles of 32, 64 or 128 that nodes
  * * q_heads / cache->heads rows make, up to 2^18.  Sequences are split over
  * workgroups (in batches of up to 256) and joined in a fixed order.  Where table_pages *
