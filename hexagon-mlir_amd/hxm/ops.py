@@ -16,8 +16,8 @@ from typing import Optional, Sequence
 import torch
 
 from ._lib import (B_KN, B_NK, BF16, F16, F32, I8, I32, IMAGE_GEMM, IMAGE_W8A16, NORM_LAYER,
-                   HEAD_NORM, HEADS, KV_CACHE, NORM_NONE, NORM_RMS, OP_W8A16, OP_W8A16_SWIGLU, ROW_NORM,
-                   W_NK, W_PACKED, GemmConfig, HxmError, check, lib)
+                   HEAD_NORM, HEADS, KV_CACHE, NORM_NONE, NORM_RMS, OP_W8A16, OP_W8A16_SWIGLU,
+                   ROW_NORM, W_NK, W_PACKED, GemmConfig, HxmError, check, lib)
 
 _DT = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32,
        torch.int8: I8, torch.int32: I32}
@@ -758,21 +758,16 @@ def _kv_cache(k: torch.Tensor, v: torch.Tensor):
     """The hxm_kv_cache of [pages, heads, page_size, dim] tensors of any strides
     (a cache that keeps tokens before heads is passed transposed), its heads
     and dim, dtype and device."""
-    if k.dim() != 4:
-        raise ValueError(f"k_cache must be [pages, heads, page_size, dim] (got {tuple(k.shape)})")
-    return _kv_pack(k, v, k.shape, k.stride(), v.stride())
-
-
-def _kv_pack(k: torch.Tensor, v: torch.Tensor, shape, k_strides, v_strides):
-    """_kv_cache() of a layer of this shape and these strides at the start of k and v."""
     dev = _on_current(k, "k_cache")
-    dtype = k.dtype
+    dtype, shape = k.dtype, k.shape
+    if len(shape) != 4:
+        raise ValueError(f"k_cache must be [pages, heads, page_size, dim] (got {tuple(shape)})")
     if dtype not in _HALVES:
         raise TypeError(f"k_cache must be {' or '.join(str(d) for d in _HALVES)} (got {dtype})")
-    _tensor(v, dtype, k.shape, dev, "v_cache")
+    _tensor(v, dtype, shape, dev, "v_cache")
     pages, heads, page, dim = shape
-    kp, kh, kt, ki = k_strides
-    vp, vh, vt, vi = v_strides
+    kp, kh, kt, ki = k.stride()
+    vp, vh, vt, vi = v.stride()
     if ki != 1 or vi != 1:
         raise ValueError("k_cache and v_cache must have a contiguous last dimension")
     return (KV_CACHE.pack(k.data_ptr(), v.data_ptr(), pages, page, heads, dim, kp, kh, kt, vp, vh,
@@ -893,8 +888,6 @@ def norm_rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor
                    interleaved, q_out, (norm, eps, q_weight, q_bias, k_weight, k_bias))
 
 
-
-
 def _block_table(t: torch.Tensor, batch: int, dev: int):
     """(address, row stride, columns) of an int32 [batch, table_pages] table."""
     _mat(t, "block_table")
@@ -934,8 +927,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if return_lse:
         lse = torch.empty(B, hq, dtype=torch.float32, device=q.device)
         lse_p = lse.data_ptr()
-    st = lib.hxm_paged_attention(qh, oh, hq, cache, table_p, ld_table, table_pages, lens_p, B, dim ** -0.5 if scale is None else scale,
-                                 window, lse_p, _DT[dtype], _current_stream(dev))
+    st = lib.hxm_paged_attention(qh, oh, hq, cache, table_p, ld_table, table_pages, lens_p, B,
+                                 dim ** -0.5 if scale is None else scale, window, lse_p,
+                                 _DT[dtype], _current_stream(dev))
     if st:
         check(st, "hxm_paged_attention")
     return (out, lse) if return_lse else out
@@ -1045,12 +1039,21 @@ def _kv_layers(k: torch.Tensor, v: torch.Tensor):
     if k.dim() == 4:
         cache, _, _, dtype, dev = _kv_cache(k, v)
         return cache, 1, 0, 0, dtype, dev
-    if k.dim() != 5 or v.shape != k.shape or not k.shape[0]:
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 5 or v.shape != shape or not shape[0]:
         raise ValueError("k_cache and v_cache must be [pages, heads, page_size, dim], or with a "
-                         f"dimension of layers before (got {tuple(k.shape)}, {tuple(v.shape)})")
-    ks, vs = k.stride(), v.stride()
-    cache, _, _, dtype, dev = _kv_pack(k, v, k.shape[1:], ks[1:], vs[1:])
-    return cache, k.shape[0], ks[0], vs[0], dtype, dev
+                         f"dimension of layers before (got {tuple(shape)}, {tuple(v.shape)})")
+    dev = _on_current(k, "k_cache")
+    if dtype not in _HALVES:
+        raise TypeError(f"k_cache must be {' or '.join(str(d) for d in _HALVES)} (got {dtype})")
+    _tensor(v, dtype, shape, dev, "v_cache")
+    layers, pages, heads, page, dim = shape
+    kl, kp, kh, kt, ki = k.stride()
+    vl, vp, vh, vt, vi = v.stride()
+    if ki != 1 or vi != 1:
+        raise ValueError("k_cache and v_cache must have a contiguous last dimension")
+    return (KV_CACHE.pack(k.data_ptr(), v.data_ptr(), pages, page, heads, dim, kp, kh, kt, vp, vh,
+                          vt), layers, kl, vl, dtype, dev)
 
 
 @_on_stream
