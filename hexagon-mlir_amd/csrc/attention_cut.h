@@ -50,7 +50,10 @@ struct Piece {
 // the device, so the host cannot.  Batches of more than 64 take the fine pieces without
 // trying the others, which took 13 us instead of 15.4 for 256 x 600 tokens, one head, 12.3 for
 // 13.7 (128 x 600, two) and 149 for 152 (256 x 2048, eight), and 15 for 11.6 where few tokens
-// are many sequences' (65 x 1024, one head) and 30 for 25 (200 x 2048, one).
+// are many sequences' (65 x 1024, one head) and 30 for 25 (200 x 2048, one).  Trees of 8, heads
+// of 128, in small steps past 64 sequences too: 65 x 2048 39.5 us for 32.0 with the steps (one
+// head of 8), 38.1 for 36.6 (two of 4), 132 for 137 (eight of 4); 256 x 2048 67 for 64, 118 for
+// 111, 397 for 411; one of 16384 among 65 of 200 tokens 39.9 for 40.3, 31.5 for 39.9, 42 for 48.
 template <uint32_t GROUPS = kAttnGroups, bool STEPS = false, typename Args>
 __device__ __forceinline__ Piece find_piece(const Args& a, uint32_t u, int lane) {
   auto tokens = [&](int32_t len, int* lo) {
@@ -106,7 +109,8 @@ __device__ __forceinline__ Piece find_piece(const Args& a, uint32_t u, int lane)
       const int l = __builtin_ctzll(hit);
       const int32_t len_l = static_cast<int32_t>(lane_u32(static_cast<uint32_t>(len[i]), l));
       const uint32_t pieces = lane_u32(c, l);
-      const int step = static_cast<int>((lane_u32(w[i], l) + pieces - 1) / pieces) * static_cast<int>(kAttnUnit);
+      const int step = static_cast<int>((lane_u32(w[i], l) + pieces - 1) / pieces) *
+                       static_cast<int>(kAttnUnit);
       r.b = 64 * i + l;
       r.n = tokens(len_l, &r.lo);
       r.over = len_l > a.capacity;

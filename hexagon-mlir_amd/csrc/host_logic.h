@@ -193,8 +193,8 @@ inline FastDiv fast_div(uint32_t d) {
 }
 
 // How paged attention cuts a batch into pieces, one for a workgroup (kAttnGroups of them where
-// the sequences allow it; an attention that runs several workgroups a CU says how many).  Lengths count in
-// units of kAttnUnit tokens (of the window, from its first tile on; no sequence is 0).  A
+// the sequences allow it; an attention that runs several workgroups a CU says how many).
+// Lengths count in units of kAttnUnit tokens (of the window, from its first tile on; no sequence is 0).  A
 // sequence of up to kAttnWhole units is one piece.  Longer ones are cut into equal pieces
 // of at most `size` units: with share = all units / kAttnGroups, the least of
 // attn_size(share, 0 .. 3) that gives no more than kAttnGroups pieces over all heads; where
@@ -237,7 +237,9 @@ constexpr uint32_t attn_cut(uint32_t w, uint32_t size) {
 }
 // Larger batches are not cut, a sequence is a piece: every workgroup goes over all lengths
 // to find its own (512 sequences of 64 tokens, 8 heads: 34 us whole, 57 cut; 250, one of
-// 16384 tokens and the others of 200, 2 heads: 157 us whole, 23 cut).
+// 16384 tokens and the others of 200, 2 heads: 157 us whole, 23 cut; trees of 8, heads of 128,
+// 257 of 600 tokens, eight of 4 146 whole, 156 cut, of 2048 409 and 416; 512 of 2048, one head of
+// 8 118 and 140; one of 16384 among 257 of 200 390 and 43, eight of 4 265 and 97).
 constexpr int64_t kAttnCutBatch = 256;
 // Workgroups that hold the pieces of any lengths, of at most `capacity` tokens.
 inline int64_t attn_grid(int64_t batch, int64_t heads, int64_t capacity,

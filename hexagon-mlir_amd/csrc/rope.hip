@@ -406,8 +406,9 @@ hxm_status check_kv_cache(const char* op, const hxm_kv_cache* c, bool written) {
 
 // The arguments of an append checked, and as the kernels take them.
 static hxm_status rope_args(const char* op, const hxm_heads* q, const hxm_heads* q_out,
-                            int64_t q_heads, const hxm_heads* k, const hxm_heads* v, const int32_t* positions,
-                            const float* cos_sin, int64_t ld_cos_sin, int64_t max_pos,
+                            int64_t q_heads, const hxm_heads* k, const hxm_heads* v,
+                            const int32_t* positions, const float* cos_sin, int64_t ld_cos_sin,
+                            int64_t max_pos,
                             int64_t rot_dim, int32_t interleaved, const int32_t* slots,
                             const hxm_kv_cache* cache, int64_t tokens, int32_t dtype,
                             RopeArgs& a) {
@@ -532,7 +533,9 @@ extern "C" hxm_status hxm_norm_rope_append(const hxm_heads* q, const hxm_heads* 
   while (a.lanes < a.chunks) a.lanes *= 2;
   // Threads of a token: as rope_append, and one wave where the tokens fill the chip that way
   // (32 + 8 heads of 128: 8192 tokens 39.9 us with 64, 45.7 with 128, 60 with 256; 4096 19.4,
-  // 20.4, 24.9; 2048 12.9, 11.7, 14.6; 1024 12.1, 9.5, 9.0; 64 8.7, 6.4, 5.3).
+  // 20.4, 24.9; 2048 12.9, 11.7, 14.6; 1024 12.1, 9.5, 9.0; 64 8.7, 6.4, 5.3; 64 + 8 of 128: 8192
+  // 61, 65, 79, 2048 19.4, 17.1, 19.1, 64 12.9, 8.7, 6.5; 16 + 16 of 256: 76, 77, 81, 20.6, 19.3,
+  // 19.4, 13.0, 8.2, 5.8; 8 + 8 of 64: 13.0 each, 5.9, 4.4).
   a.tt = 64;
   const int most = tokens >= 4096 ? 64 : tokens >= 2048 ? 128 : 256;
   while (a.tt < most && a.tt < a.lanes * (a.hq + a.hkv)) a.tt *= 2;

@@ -4,9 +4,11 @@
 // MFMAs, so that one read of the keys and values serves up to 128 rows: 4 * dim bytes a
 // token against 4 * dim * rows operations.  Few rows are bound by memory, many by the matrix
 // cores and the exponentials beside them: 4 sequences to 32768 tokens, 64 nodes, 8 x 4 heads of
-// 128, 109 GFLOP in 201 us (545 TFLOP/s; with the second half of the probabilities, below,
-// 815 on the matrix cores, 43% of their cycles); 16 sequences to 4096, 16 nodes, 45 us, 3.0
-// TB/s, of which the join takes 6 and a workgroup's start and end 9.
+// 128, 109 GFLOP in 202 to 207 us (538 TFLOP/s at 203; with the second half of the
+// probabilities, below, 807 on the matrix cores, 44% of their cycles); 16 sequences to 4096, 16
+// nodes, 44.5 us, 3.0 TB/s, of which the join takes 6 and a workgroup's start and end 9.  Heads
+// of 256 keep one wave a SIMD, and up to 32 rows spill 47 registers: 16 x 16 to 4096, 4 x 2 heads
+// 66 us, 4 x 4 (64 rows) 56; 4 x 64 to 32768, 4 x 4 heads 188.
 //
 // A workgroup has four waves of 32 rows.  Up to 32 rows, its waves take tokens in turn, each
 // with tiles of its own; up to 64 rows two by two; more, all four share a tile of 64 tokens,
@@ -679,8 +681,8 @@ extern "C" hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* ou
                                          int64_t batch, int64_t nodes, float scale, int64_t window,
                                          float* lse, int32_t dtype, void* stream) {
   if (dtype != HXM_F16 && dtype != HXM_BF16)
-    return fail(HXM_UNSUPPORTED_DTYPE, "unsupported-dtype: tree_attention takes f16 or bf16 (got %d)",
-                dtype);
+    return fail(HXM_UNSUPPORTED_DTYPE,
+                "unsupported-dtype: tree_attention takes f16 or bf16 (got %d)", dtype);
   hxm_status st = check_kv_cache("tree_attention", cache, false);
   if (st != HXM_OK) return st;
   if (batch < 0 || nodes < 1 || q_heads < 1 || q_heads % cache->heads != 0 || window < 0)

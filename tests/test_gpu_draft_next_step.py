@@ -15,7 +15,8 @@ NEAR = dict(rtol=5e-2, atol=1e-2)
 def test_the_next_step_is_the_kept_tokens_one_at_a_time(dev):
     g = torch.Generator().manual_seed(17)
     ctx, T, B = [5, 14, 9], 9, 3
-    rows = [[-1, 0, 0, 0, 3, 2, 4, 4, 7], [-1, 0, 1, 0, 3, 4, 4, 6, 6], [-1, 0, 0, 1, 2, 4, -2, -2, -2]]
+    rows = [[-1, 0, 0, 0, 3, 2, 4, 4, 7], [-1, 0, 1, 0, 3, 4, 4, 6, 6],
+            [-1, 0, 0, 1, 2, 4, -2, -2, -2]]
     kept = [[0, 3, 4, 7, 8], [0, 3, 4, 6], [0, 2, 4, 5]]       # none of them where it has to go
     order = torch.randperm(12, generator=g).int()
     table = torch.stack([order[:4], order[4:8], order[8:12]])
@@ -28,7 +29,8 @@ def test_the_next_step_is_the_kept_tokens_one_at_a_time(dev):
             depth[b][i] = depth[b][row[i]] + 1 if row[i] >= 0 else 0
     tokens = torch.randperm(V, generator=g)[:B * T].view(B, T).int()
     at = lambda b, t: slot(table, b, t)                                          # noqa: E731
-    p = model.run(tokens.to(dev), i32([[ctx[b] + depth[b][i] for i in range(T)] for b in range(B)], dev),
+    p = model.run(tokens.to(dev),
+                  i32([[ctx[b] + depth[b][i] for i in range(T)] for b in range(B)], dev),
                   i32([[at(b, ctx[b] + i) if rows[b][i] > -2 else -1 for i in range(T)]
                        for b in range(B)], dev),
                   table.to(dev), i32([n + T for n in ctx], dev), i32(rows, dev))
@@ -38,8 +40,8 @@ def test_the_next_step_is_the_kept_tokens_one_at_a_time(dev):
         for i, j in zip(path, path[1:]):
             sure[b, i, tokens[b, j]] = 1
         sure[b, path[-1]] = p[b, path[-1]]
-    path, counts, following = ops.verify_draft(tokens.to(dev), sure,
-                                               torch.rand(B, T, generator=g).to(dev), i32(rows, dev))
+    u = torch.rand(B, T, generator=g).to(dev)
+    path, counts, following = ops.verify_draft(tokens.to(dev), sure, u, i32(rows, dev))
     assert path.tolist() == [k + [-1] * (T - len(k)) for k in kept]
     lens = i32([n + T for n in ctx], dev)
     drafted = model.k.clone(), model.v.clone()
@@ -58,7 +60,8 @@ def test_the_next_step_is_the_kept_tokens_one_at_a_time(dev):
                          i32([[at(b, int(new[b]))] for b in range(B)], dev), table.to(dev), new + 1)
 
     def tree_more():
-        return model.run(tokens2.to(dev), i32([[int(new[b]) + d for d in depth2] for b in range(B)], dev),
+        return model.run(tokens2.to(dev),
+                         i32([[int(new[b]) + d for d in depth2] for b in range(B)], dev),
                          i32([[at(b, int(new[b]) + i) for i in range(6)] for b in range(B)], dev),
                          table.to(dev), new + 6, i32(rows2, dev))
 

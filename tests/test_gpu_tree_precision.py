@@ -53,4 +53,5 @@ def test_bits_of_a_probability(dev, name, s, group):
     noise = (3 * 2.0 ** -24 + (2.0 ** -22 if name == "f16" else 0)) * math.log(2.0) + 2 * 2.0 ** -23
     tol = 2.0 ** -(2 * s + 2) + noise + 2.0 ** -s * got.abs()
     bad = ~((got - left).abs() <= tol)
-    assert not bad.any(), (int(bad[:, 0, 0].sum()), float((got - left).abs().max() * 2 ** (2 * s + 2)))
+    worst = float((got - left).abs().max() * 2 ** (2 * s + 2))
+    assert not bad.any(), (int(bad[:, 0, 0].sum()), worst)
