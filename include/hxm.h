@@ -656,11 +656,12 @@ hxm_status hxm_paged_attention(const hxm_heads* q, const hxm_heads* out, int64_t
  * whose V is infinite infinite or NaN.  out must not overlap q; out and lse
  * nothing else.  batch * cache->heads, times the tiles of 32, 64 or 128 that nodes
  * * q_heads / cache->heads rows make, up to 2^18.  Sequences are split over
- * workgroups (in batches of up to 256) and joined in a fixed order.  Where table_pages *
- * page_size is over 512 (with a window: window + nodes + 30 too) and batch up to 256 it uses the
- * per-stream workspace: tile * (dim + 2) * 4 bytes for each piece, up to 512 of them (256 past
- * dim 128) with up to 64 sequences and batch * heads * tiles up to half of that, up to 3072
- * (1536) else: 34 MB of tiles of 128 at dim 128, and 204 MB. */
+ * workgroups (in batches of up to 256) and joined in a fixed order.  Where
+ * table_pages * page_size is over 512 (with a window: window + nodes + 30 too) and
+ * batch up to 256 it uses the per-stream workspace: tile * (dim + 2) * 4 bytes for
+ * each piece, up to 512 of them (256 past dim 128) with up to 64 sequences and
+ * batch * heads * tiles up to half of that, up to six times as many else: 34 MB with
+ * tiles of 128 rows at dim 128, and 204 MB. */
 hxm_status hxm_tree_attention(const hxm_heads* q, const hxm_heads* out, int64_t q_heads,
                               const hxm_kv_cache* cache, const int32_t* block_table,
                               int64_t ld_table, int64_t table_pages, const int32_t* seq_lens,
